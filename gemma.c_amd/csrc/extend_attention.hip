@@ -1,0 +1,472 @@
+// Attention of a ragged batch of new tokens over the paged cache, gfx950: the
+// plan that shares the work out, the merge of split row blocks and the entry
+// points. No counterpart in the reference.
+#include "extend_common.hpp"
+
+#include <math.h>
+
+#include <algorithm>
+
+namespace gemma4 {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / kWave;
+
+struct PlanParams {
+  char *plan;
+  int32_t share_first, segments, merges;
+  const int32_t *row_offsets;
+  const int32_t *prior_lengths;
+  ExtendGeometry g;
+  int32_t batch, total_rows, window, sinks, heads, page_size;
+  int32_t max_prior;
+};
+
+struct Sum {
+  template <class T> __device__ T operator()(T a, T b) const { return a + b; }
+};
+struct Max {
+  template <class T> __device__ T operator()(T a, T b) const { return a > b ? a : b; }
+};
+// Inclusive prefix of one value per thread over the workgroup; the last
+// thread's in `total`.
+template <class T, class F>
+__device__ __forceinline__ T block_prefix(T x, T &total, T *waves, F f) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const T other = __shfl_up(x, d);
+    if (lane >= d) x = f(other, x);
+  }
+  if (lane == kWave - 1) waves[wave] = x;
+  __syncthreads();
+  T head = waves[0], all = waves[0];
+#pragma unroll
+  for (int w = 1; w < kPlanWaves; ++w) {
+    if (w < wave) head = f(head, waves[w]);
+    all = f(all, waves[w]);
+  }
+  total = all;
+  __syncthreads();
+  return wave > 0 ? f(head, x) : x;
+}
+
+constexpr int kBlockCost = 1;  // of a row block besides its tiles: queries, end of the rows
+constexpr int kShareCost = 2;  // least cost worth a workgroup
+
+// One workgroup. The row blocks laid end to end, each at the cost of its tiles
+// and kBlockCost, are cut into shares of equal cost. A cut near a block's end moves
+// there: a split block costs its partial sums, written, read and merged (64 rows
+// about four tiles' time, few rows less).
+__global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p) {
+  __shared__ int32_t s_begin[kExtendBatch + 1];   // first row of a sequence
+  __shared__ int32_t s_blocks[kExtendBatch + 1];  // row blocks before it
+  __shared__ int64_t s_waves[kPlanWaves];
+  __shared__ int32_t s_waves32[kPlanWaves];
+  const int t = threadIdx.x;
+  auto *share_first = reinterpret_cast<int32_t *>(p.plan + p.share_first);
+  auto *segments = reinterpret_cast<ExtendSegment *>(p.plan + p.segments);
+  auto *merges = reinterpret_cast<ExtendMerge *>(p.plan + p.merges);
+
+  // Offsets within the batch and, by a running maximum, ascending: whatever they
+  // say, no row belongs to two sequences and the sections above hold the plan.
+  int32_t reach = 0;
+  for (int32_t b0 = 0; b0 <= p.batch; b0 += kPlanThreads) {
+    const int32_t b = b0 + t;
+    int32_t last;
+    const int32_t own = b <= p.batch ? min(max(p.row_offsets[b], 0), p.total_rows) : 0;
+    const int32_t top = max(block_prefix(own, last, s_waves32, Max()), reach);
+    if (b <= p.batch) s_begin[b] = top;
+    reach = max(reach, last);
+  }
+  __syncthreads();
+  int32_t n_blocks = 0;
+  for (int32_t b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+    const int32_t b = b0 + t;
+    int32_t all;
+    const int32_t own =
+        b < p.batch ? (s_begin[b + 1] - s_begin[b] + p.g.rows - 1) / p.g.rows : 0;
+    const int32_t sum = block_prefix(own, all, s_waves32, Sum());
+    if (b < p.batch) s_blocks[b] = n_blocks + sum - own;
+    n_blocks += all;
+  }
+  if (t == 0) s_blocks[p.batch] = n_blocks;
+  __syncthreads();
+
+  struct Block {
+    int32_t sequence, row0, rows, prior, tiles;
+    int64_t cost;
+  };
+  auto block_of = [&](int32_t j) {
+    Block r{0, 0, 0, 0, 0, 0};
+    if (j >= n_blocks) return r;
+    // The last sequence whose blocks begin at or before j.
+    int32_t lo = 0, hi = p.batch;
+    while (hi - lo > 1) {
+      const int32_t mid = (lo + hi) >> 1;
+      if (s_blocks[mid] <= j) lo = mid; else hi = mid;
+    }
+    r.sequence = lo;
+    r.row0 = (j - s_blocks[lo]) * p.g.rows;
+    r.rows = min(s_begin[lo + 1] - s_begin[lo] - r.row0, p.g.rows);
+    r.prior = min(max(p.prior_lengths[lo], 0), p.max_prior);
+    const int32_t first = r.prior + r.row0;
+    r.tiles = extend_tiles(first, first + r.rows - 1, p.window, p.sinks, p.g.tile).count;
+    r.cost = (int64_t)r.tiles + kBlockCost;
+    return r;
+  };
+  int64_t cost = 0;
+  for (int32_t j0 = 0; j0 < n_blocks; j0 += kPlanThreads) {
+    int64_t all;
+    block_prefix(block_of(j0 + t).cost, all, s_waves, Sum());
+    cost += all;
+  }
+  const int32_t shares =
+      (int32_t)min((int64_t)p.g.shares, max(cost / kShareCost, (int64_t)1));
+  // Cut k of 1 .. shares - 1 lies at this cost. Every thread evaluates the same
+  // expression, so the blocks agree on it.
+  const double step = (double)cost / (double)shares;
+  auto cut_at = [&](int32_t k) { return (int64_t)((double)k * step); };
+
+  int64_t before = 0;                        // cost of the blocks of earlier rounds
+  int64_t counts = 0;                        // their segments, partial and merged rows
+  for (int32_t j0 = 0; j0 < n_blocks; j0 += kPlanThreads) {
+    const Block r = block_of(j0 + t);
+    int64_t all;
+    const int64_t end = before + block_prefix(r.cost, all, s_waves, Sum());
+    const int64_t begin = end - r.cost;
+    before += all;
+    const int32_t snap = 1 + r.rows * 3 / p.g.rows;
+    // f(cut k, the tile it lies at: 0 and r.tiles are no cuts of the block)
+    auto for_cuts = [&](auto &&f) {
+      if (r.rows == 0) return;
+      int32_t k = max((int32_t)((double)begin / step), 1);
+      while (k > 1 && cut_at(k - 1) >= begin) --k;
+      while (k < shares && cut_at(k) < begin) ++k;
+      for (; k < shares && cut_at(k) < end; ++k) {
+        int32_t tile = (int32_t)max(cut_at(k) - begin - kBlockCost, (int64_t)0);
+        if (tile < snap) tile = 0;
+        if (r.tiles - tile < snap) tile = r.tiles;
+        f(k, tile);
+      }
+    };
+    int32_t parts = r.rows > 0 ? 1 : 0, last = 0;
+    for_cuts([&](int32_t, int32_t tile) {
+      if (tile > last && tile < r.tiles) {
+        ++parts;
+        last = tile;
+      }
+    });
+    // Three counts in one word: partial rows stay below 2^16, merged ones too.
+    const int64_t own = (int64_t)parts << 32 |
+                        (parts > 1 ? (int64_t)(parts * r.rows) << 16 | r.rows : (int64_t)0);
+    int64_t sums;
+    const int64_t at = counts + block_prefix(own, sums, s_waves, Sum()) - own;
+    counts += sums;
+    const int32_t segment = (int32_t)(at >> 32);
+    const int32_t partial = (int32_t)(at >> 16) & 0xFFFF, merge = (int32_t)at & 0xFFFF;
+    int32_t part = 0;
+    last = 0;
+    auto emit = [&](int32_t lo, int32_t hi) {
+      segments[segment + part] = {r.row0, r.rows, s_begin[r.sequence], r.prior, r.sequence, lo, hi,
+                                  parts > 1 ? partial + part * r.rows : -1};
+    };
+    for_cuts([&](int32_t k, int32_t tile) {
+      if (tile > last && tile < r.tiles) {
+        emit(last, tile);
+        ++part;
+        last = tile;
+      }
+      share_first[k] = segment + part + (tile >= r.tiles ? 1 : 0);
+    });
+    if (r.rows > 0) emit(last, r.tiles);
+    if (parts > 1) {
+      for (int32_t i = 0; i < r.rows; ++i)
+        merges[merge + i] = {s_begin[r.sequence] + r.row0 + i, partial + i, parts, r.rows};
+    }
+  }
+  const int32_t n_segments = (int32_t)(counts >> 32);
+  if (t == 0) share_first[0] = 0;
+  for (int32_t k = max(shares, 1) + t; k <= p.g.shares; k += kPlanThreads)
+    share_first[k] = n_segments;
+  if (t == 0) {
+    *reinterpret_cast<ExtendHeader *>(p.plan) = {
+        kExtendMagic, p.batch, p.total_rows, p.heads, p.window, p.sinks, p.page_size, n_segments,
+        (int32_t)counts & 0xFFFF};
+  }
+}
+
+// ---- the rows' attention --------------------------------------------------------
+// A wave per (row, query head), one key at a time.
+template <int kHeads, int kDim>
+__global__ __launch_bounds__(256) void extend_rows_kernel(ExtendParams p, ExtendGeometry g) {
+  if (!extend_plan_fits(p)) return;
+  constexpr int kGroup = kQueryHeads / kHeads, kPer = kDim / kWave;
+  const auto *h = reinterpret_cast<const ExtendHeader *>(p.plan);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int head = blockIdx.x % kHeads, share = blockIdx.x / kHeads;
+  const auto *share_first = reinterpret_cast<const int32_t *>(p.plan + p.share_first);
+  const auto *segments = reinterpret_cast<const ExtendSegment *>(p.plan + p.segments);
+  const int64_t layer = (int64_t)p.layer * p.c.num_pages * p.c.page_size;
+  for (int32_t i = share_first[share]; i < share_first[share + 1]; ++i) {
+    const ExtendSegment s = segments[i];
+    const int32_t first = s.prior + s.row0;
+    const ExtendTiles tiles =
+        extend_tiles(first, first + s.rows - 1, h->window, h->sinks, g.tile);
+    for (int32_t w = wave; w < s.rows * kGroup; w += 4) {
+      const int32_t r = w / kGroup, qh = head * kGroup + w % kGroup;
+      const int32_t at = first + r;
+      const int64_t row = s.base + s.row0 + r;
+      float q[kPer], o[kPer], m = -INFINITY, l = 0.0f;
+      for (int e = 0; e < kPer; ++e) {
+        q[e] = bf16_lo(p.q[row * p.q_stride + qh * kDim + lane + kWave * e]) * p.q_scale;
+        o[e] = 0.0f;
+      }
+      for (int32_t tile = s.tile_lo; tile < s.tile_hi; ++tile) {
+        const int32_t k0 =
+            (tile < tiles.sink_tiles ? tile : tile - tiles.sink_tiles + tiles.window_tile) * g.tile;
+        for (int32_t key = k0; key < k0 + g.tile && key <= at; ++key) {
+          if (h->window > 0 && key <= at - h->window && key >= h->sinks) continue;
+          const uint16_t *k, *v;
+          if (key >= s.prior) {
+            const int64_t from = (s.base + key - s.prior) * p.kv_stride + head * kDim;
+            k = p.k + from;
+            v = p.v + from;
+          } else {
+            const uint32_t logical = fast_div(key, p.page_div);
+            if (p.c.window_size == 0 && logical >= (uint32_t)p.c.max_pages_per_seq) continue;
+            const int32_t page = p.page_table[(int64_t)s.sequence * p.c.max_pages_per_seq +
+                                              fast_mod(logical, p.slot_div)];
+            if (page < 0 || page >= p.c.num_pages) continue;
+            const int64_t from = ((layer + (int64_t)page * p.c.page_size + key -
+                                   (int64_t)logical * p.c.page_size) * kHeads + head) * kDim;
+            k = p.cache_k + from;
+            v = p.cache_v + from;
+          }
+          float x = 0.0f;
+          for (int e = 0; e < kPer; ++e) x += q[e] * bf16_lo(k[lane + kWave * e]);
+          for (int d = 1; d < kWave; d <<= 1) x += __shfl_xor(x, d);
+          const float top = fmaxf(m, x), a = exp2f(m - top), w1 = exp2f(x - top);
+          l = l * a + w1;
+          for (int e = 0; e < kPer; ++e) o[e] = o[e] * a + w1 * bf16_lo(v[lane + kWave * e]);
+          m = top;
+        }
+      }
+      if (s.partial < 0) {
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        for (int e = 0; e < kPer; ++e)
+          p.out[(row * kQueryHeads + qh) * kDim + lane + kWave * e] =
+              (uint16_t)f32_to_bf16_bits(o[e] * inv);
+      } else {
+        const int64_t part = (int64_t)(s.partial + r) * kQueryHeads + qh;
+        for (int e = 0; e < kPer; ++e) p.partial[part * kDim + lane + kWave * e] = o[e];
+        if (lane == 0) {
+          p.stats[2 * part] = m;
+          p.stats[2 * part + 1] = l;
+        }
+      }
+    }
+  }
+}
+
+// ---- merge ----------------------------------------------------------------------
+// Workgroup (merged row, query head, 256 dims), four waves: lane l holds dims
+// 4 l .. + 3, the waves take the parts in turn.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeWaves = kMergeThreads / kWave;
+constexpr int kMergeGrid = 2048;
+template <int kDim>
+__global__ __launch_bounds__(kMergeThreads) void extend_merge_kernel(ExtendParams p) {
+  if (!extend_plan_fits(p)) return;
+  __shared__ float4 s_acc[kMergeWaves][kWave];
+  __shared__ float2 s_stats[kMergeWaves];
+  constexpr int kSlices = kDim / 256;
+  const auto *h = reinterpret_cast<const ExtendHeader *>(p.plan);
+  const auto *merges = reinterpret_cast<const ExtendMerge *>(p.plan + p.merges);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int32_t items = h->merges * kQueryHeads * kSlices;
+  for (int32_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const ExtendMerge r = merges[i / (kQueryHeads * kSlices)];
+    const int qh = i / kSlices % kQueryHeads, d0 = i % kSlices * 256 + 4 * lane;
+    float m = -INFINITY, l = 0.0f;
+    float4 acc = {0, 0, 0, 0};
+    for (int32_t part = wave; part < r.parts; part += kMergeWaves) {
+      const int64_t at = ((int64_t)r.partial + (int64_t)part * r.stride) * kQueryHeads + qh;
+      const float2 s = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
+      const float4 a = *reinterpret_cast<const float4 *>(p.partial + at * kDim + d0);
+      if (s.x == -INFINITY) continue;
+      const float top = fmaxf(m, s.x);
+      const float fa = __builtin_amdgcn_exp2f(m - top), fb = __builtin_amdgcn_exp2f(s.x - top);
+      l = l * fa + s.y * fb;
+      acc.x = acc.x * fa + a.x * fb;
+      acc.y = acc.y * fa + a.y * fb;
+      acc.z = acc.z * fa + a.z * fb;
+      acc.w = acc.w * fa + a.w * fb;
+      m = top;
+    }
+    s_acc[wave][lane] = acc;
+    if (lane == 0) s_stats[wave] = make_float2(m, l);
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < kMergeWaves; ++w) {
+        const float2 s = s_stats[w];
+        const float4 a = s_acc[w][lane];
+        if (s.x == -INFINITY) continue;
+        const float top = fmaxf(m, s.x);
+        const float fa = __builtin_amdgcn_exp2f(m - top), fb = __builtin_amdgcn_exp2f(s.x - top);
+        l = l * fa + s.y * fb;
+        acc.x = acc.x * fa + a.x * fb;
+        acc.y = acc.y * fa + a.y * fb;
+        acc.z = acc.z * fa + a.z * fb;
+        acc.w = acc.w * fa + a.w * fb;
+        m = top;
+      }
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      *reinterpret_cast<uint2 *>(p.out + ((int64_t)r.row * kQueryHeads + qh) * kDim + d0) =
+          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host -------------------------------------------------------------------------
+bool valid_extend(const Gemma4KvCacheConfig &c, int32_t batch, int32_t total_rows) {
+  const bool geometry =
+      (c.num_heads == 8 && c.head_dim == 256) || (c.num_heads == 1 && c.head_dim == 512);
+  return geometry && batch > 0 && batch <= kExtendBatch && batch <= c.batch_size &&
+         total_rows >= 0 && total_rows <= (1 << 24) && c.num_layers > 0 && c.num_pages > 0 &&
+         c.page_size > 0 && c.max_pages_per_seq > 0 && c.window_size >= 0 &&
+         (int64_t)c.num_pages * c.page_size <= 0x7fffffff;
+}
+bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace
+}  // namespace gemma4
+
+using namespace gemma4;
+
+extern "C" size_t gemma4_flash_attention_extend_plan_bytes(Gemma4KvCacheConfig config,
+                                                           int32_t batch_size,
+                                                           int32_t total_rows) {
+  if (!valid_extend(config, batch_size, total_rows)) return 0;
+  return (size_t)extend_layout(extend_geometry(config), batch_size, total_rows).bytes;
+}
+
+extern "C" size_t gemma4_flash_attention_extend_workspace_bytes(Gemma4KvCacheConfig config,
+                                                                int32_t batch_size,
+                                                                int32_t total_rows) {
+  if (!valid_extend(config, batch_size, total_rows)) return 0;
+  const ExtendPlanLayout l = extend_layout(extend_geometry(config), batch_size, total_rows);
+  return (size_t)(extend_stats_offset(l, config.head_dim) +
+                  extend_round(l.max_partials * kQueryHeads * 8));
+}
+
+extern "C" hipError_t gemma4_flash_attention_extend_plan(
+    void *d_plan, size_t plan_bytes, const int32_t *d_row_offsets, const int32_t *d_prior_lengths,
+    Gemma4KvCacheConfig config, int32_t batch_size, int32_t total_rows, int32_t window_size,
+    int32_t sink_tokens, hipStream_t stream) {
+  if (!valid_extend(config, batch_size, total_rows) || d_plan == nullptr || !aligned(d_plan, 256) ||
+      d_row_offsets == nullptr || d_prior_lengths == nullptr || window_size < 0 ||
+      sink_tokens < 0) {
+    return hipErrorInvalidValue;
+  }
+  const int64_t capacity = (int64_t)config.max_pages_per_seq * config.page_size;
+  if (config.window_size > 0 && (window_size < 1 || window_size > config.window_size ||
+                                 window_size > capacity || sink_tokens > 0)) {
+    return hipErrorInvalidValue;
+  }
+  const ExtendGeometry &g = extend_geometry(config);
+  const ExtendPlanLayout l = extend_layout(g, batch_size, total_rows);
+  if (plan_bytes < (size_t)l.bytes) return hipErrorInvalidValue;
+  PlanParams p{};
+  p.plan = static_cast<char *>(d_plan);
+  p.share_first = (int32_t)l.share_first;
+  p.segments = (int32_t)l.segments;
+  p.merges = (int32_t)l.merges;
+  p.row_offsets = d_row_offsets;
+  p.prior_lengths = d_prior_lengths;
+  p.g = g;
+  p.batch = batch_size;
+  p.total_rows = total_rows;
+  p.window = window_size;
+  p.sinks = sink_tokens;
+  p.heads = config.num_heads;
+  p.page_size = config.page_size;
+  // A full-length cache holds no key past its table; a ring's positions only have
+  // to stay below 2^31 with the new rows.
+  p.max_prior = (int32_t)std::min<int64_t>(config.window_size > 0 ? 0x7fffffff : capacity,
+                                           0x7fffffff - total_rows - 256);
+  hipLaunchKernelGGL(extend_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+extern "C" hipError_t gemma4_flash_attention_extend_paged_bf16(
+    gemma4_bf16 *d_out, const gemma4_bf16 *d_q, const gemma4_bf16 *d_k, const gemma4_bf16 *d_v,
+    const gemma4_bf16 *d_cache_k, const gemma4_bf16 *d_cache_v, const int32_t *d_page_table,
+    const void *d_plan, size_t plan_bytes, Gemma4KvCacheConfig config, int32_t layer,
+    int32_t batch_size, int32_t total_rows, int64_t q_stride, int64_t kv_stride,
+    float softmax_scale, void *d_workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (total_rows == 0) return hipSuccess;
+  if (!valid_extend(config, batch_size, total_rows) || d_out == nullptr || d_q == nullptr ||
+      d_k == nullptr || d_v == nullptr || d_cache_k == nullptr || d_cache_v == nullptr ||
+      d_page_table == nullptr || d_plan == nullptr || d_workspace == nullptr || layer < 0 ||
+      layer >= config.num_layers || !(softmax_scale > 0.0f) || !isfinite(softmax_scale)) {
+    return hipErrorInvalidValue;
+  }
+  const int64_t q_width = (int64_t)kQueryHeads * config.head_dim;
+  const int64_t kv_width = (int64_t)config.num_heads * config.head_dim;
+  if (q_stride == 0) q_stride = q_width;
+  if (kv_stride == 0) kv_stride = kv_width;
+  const int64_t most = (int64_t)1 << 31;
+  if (q_stride < q_width || kv_stride < kv_width || q_stride % kPackElems != 0 ||
+      kv_stride % kPackElems != 0 || q_stride > most || kv_stride > most || !aligned(d_out, 16) ||
+      !aligned(d_q, 16) || !aligned(d_k, 16) || !aligned(d_v, 16) || !aligned(d_cache_k, 16) ||
+      !aligned(d_cache_v, 16) || !aligned(d_plan, 256) || !aligned(d_workspace, 256)) {
+    return hipErrorInvalidValue;
+  }
+  const ExtendGeometry &g = extend_geometry(config);
+  const ExtendPlanLayout l = extend_layout(g, batch_size, total_rows);
+  if (plan_bytes < (size_t)l.bytes ||
+      workspace_bytes <
+          gemma4_flash_attention_extend_workspace_bytes(config, batch_size, total_rows)) {
+    return hipErrorInvalidValue;
+  }
+  ExtendParams p{};
+  p.out = reinterpret_cast<uint16_t *>(d_out);
+  p.q = reinterpret_cast<const uint16_t *>(d_q);
+  p.k = reinterpret_cast<const uint16_t *>(d_k);
+  p.v = reinterpret_cast<const uint16_t *>(d_v);
+  p.cache_k = reinterpret_cast<const uint16_t *>(d_cache_k);
+  p.cache_v = reinterpret_cast<const uint16_t *>(d_cache_v);
+  p.page_table = d_page_table;
+  p.plan = static_cast<const char *>(d_plan);
+  p.share_first = (int32_t)l.share_first;
+  p.segments = (int32_t)l.segments;
+  p.merges = (int32_t)l.merges;
+  p.c = config;
+  p.page_div = make_fast_div(config.page_size);
+  p.slot_div = make_fast_div(config.max_pages_per_seq);
+  p.layer = layer;
+  p.batch = batch_size;
+  p.total_rows = total_rows;
+  p.q_stride = q_stride;
+  p.kv_stride = kv_stride;
+  p.q_scale = softmax_scale * kLog2e;
+  p.partial = static_cast<float *>(d_workspace);
+  p.stats = reinterpret_cast<float *>(static_cast<char *>(d_workspace) +
+                                      extend_stats_offset(l, config.head_dim));
+  const uint32_t merge_grid = (uint32_t)std::min<int64_t>(
+      kMergeGrid, std::max<int64_t>(l.max_merges, 1) * kQueryHeads * (config.head_dim / 256));
+  if (config.num_heads == 1) {
+    hipLaunchKernelGGL((extend_rows_kernel<1, 512>), dim3(g.shares), dim3(256), 0, stream, p, g);
+    hipLaunchKernelGGL(extend_merge_kernel<512>, dim3(merge_grid), dim3(kMergeThreads), 0, stream,
+                       p);
+  } else {
+    hipLaunchKernelGGL((extend_rows_kernel<8, 256>), dim3(8 * g.shares), dim3(256), 0, stream, p,
+                       g);
+    hipLaunchKernelGGL(extend_merge_kernel<256>, dim3(merge_grid), dim3(kMergeThreads), 0, stream,
+                       p);
+  }
+  return hipGetLastError();
+}

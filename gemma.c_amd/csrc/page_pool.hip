@@ -1,0 +1,684 @@
+// Pages of a pool: taking and returning them, branches of sequences (fork) and
+// the closing up of kept tokens (compact), gfx950. No counterpart in the
+// reference, whose page tables map a fixed page to every slot
+// (src/gemma4_kv_cache.cu:108-122).
+//
+// State, all on the device: a page table [batch_size][max_pages_per_seq] (-1:
+// unmapped) and refs[num_pages], the number of table entries that map a page (0:
+// free). Free pages are given out lowest first, in table order, so the result does
+// not depend on scheduling; a call that cannot be served whole changes nothing.
+#include "gemma4_device.hpp"
+#include "fast_div.hpp"
+
+#include <algorithm>
+
+namespace gemma4 {
+namespace {
+
+constexpr int kPoolThreads = 1024;
+constexpr int kPoolWaves = kPoolThreads / kWave;
+constexpr int kPoolUnroll = 4;                            // items per thread and round
+constexpr int kPoolRound = kPoolThreads * kPoolUnroll;    // items per round
+constexpr int kPoolBatch = 4096;                          // sequences at most
+constexpr int kPoolList = 16384;                          // free pages held in LDS at a time
+
+constexpr int kStatusOk = 0, kStatusPages = 1, kStatusArguments = 2;
+
+struct PoolParams {
+  int32_t *page_table;
+  int32_t *refs;
+  Gemma4KvCacheConfig c;
+  FastDiv page_div, slot_div;
+};
+
+// Logical pages [lo, hi) of one sequence as table slots: `count` of them from
+// slot `first` on, around the ring's end (a full-length cache never wraps).
+struct SlotRange {
+  int32_t first, count;
+  bool ok;
+};
+__device__ __forceinline__ SlotRange slot_range(const PoolParams &p, int32_t lo, int32_t hi) {
+  const int32_t pages = p.c.max_pages_per_seq;
+  SlotRange r{0, 0, true};
+  if (hi <= lo) return r;
+  if (p.c.window_size == 0) {
+    r.ok = hi <= pages;
+    r.first = min(lo, pages);
+    r.count = min(hi, pages) - r.first;
+  } else {
+    r.first = (int32_t)fast_mod((uint32_t)lo, p.slot_div);
+    r.count = min(hi - lo, pages);
+  }
+  return r;
+}
+
+// ---- release --------------------------------------------------------------
+// One thread per table entry; what is read and written is a few kilobytes and
+// the launch is its time.
+__global__ __launch_bounds__(256) void release_pages_kernel(
+    PoolParams p, const int32_t *__restrict__ first_position,
+    const int32_t *__restrict__ end_position, int64_t entries) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= entries) return;
+  const int32_t pages = p.c.max_pages_per_seq;
+  const int32_t b = (int32_t)fast_div((uint32_t)i, p.slot_div);
+  const int32_t slot = (int32_t)i - b * pages;
+  const int32_t physical = p.page_table[i];
+  const int32_t first = max(first_position[b], 0), end = max(end_position[b], 0);
+  // Whole pages only: first rounded up, end down.
+  int32_t lo = (int32_t)fast_div((uint32_t)first, p.page_div);
+  if (lo * p.c.page_size != first) ++lo;
+  const SlotRange r = slot_range(p, lo, (int32_t)fast_div((uint32_t)end, p.page_div));
+  int32_t d = slot - r.first;
+  if (d < 0) d += pages;
+  if (d >= r.count || physical < 0) return;
+  p.page_table[i] = -1;
+  if (physical >= p.c.num_pages) return;
+  // A count that is zero already stays zero.
+  if (atomicSub(&p.refs[physical], 1) <= 0) atomicAdd(&p.refs[physical], 1);
+}
+
+// ---- ordered ranks over one workgroup ----------------------------------------
+// Ranks of the true flags of one round in the order (u, thread): item u of
+// thread t comes at u * kPoolThreads + t, so loads of a round are coalesced.
+struct RankScratch {
+  int32_t counts[kPoolUnroll * kPoolWaves];
+};
+__device__ __forceinline__ int32_t round_ranks(const bool (&flag)[kPoolUnroll],
+                                               int32_t (&rank)[kPoolUnroll], RankScratch &s) {
+  static_assert(kPoolUnroll * kPoolWaves == kWave, "one lane per (u, wave) count");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t votes[kPoolUnroll];
+#pragma unroll
+  for (int u = 0; u < kPoolUnroll; ++u) votes[u] = __ballot(flag[u]);
+  if (lane == 0) {
+#pragma unroll
+    for (int u = 0; u < kPoolUnroll; ++u) s.counts[u * kPoolWaves + wave] = __popcll(votes[u]);
+  }
+  __syncthreads();
+  const int32_t own = s.counts[lane];
+  int32_t sum = own;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int32_t other = __shfl_up(sum, d);
+    if (lane >= d) sum += other;
+  }
+  const int32_t total = __shfl(sum, kWave - 1);
+#pragma unroll
+  for (int u = 0; u < kPoolUnroll; ++u) {
+    rank[u] = __shfl(sum - own, u * kPoolWaves + wave) +
+              __popcll(votes[u] & ((1ull << lane) - 1));
+  }
+  __syncthreads();  // the counts may be written again
+  return total;
+}
+
+// Free pages with ranks [from, from + kPoolList) into `list`, in page order.
+// Looks no further than to the one with rank wanted - 1; returns how many free
+// pages it has seen.
+__device__ __forceinline__ int32_t find_free(const PoolParams &p, int32_t from, int32_t wanted,
+                                             int32_t *list, RankScratch &scratch) {
+  int32_t seen = 0;
+  for (int32_t base = 0; base < p.c.num_pages && seen < wanted; base += kPoolRound) {
+    bool flag[kPoolUnroll];
+    int32_t rank[kPoolUnroll];
+#pragma unroll
+    for (int u = 0; u < kPoolUnroll; ++u) {
+      const int32_t page = base + u * kPoolThreads + (int32_t)threadIdx.x;
+      flag[u] = page < p.c.num_pages && p.refs[page] <= 0;
+    }
+    const int32_t found = round_ranks(flag, rank, scratch);
+#pragma unroll
+    for (int u = 0; u < kPoolUnroll; ++u) {
+      const int32_t at = seen + rank[u] - from;
+      if (flag[u] && at >= 0 && at < kPoolList)
+        list[at] = base + u * kPoolThreads + (int32_t)threadIdx.x;
+    }
+    seen += found;
+  }
+  __syncthreads();
+  return seen;
+}
+
+// ---- reserve ----------------------------------------------------------------
+// One workgroup: the order of the pages handed out is the order of the entries.
+// The entries of all ranges form one list (offsets by a prefix sum over the
+// sequences), read twice: to count what is missing, then to fill it.
+struct ReserveLds {
+  int32_t offset[kPoolBatch + 1];  // of a sequence's entries in the list
+  int32_t first[kPoolBatch];       // its first table slot
+  int32_t list[kPoolList];
+  RankScratch scratch;
+  int32_t bad;
+};
+__global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
+    PoolParams p, const int32_t *__restrict__ first_position,
+    const int32_t *__restrict__ end_position, int32_t *__restrict__ status) {
+  __shared__ ReserveLds lds;
+  const int t = threadIdx.x, lane = t & 63;
+  const int32_t batch = p.c.batch_size, pages = p.c.max_pages_per_seq;
+  if (t == 0) lds.bad = 0;
+  __syncthreads();
+  for (int32_t b = t; b < batch; b += kPoolThreads) {
+    const int32_t first = first_position[b], end = end_position[b];
+    SlotRange r{0, 0, true};
+    if (end > first) {
+      if (first < 0) {
+        r.ok = false;
+      } else {
+        const int32_t last = (int32_t)fast_div((uint32_t)(end - 1), p.page_div);
+        r = slot_range(p, (int32_t)fast_div((uint32_t)first, p.page_div), last + 1);
+      }
+    }
+    if (!r.ok) lds.bad = 1;
+    lds.first[b] = r.first;
+    lds.offset[b] = r.count;
+  }
+  __syncthreads();
+  if (lds.bad) {
+    if (t == 0) *status = kStatusArguments;
+    return;
+  }
+  // Exclusive prefix sum over the counts by the first wave. A table has fewer
+  // than 2^31 entries (checked by the caller), so the sums fit.
+  if (t < kWave) {
+    int32_t carry = 0;
+    for (int32_t b0 = 0; b0 < batch; b0 += kWave) {
+      const int32_t own = b0 + lane < batch ? lds.offset[b0 + lane] : 0;
+      int32_t sum = own;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int32_t other = __shfl_up(sum, d);
+        if (lane >= d) sum += other;
+      }
+      if (b0 + lane < batch) lds.offset[b0 + lane] = carry + sum - own;
+      carry += __shfl(sum, kWave - 1);
+    }
+    if (lane == 0) lds.offset[batch] = carry;
+  }
+  __syncthreads();
+  const int32_t items = lds.offset[batch];
+  // Table index of an item: its sequence is the last one that begins at or
+  // before it.
+  auto entry_of = [&](int32_t item) -> int64_t {
+    int32_t lo = 0, hi = batch;
+    while (hi - lo > 1) {
+      const int32_t mid = (lo + hi) >> 1;
+      if (lds.offset[mid] <= item) lo = mid; else hi = mid;
+    }
+    int32_t slot = lds.first[lo] + (item - lds.offset[lo]);
+    if (slot >= pages) slot -= pages;
+    return (int64_t)lo * pages + slot;
+  };
+  // f(table index or -1, rank of a missing entry or -1) for every item; returns
+  // how many are missing.
+  auto for_missing = [&](auto &&f) -> int32_t {
+    int32_t missing = 0;
+    for (int32_t base = 0; base < items; base += kPoolRound) {
+      int64_t at[kPoolUnroll];
+      bool flag[kPoolUnroll];
+      int32_t rank[kPoolUnroll];
+#pragma unroll
+      for (int u = 0; u < kPoolUnroll; ++u) {
+        const int32_t item = base + u * kPoolThreads + t;
+        at[u] = item < items ? entry_of(item) : -1;
+        flag[u] = at[u] >= 0 && p.page_table[at[u]] < 0;
+      }
+      const int32_t found = round_ranks(flag, rank, lds.scratch);
+#pragma unroll
+      for (int u = 0; u < kPoolUnroll; ++u)
+        if (flag[u]) f(at[u], missing + rank[u]);
+      missing += found;
+    }
+    return missing;
+  };
+  const int32_t wanted = for_missing([](int64_t, int32_t) {});
+  int32_t seen = find_free(p, 0, wanted, lds.list, lds.scratch);
+  if (seen < wanted) {
+    if (t == 0) *status = kStatusPages;
+    return;
+  }
+  if (t == 0) *status = kStatusOk;
+  // A window of the list at a time. What an earlier window filled is no longer
+  // missing: the ranks of what is left start at the window's own first.
+  for (int32_t from = 0; from < wanted; from += kPoolList) {
+    if (from > 0) find_free(p, 0, wanted - from, lds.list, lds.scratch);
+    for_missing([&](int64_t at, int32_t rank) {
+      if (rank >= kPoolList) return;
+      const int32_t page = lds.list[rank];
+      p.page_table[at] = page;
+      p.refs[page] = 1;
+    });
+    __threadfence_block();
+    __syncthreads();
+  }
+}
+
+// ---- fork -------------------------------------------------------------------
+struct ForkParams {
+  PoolParams pool;
+  int32_t *seq_lengths;
+  const int32_t *parents;
+  const int32_t *children;
+  int32_t count;
+  int32_t *status;
+};
+// What a branch gets in place of a parent's page.
+enum class Share { kNone, kSame, kCopy };
+__device__ __forceinline__ Share fork_share(const PoolParams &p, int32_t length, int32_t slot,
+                                            int32_t physical) {
+  if (physical < 0 || physical >= p.c.num_pages) return Share::kNone;
+  if (p.c.window_size > 0) return Share::kCopy;  // any ring page will be written again
+  const int32_t whole = (int32_t)fast_div((uint32_t)length, p.page_div);
+  if (slot < whole) return Share::kSame;
+  return slot == whole && length > whole * p.c.page_size ? Share::kCopy : Share::kNone;
+}
+
+struct ForkLds {
+  int32_t role[kPoolBatch];  // bit 0: a parent, bit 1: a child
+  int32_t list[kPoolList];
+  RankScratch scratch;
+  int32_t bad;
+};
+__global__ __launch_bounds__(kPoolThreads) void fork_tables_kernel(ForkParams f) {
+  __shared__ ForkLds lds;
+  const PoolParams &p = f.pool;
+  const int t = threadIdx.x;
+  const int32_t batch = p.c.batch_size, pages = p.c.max_pages_per_seq;
+  for (int32_t b = t; b < batch; b += kPoolThreads) lds.role[b] = 0;
+  if (t == 0) lds.bad = 0;
+  __syncthreads();
+  for (int32_t r = t; r < f.count; r += kPoolThreads) {
+    const int32_t parent = f.parents[r], child = f.children[r];
+    bool ok = parent >= 0 && parent < batch && child >= 0 && child < batch;
+    if (ok) {
+      const int32_t length = f.seq_lengths[parent];
+      ok = length >= 0 && (p.c.window_size > 0 || length <= (int64_t)pages * p.c.page_size);
+      atomicOr(&lds.role[parent], 1);
+      if (atomicOr(&lds.role[child], 2) & 2) ok = false;  // a child of two
+    }
+    if (!ok) lds.bad = 1;
+  }
+  __syncthreads();
+  for (int32_t b = t; b < batch; b += kPoolThreads)
+    if (lds.role[b] == 3) lds.bad = 1;
+  __syncthreads();
+  if (lds.bad) {
+    if (t == 0) *f.status = kStatusArguments;
+    return;
+  }
+  // Entry (request r, slot s) of the list at r * pages + s.
+  const int32_t items = f.count * pages;
+  // visit(share, child's table index, parent's page, rank among the copies).
+  auto for_entries = [&](auto &&visit) -> int32_t {
+    int32_t copies = 0;
+    for (int32_t base = 0; base < items; base += kPoolRound) {
+      int64_t to[kPoolUnroll];
+      int32_t physical[kPoolUnroll], rank[kPoolUnroll];
+      Share share[kPoolUnroll];
+      bool flag[kPoolUnroll];
+#pragma unroll
+      for (int u = 0; u < kPoolUnroll; ++u) {
+        const int32_t item = base + u * kPoolThreads + t;
+        to[u] = -1;
+        physical[u] = -1;
+        share[u] = Share::kNone;
+        if (item < items) {
+          const int32_t r = (int32_t)fast_div((uint32_t)item, p.slot_div);
+          const int32_t slot = item - r * pages;
+          const int32_t parent = f.parents[r];
+          to[u] = (int64_t)f.children[r] * pages + slot;
+          physical[u] = p.page_table[(int64_t)parent * pages + slot];
+          share[u] = fork_share(p, f.seq_lengths[parent], slot, physical[u]);
+        }
+        flag[u] = share[u] == Share::kCopy;
+      }
+      const int32_t found = round_ranks(flag, rank, lds.scratch);
+#pragma unroll
+      for (int u = 0; u < kPoolUnroll; ++u)
+        if (to[u] >= 0) visit(share[u], to[u], physical[u], copies + rank[u]);
+      copies += found;
+    }
+    return copies;
+  };
+  // A child holds nothing yet.
+  const int32_t wanted = for_entries([&](Share, int64_t to, int32_t, int32_t) {
+    if (p.page_table[to] >= 0) lds.bad = 1;
+  });
+  __syncthreads();
+  if (lds.bad) {
+    if (t == 0) *f.status = kStatusArguments;
+    return;
+  }
+  const int32_t seen = find_free(p, 0, wanted, lds.list, lds.scratch);
+  if (seen < wanted) {
+    if (t == 0) *f.status = kStatusPages;
+    return;
+  }
+  // The first window also shares; later ones only hand out their pages. A page
+  // handed out is free no more, so the list of the next window starts with its
+  // own first page.
+  for (int32_t from = 0; from == 0 || from < wanted; from += kPoolList) {
+    if (from > 0) find_free(p, 0, wanted - from, lds.list, lds.scratch);
+    for_entries([&](Share share, int64_t to, int32_t physical, int32_t rank) {
+      if (share == Share::kSame && from == 0) {
+        p.page_table[to] = physical;
+        atomicAdd(&p.refs[physical], 1);
+      } else if (share == Share::kCopy && rank >= from && rank - from < kPoolList) {
+        const int32_t page = lds.list[rank - from];
+        p.page_table[to] = page;
+        p.refs[page] = 1;
+      }
+    });
+    __threadfence_block();
+    __syncthreads();
+  }
+  for (int32_t r = t; r < f.count; r += kPoolThreads)
+    f.seq_lengths[f.children[r]] = f.seq_lengths[f.parents[r]];
+  if (t == 0) *f.status = kStatusOk;
+}
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 8;
+constexpr int kCopyPacks = kCopyThreads * kCopyUnroll;  // 16-byte packs per workgroup
+
+// Workgroup (piece of a page, copied page of a branch, layer x {K, V}): the
+// branch's table says where to, what the parent's length leaves in a begun page
+// how much. All loads of a piece are in flight before its first store.
+__global__ __launch_bounds__(kCopyThreads) void fork_copy_kernel(ForkParams f, uint16_t *cache_k,
+                                                                 uint16_t *cache_v, int32_t pieces,
+                                                                 int32_t slots) {
+  if (*f.status != kStatusOk) return;
+  const PoolParams &p = f.pool;
+  const int32_t pages = p.c.max_pages_per_seq;
+  const int32_t piece = blockIdx.x % pieces, which = blockIdx.x / pieces;
+  const int32_t r = which / slots;
+  const int32_t parent = f.parents[r], child = f.children[r];
+  const int32_t length = f.seq_lengths[parent];
+  int32_t slot = which - r * slots, rows = p.c.page_size;
+  if (p.c.window_size == 0) {
+    slot = (int32_t)fast_div((uint32_t)length, p.page_div);
+    rows = length - slot * p.c.page_size;
+    if (rows == 0) return;
+  }
+  const int32_t from = p.page_table[(int64_t)parent * pages + slot];
+  const int32_t to = p.page_table[(int64_t)child * pages + slot];
+  if (fork_share(p, length, slot, from) != Share::kCopy || to < 0) return;
+  const int64_t row_packs = (int64_t)p.c.num_heads * p.c.head_dim / kPackElems;
+  const int64_t packs = rows * row_packs, page_packs = p.c.page_size * row_packs;
+  const int64_t layer = (int64_t)(blockIdx.y >> 1) * p.c.num_pages;
+  uint16_t *cache = blockIdx.y & 1 ? cache_v : cache_k;
+  const uint16_t *src = cache + (layer + from) * page_packs * kPackElems;
+  uint16_t *dst = cache + (layer + to) * page_packs * kPackElems;
+  const int64_t first = (int64_t)piece * kCopyPacks + threadIdx.x;
+  uint4 x[kCopyUnroll];
+#pragma unroll
+  for (int u = 0; u < kCopyUnroll; ++u) {
+    const int64_t i = first + u * kCopyThreads;
+    if (i < packs) x[u] = load128(src + i * kPackElems);
+  }
+#pragma unroll
+  for (int u = 0; u < kCopyUnroll; ++u) {
+    const int64_t i = first + u * kCopyThreads;
+    if (i < packs) store128(dst + i * kPackElems, x[u]);
+  }
+}
+
+// ---- compact ------------------------------------------------------------------
+struct CompactParams {
+  uint16_t *cache_k;
+  uint16_t *cache_v;
+  Gemma4KvCacheConfig c;
+  FastDiv page_div, slot_div;
+  const int32_t *page_table;
+  const int32_t *refs;  // null: no page is shared
+  const int32_t *sequences;
+  const int32_t *first;
+  const int32_t *offsets;
+  const int32_t *positions;
+  int32_t count, total;
+  int32_t slices;  // parts of a row, one workgroup each
+  int32_t *status;
+};
+constexpr int kCompactThreads = 1024;
+constexpr int kCompactList = 4096;   // rows whose places LDS holds at a time
+constexpr int kCompactUnroll = 4;
+constexpr int kStatusList = 1, kStatusUnmapped = 2, kStatusShared = 3;
+
+// Workgroup (request, slice of a row, layer x {K, V}). Kept token j moves from
+// position kept[j] to first + j <= kept[j], in place. Rows are taken in order,
+// a batch at a time: every load of a batch has arrived before its first store,
+// and a later batch's sources lie behind everything that was stored before
+// (kept[j] > kept[i] >= first + i for j > i), so nothing is overwritten unread and
+// the next batch's loads go out ahead of the stores.
+__global__ __launch_bounds__(kCompactThreads) void compact_kernel(CompactParams p) {
+  __shared__ int32_t s_src[kCompactList], s_dst[kCompactList];
+  __shared__ int32_t s_error;
+  const int t = threadIdx.x;
+  const int32_t i = blockIdx.x / p.slices, slice = blockIdx.x - i * p.slices;
+  const int32_t pages = p.c.max_pages_per_seq;
+  const int32_t b = p.sequences[i], first = p.first[i];
+  const int32_t begin = p.offsets[i], end = p.offsets[i + 1];
+  const int64_t capacity = (int64_t)pages * p.c.page_size;
+  const int32_t n = end - begin;
+  if (t == 0)
+    s_error = b >= 0 && b < p.c.batch_size && first >= 0 && begin >= 0 && end >= begin &&
+                      end <= p.total && first <= 0x7fffffff - n
+                  ? 0 : kStatusList;
+  __syncthreads();
+  int32_t error = s_error;
+  // One request per sequence.
+  if (error == 0) {
+    for (int32_t j = t; j < p.count; j += kCompactThreads)
+      if (j != i && p.sequences[j] == b) error = kStatusList;
+  }
+  const int32_t *table = p.page_table + (int64_t)b * pages;
+  const int32_t *kept = p.positions + begin;
+  // Row of the layer at a position, -1 where no page is mapped.
+  auto row_of = [&](int32_t position, int32_t &page) -> int64_t {
+    const uint32_t logical = fast_div((uint32_t)position, p.page_div);
+    const uint32_t slot = p.c.window_size > 0 ? fast_mod(logical, p.slot_div) : logical;
+    page = table[slot];
+    if (page < 0 || page >= p.c.num_pages) return -1;
+    return (int64_t)page * p.c.page_size + (position - (int32_t)logical * p.c.page_size);
+  };
+  if (s_error == 0) {
+    for (int32_t j = t; j < n; j += kCompactThreads) {
+      const int32_t from = kept[j], to = first + j;
+      if (from < to || (j > 0 && kept[j - 1] >= from) ||
+          (p.c.window_size > 0 ? from - first >= capacity : from >= capacity)) {
+        error = max(error, kStatusList);
+        continue;
+      }
+      int32_t src_page, dst_page;
+      const int64_t src = row_of(from, src_page), dst = row_of(to, dst_page);
+      if (src < 0 || dst < 0) {
+        error = max(error, kStatusUnmapped);
+      } else if (from != to && p.refs != nullptr && p.refs[dst_page] > 1) {
+        error = max(error, kStatusShared);
+      }
+      if (j < kCompactList) {
+        s_src[j] = (int32_t)src;
+        s_dst[j] = from == to ? -1 : (int32_t)dst;
+      }
+    }
+  }
+  if (error != 0) atomicMax(&s_error, error);
+  __syncthreads();
+  error = s_error;
+  if (t == 0 && slice == 0 && blockIdx.y == 0) p.status[i] = error;
+  if (error != 0) return;
+
+  const int32_t row_packs = p.c.num_heads * p.c.head_dim / kPackElems;
+  const int32_t c0 = (int32_t)((int64_t)row_packs * slice / p.slices);
+  const int32_t width = (int32_t)((int64_t)row_packs * (slice + 1) / p.slices) - c0;
+  uint16_t *cache = (blockIdx.y & 1 ? p.cache_v : p.cache_k) +
+                    ((int64_t)(blockIdx.y >> 1) * p.c.num_pages * p.c.page_size * row_packs + c0) *
+                        kPackElems;
+  // Thread t: pack t % width of rows t / width + k * stride.
+  const int32_t stride = kCompactThreads / width;
+  const int32_t my_row = t / width, my_pack = t - my_row * width;
+  const bool idle = my_row >= stride;
+  for (int32_t base = 0; base < n; base += kCompactList) {
+    const int32_t rows = min(n - base, kCompactList);
+    if (base > 0) {
+      __syncthreads();
+      for (int32_t j = t; j < rows; j += kCompactThreads) {
+        int32_t page;
+        s_src[j] = (int32_t)row_of(kept[base + j], page);
+        s_dst[j] = kept[base + j] == first + base + j ? -1 : (int32_t)row_of(first + base + j, page);
+      }
+      __syncthreads();
+    }
+    const int32_t step = stride * kCompactUnroll;
+    uint4 x[kCompactUnroll], next[kCompactUnroll];
+    auto load = [&](int32_t at, uint4 (&v)[kCompactUnroll]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < kCompactUnroll; ++u) {
+        const int32_t j = at + u * stride + my_row;
+        if (!idle && j < rows && s_dst[j] >= 0)
+          v[u] = load128(cache + ((int64_t)s_src[j] * row_packs + my_pack) * kPackElems);
+      }
+    };
+    load(0, x);
+    for (int32_t at = 0; at < rows; at += step) {
+      load(at + step, next);
+      // Every thread's loads of this batch (and the next) have arrived.
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < kCompactUnroll; ++u) {
+        const int32_t j = at + u * stride + my_row;
+        if (!idle && j < rows && s_dst[j] >= 0)
+          store128(cache + ((int64_t)s_dst[j] * row_packs + my_pack) * kPackElems, x[u]);
+        x[u] = next[u];
+      }
+    }
+    // The next list's sources lie behind what was stored: no wait for the stores.
+  }
+}
+
+// ---- host -------------------------------------------------------------------
+bool valid_pool(const Gemma4KvCacheConfig &c) {
+  return c.num_pages > 0 && c.page_size > 0 && c.max_pages_per_seq > 0 && c.batch_size > 0 &&
+         c.batch_size <= kPoolBatch && c.window_size >= 0 &&
+         (int64_t)c.batch_size * c.max_pages_per_seq <= 0x7fffffff &&
+         (int64_t)c.num_pages * c.page_size <= 0x7fffffff;
+}
+bool valid_rows(const Gemma4KvCacheConfig &c) {
+  return c.num_layers > 0 && c.num_layers <= 32767 && c.num_heads > 0 && c.head_dim > 0 &&
+         c.head_dim % kPackElems == 0 && (int64_t)c.num_heads * c.head_dim <= (1 << 20);
+}
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+PoolParams pool_params(int32_t *page_table, int32_t *refs, const Gemma4KvCacheConfig &c) {
+  return {page_table, refs, c, make_fast_div(c.page_size), make_fast_div(c.max_pages_per_seq)};
+}
+
+}  // namespace
+}  // namespace gemma4
+
+using namespace gemma4;
+
+extern "C" {
+
+hipError_t gemma4_kv_cache_release_pages(int32_t *d_page_table, int32_t *d_page_refs,
+                                         Gemma4KvCacheConfig config,
+                                         const int32_t *d_first_position,
+                                         const int32_t *d_end_position, hipStream_t stream) {
+  if (!valid_pool(config) || d_page_table == nullptr || d_page_refs == nullptr ||
+      d_first_position == nullptr || d_end_position == nullptr) {
+    return hipErrorInvalidValue;
+  }
+  const int64_t entries = (int64_t)config.batch_size * config.max_pages_per_seq;
+  hipLaunchKernelGGL(release_pages_kernel, dim3((uint32_t)((entries + 255) / 256)), dim3(256), 0,
+                     stream, pool_params(d_page_table, d_page_refs, config), d_first_position,
+                     d_end_position, entries);
+  return hipGetLastError();
+}
+
+hipError_t gemma4_kv_cache_reserve_pages(int32_t *d_page_table, int32_t *d_page_refs,
+                                         Gemma4KvCacheConfig config,
+                                         const int32_t *d_first_position,
+                                         const int32_t *d_end_position, int32_t *d_status,
+                                         hipStream_t stream) {
+  if (!valid_pool(config) || d_page_table == nullptr || d_page_refs == nullptr ||
+      d_first_position == nullptr || d_end_position == nullptr || d_status == nullptr) {
+    return hipErrorInvalidValue;
+  }
+  hipLaunchKernelGGL(reserve_pages_kernel, dim3(1), dim3(kPoolThreads), 0, stream,
+                     pool_params(d_page_table, d_page_refs, config), d_first_position,
+                     d_end_position, d_status);
+  return hipGetLastError();
+}
+
+hipError_t gemma4_kv_cache_fork_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cache_v,
+                                     Gemma4KvCacheConfig config, int32_t *d_page_table,
+                                     int32_t *d_page_refs, int32_t *d_seq_lengths,
+                                     const int32_t *d_parents, const int32_t *d_children,
+                                     int32_t fork_count, int32_t *d_status, hipStream_t stream) {
+  if (fork_count == 0) return hipSuccess;
+  if (fork_count < 0 || !valid_pool(config) || !valid_rows(config) ||
+      fork_count > config.batch_size || d_cache_k == nullptr || d_cache_v == nullptr ||
+      !aligned16(d_cache_k) || !aligned16(d_cache_v) || d_page_table == nullptr ||
+      d_page_refs == nullptr || d_seq_lengths == nullptr || d_parents == nullptr ||
+      d_children == nullptr || d_status == nullptr) {
+    return hipErrorInvalidValue;
+  }
+  const ForkParams f = {pool_params(d_page_table, d_page_refs, config), d_seq_lengths, d_parents,
+                        d_children, fork_count, d_status};
+  const int64_t page_packs =
+      (int64_t)config.page_size * config.num_heads * config.head_dim / kPackElems;
+  const int32_t slots = config.window_size > 0 ? config.max_pages_per_seq : 1;
+  const int64_t pieces = (page_packs + kCopyPacks - 1) / kCopyPacks;
+  const int64_t blocks = pieces * slots * fork_count;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(fork_tables_kernel, dim3(1), dim3(kPoolThreads), 0, stream, f);
+  hipLaunchKernelGGL(fork_copy_kernel, dim3((uint32_t)blocks, 2 * config.num_layers),
+                     dim3(kCopyThreads), 0, stream, f, reinterpret_cast<uint16_t *>(d_cache_k),
+                     reinterpret_cast<uint16_t *>(d_cache_v), (int32_t)pieces, slots);
+  return hipGetLastError();
+}
+
+hipError_t gemma4_kv_cache_compact_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cache_v,
+                                        Gemma4KvCacheConfig config, const int32_t *d_page_table,
+                                        const int32_t *d_page_refs, const int32_t *d_sequences,
+                                        const int32_t *d_first_positions,
+                                        const int32_t *d_kept_offsets,
+                                        const int32_t *d_kept_positions, int32_t sequence_count,
+                                        int32_t total_kept, int32_t *d_status,
+                                        hipStream_t stream) {
+  if (sequence_count == 0) return hipSuccess;
+  if (sequence_count < 0 || total_kept < 0 || !valid_pool(config) || !valid_rows(config) ||
+      sequence_count > config.batch_size || d_cache_k == nullptr || d_cache_v == nullptr ||
+      !aligned16(d_cache_k) || !aligned16(d_cache_v) || d_page_table == nullptr ||
+      d_sequences == nullptr || d_first_positions == nullptr || d_kept_offsets == nullptr ||
+      (d_kept_positions == nullptr && total_kept > 0) || d_status == nullptr) {
+    return hipErrorInvalidValue;
+  }
+  const int32_t row_packs = config.num_heads * (config.head_dim / kPackElems);
+  // Slices of 256 bytes or more, at most a workgroup's width, until there are two
+  // workgroups per CU.
+  const int64_t wide = (int64_t)sequence_count * 2 * config.num_layers;
+  int32_t slices = (row_packs + kCompactThreads - 1) / kCompactThreads;
+  while (row_packs / (2 * slices) >= 16 && wide * slices < 512) slices *= 2;
+  const CompactParams p = {reinterpret_cast<uint16_t *>(d_cache_k),
+                           reinterpret_cast<uint16_t *>(d_cache_v),
+                           config,
+                           make_fast_div(config.page_size),
+                           make_fast_div(config.max_pages_per_seq),
+                           d_page_table,
+                           d_page_refs,
+                           d_sequences,
+                           d_first_positions,
+                           d_kept_offsets,
+                           d_kept_positions,
+                           sequence_count,
+                           total_kept,
+                           slices,
+                           d_status};
+  hipLaunchKernelGGL(compact_kernel, dim3((uint32_t)(sequence_count * slices), 2 * config.num_layers),
+                     dim3(kCompactThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // extern "C"

@@ -84,6 +84,18 @@ SIGNATURES = {
     "gemma4_flash_attention_prefill_chunk_workspace_bytes": (ctypes.c_size_t, [_I32, _I32, _CFG]),
     "gemma4_flash_attention_prefill_chunk_paged_bf16_ws": (
         _I32, [_P, _P, _P, _P, _P, _P, _P, _P, _CFG, _I32, _I32, _I32, _F32, _P, ctypes.c_size_t, _P]),
+    "gemma4_flash_attention_extend_plan_bytes": (ctypes.c_size_t, [_CFG, _I32, _I32]),
+    "gemma4_flash_attention_extend_workspace_bytes": (ctypes.c_size_t, [_CFG, _I32, _I32]),
+    "gemma4_flash_attention_extend_plan": (
+        _I32, [_P, ctypes.c_size_t, _P, _P, _CFG, _I32, _I32, _I32, _I32, _P]),
+    "gemma4_flash_attention_extend_paged_bf16": (
+        _I32, [_P] * 8 + [ctypes.c_size_t, _CFG, _I32, _I32, _I32, _I64, _I64, _F32, _P,
+                          ctypes.c_size_t, _P]),
+    "gemma4_kv_cache_release_pages": (_I32, [_P, _P, _CFG, _P, _P, _P]),
+    "gemma4_kv_cache_reserve_pages": (_I32, [_P, _P, _CFG, _P, _P, _P, _P]),
+    "gemma4_kv_cache_fork_bf16": (_I32, [_P, _P, _CFG, _P, _P, _P, _P, _P, _I32, _P, _P]),
+    "gemma4_kv_cache_compact_bf16": (
+        _I32, [_P, _P, _CFG, _P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P]),
     "gemma4_flash_attention_sliding_fwd_bf16_norm_rope": (
         _I32, [_P] * 12 + [_I32, _I32, _I32, _I32, _F32, _P]),
     "gemma4_flash_attention_global_fwd_bf16_norm_rope": (
@@ -526,3 +538,63 @@ def flash_attention_prefill_chunk_paged_bf16(out, q, k, v, cache_k, cache_v, pag
         ptr(out), ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(page_table),
         ptr(prior_lengths), config, layer, batch_size, chunk_len, softmax_scale,
         stream_handle(stream))
+
+
+# ---- pages of a pool ---------------------------------------------------------
+
+def kv_cache_release_pages(page_table, page_refs, config, first_position, end_position,
+                           stream=None) -> int:
+    return lib().gemma4_kv_cache_release_pages(
+        ptr(page_table), ptr(page_refs), config, ptr(first_position), ptr(end_position),
+        stream_handle(stream))
+
+
+def kv_cache_reserve_pages(page_table, page_refs, config, first_position, end_position, status,
+                           stream=None) -> int:
+    return lib().gemma4_kv_cache_reserve_pages(
+        ptr(page_table), ptr(page_refs), config, ptr(first_position), ptr(end_position),
+        ptr(status), stream_handle(stream))
+
+
+def kv_cache_fork_bf16(cache_k, cache_v, config, page_table, page_refs, seq_lengths, parents,
+                       children, fork_count, status, stream=None) -> int:
+    return lib().gemma4_kv_cache_fork_bf16(
+        ptr(cache_k), ptr(cache_v), config, ptr(page_table), ptr(page_refs), ptr(seq_lengths),
+        ptr(parents), ptr(children), fork_count, ptr(status), stream_handle(stream))
+
+
+def kv_cache_compact_bf16(cache_k, cache_v, config, page_table, page_refs, sequences,
+                          first_positions, kept_offsets, kept_positions, sequence_count,
+                          total_kept, status, stream=None) -> int:
+    """page_refs: the pool's counts, or None where no page is shared."""
+    return lib().gemma4_kv_cache_compact_bf16(
+        ptr(cache_k), ptr(cache_v), config, ptr(page_table), ptr(page_refs), ptr(sequences),
+        ptr(first_positions), ptr(kept_offsets), ptr(kept_positions), sequence_count, total_kept,
+        ptr(status), stream_handle(stream))
+
+
+# ---- attention of a ragged batch of new tokens -------------------------------
+
+def flash_attention_extend_plan_bytes(config, batch_size, total_rows) -> int:
+    return lib().gemma4_flash_attention_extend_plan_bytes(config, batch_size, total_rows)
+
+
+def flash_attention_extend_workspace_bytes(config, batch_size, total_rows) -> int:
+    return lib().gemma4_flash_attention_extend_workspace_bytes(config, batch_size, total_rows)
+
+
+def flash_attention_extend_plan(plan, plan_bytes, row_offsets, prior_lengths, config, batch_size,
+                                total_rows, window_size, sink_tokens, stream=None) -> int:
+    return lib().gemma4_flash_attention_extend_plan(
+        ptr(plan), plan_bytes, ptr(row_offsets), ptr(prior_lengths), config, batch_size,
+        total_rows, window_size, sink_tokens, stream_handle(stream))
+
+
+def flash_attention_extend_paged_bf16(out, q, k, v, cache_k, cache_v, page_table, plan,
+                                      plan_bytes, config, layer, batch_size, total_rows,
+                                      softmax_scale, workspace, workspace_bytes, stream=None,
+                                      q_stride=0, kv_stride=0) -> int:
+    return lib().gemma4_flash_attention_extend_paged_bf16(
+        ptr(out), ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(page_table), ptr(plan),
+        plan_bytes, config, layer, batch_size, total_rows, q_stride, kv_stride, softmax_scale,
+        ptr(workspace), workspace_bytes, stream_handle(stream))

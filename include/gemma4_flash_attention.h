@@ -187,6 +187,59 @@ hipError_t gemma4_flash_attention_prefill_chunk_paged_bf16_ws(
     int32_t layer, int32_t batch_size, int32_t chunk_len, float softmax_scale,
     void *d_workspace, size_t workspace_bytes, hipStream_t stream);
 
+// ---- attention of a ragged batch of new tokens over the cache ---------------
+// One step of a server: every sequence b < batch_size brings its own number of
+// new tokens, one (a decode step), a few (drafts to verify) or many (a prompt's
+// chunk), over the d_prior_lengths[b] keys it has in the cache. The rows are
+// packed: sequence b's are d_row_offsets[b] .. d_row_offsets[b + 1] of q, k, v and
+// out (d_row_offsets [batch_size + 1], ascending from 0, total_rows at its end; a
+// sequence may have none). Row r of a sequence sits at position P + r,
+// P = d_prior_lengths[b], and sees the keys j <= P + r with j > P + r -
+// window_size or j < sink_tokens (window_size 0: all of them): those at P and
+// after from the rows' own prepared k and v, earlier ones from the cache through
+// the page table; keys on unmapped pages are skipped. The cache is only read: the
+// caller writes the rows afterwards (gemma4_kv_cache_write_bf16), as for a prefill
+// chunk. Geometries 8 KV heads x 256 and 1 KV head x 512, 16 query heads.
+// window_size: 1 .. config.window_size over a sliding cache (whose ring must hold
+// that many slots; sink_tokens is 0 there, the ring has overwritten them); any
+// over a full-length one, where the pages between the sinks and the window may
+// have been released. No counterpart in the reference, whose prefill is one
+// sequence length for the batch (src/gemma4_flash_attention_prefill.cu:1131-1183)
+// and whose decode is batch 1 (src/gemma4_decode_megakernel.cu:143).
+//
+// The plan cuts the batch's work into equal shares for the chip's workgroups; it
+// depends on the lengths, the window and the geometry only, so one plan serves all
+// layers of a kind in a step. d_plan and d_workspace are 256-byte aligned and need
+// no initialisation; sizes for the largest batch_size and total_rows of a program
+// serve its smaller calls. Calls that share a workspace must not overlap; a plan
+// may be read by several. Offsets that do not ascend or pass total_rows are
+// clamped to it, a negative prior length counts as 0: such a plan attends to the
+// wrong keys but reads and writes within the tensors. Rows that no sequence
+// holds (total_rows past the last offset) are left as they were.
+size_t gemma4_flash_attention_extend_plan_bytes(Gemma4KvCacheConfig config, int32_t batch_size,
+                                                int32_t total_rows);
+size_t gemma4_flash_attention_extend_workspace_bytes(Gemma4KvCacheConfig config,
+                                                     int32_t batch_size, int32_t total_rows);
+hipError_t gemma4_flash_attention_extend_plan(void *d_plan, size_t plan_bytes,
+                                              const int32_t *d_row_offsets,
+                                              const int32_t *d_prior_lengths,
+                                              Gemma4KvCacheConfig config, int32_t batch_size,
+                                              int32_t total_rows, int32_t window_size,
+                                              int32_t sink_tokens, hipStream_t stream);
+
+// The attention of one layer by a plan made with the same config geometry,
+// batch_size and total_rows (a plan of other sizes writes nothing).
+// q_stride, kv_stride: elements from one row of q, and of k and v, to the next
+// (slices of a wider projection), multiples of 8; 0 for packed rows, 16 * head_dim
+// and num_heads * head_dim. out [total_rows][16][head_dim] is packed. q, k, v, out
+// and the caches are 16-byte aligned. total_rows == 0 is a no-op success.
+hipError_t gemma4_flash_attention_extend_paged_bf16(
+    gemma4_bf16 *d_out, const gemma4_bf16 *d_q, const gemma4_bf16 *d_k, const gemma4_bf16 *d_v,
+    const gemma4_bf16 *d_cache_k, const gemma4_bf16 *d_cache_v, const int32_t *d_page_table,
+    const void *d_plan, size_t plan_bytes, Gemma4KvCacheConfig config, int32_t layer,
+    int32_t batch_size, int32_t total_rows, int64_t q_stride, int64_t kv_stride,
+    float softmax_scale, void *d_workspace, size_t workspace_bytes, hipStream_t stream);
+
 // Prefill self-attention with Q/K/V preparation (seqlen_q == seqlen_k, no
 // prior context), same names, argument order and validation as the
 // reference launchers (src/gemma4_flash_attention.cuh:9-45,

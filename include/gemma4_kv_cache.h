@@ -123,6 +123,84 @@ hipError_t gemma4_kv_cache_write_prefill_bf16(
     int32_t layer, const gemma4_bf16 *d_k, const gemma4_bf16 *d_v,
     hipStream_t stream);
 
+// ---- pages of a pool -------------------------------------------------------
+// The operators below let page tables map any page of the cache instead of a
+// fixed one per slot (no counterparts in the reference, whose
+// src/gemma4_kv_cache.cu:108-122 maps physical page batch * max_pages_per_seq +
+// slot). The state is the page table [batch_size][max_pages_per_seq] (-1:
+// unmapped) and d_page_refs [num_pages], the number of table entries that map a
+// page (0: free); both start as -1 and 0 everywhere. One table and one count
+// array per cache: the layers of a cache share them, and `config` is that
+// cache's. batch_size is at most 4096, batch_size * max_pages_per_seq and
+// num_pages * page_size below 2^31. All are stream-ordered, allocate nothing, and
+// give the same result on every run: free pages are handed out lowest first, in
+// the order of the table entries. Calls that share a table, counts or a cache
+// must not overlap.
+//
+// Positions of a sliding cache name ring slots: logical page p sits in slot
+// p % max_pages_per_seq, as in gemma4_kv_cache_write_bf16.
+
+// Returns pages: for every sequence b < batch_size, the pages that lie wholly in
+// positions [d_first_position[b], d_end_position[b]) are unmapped and lose one
+// reference each (0 .. INT32_MAX: all of the sequence's; length .. INT32_MAX:
+// what a shortened sequence no longer needs; sinks .. length - window: what no
+// row of a windowed sequence will see again). An empty range changes nothing.
+hipError_t gemma4_kv_cache_release_pages(int32_t *d_page_table, int32_t *d_page_refs,
+                                         Gemma4KvCacheConfig config,
+                                         const int32_t *d_first_position,
+                                         const int32_t *d_end_position, hipStream_t stream);
+
+// Takes pages: for every sequence b < batch_size, every unmapped page that holds
+// a position of [d_first_position[b], d_end_position[b]) gets a free page with
+// one reference. *d_status: 0, or with nothing changed 1 (not enough free pages)
+// or 2 (a negative first position of a range, or one past a full-length table's
+// end).
+hipError_t gemma4_kv_cache_reserve_pages(int32_t *d_page_table, int32_t *d_page_refs,
+                                         Gemma4KvCacheConfig config,
+                                         const int32_t *d_first_position,
+                                         const int32_t *d_end_position, int32_t *d_status,
+                                         hipStream_t stream);
+
+// Branches sequences: child d_children[i] becomes a copy of d_parents[i] as it
+// stands at d_seq_lengths[d_parents[i]], which becomes the child's length too. A
+// full-length cache's whole pages are shared (one more reference each); the begun
+// page, which both will write to, is copied into a page of the child's own: its
+// live rows of every layer, K and V. Pages mapped ahead of the length stay the
+// parent's. A sliding ring's pages will all be written again and are all copied.
+// A child must hold no page (release it first), be named once and be no parent
+// in the call; fork_count <= batch_size. *d_status: 0, or with nothing changed 1
+// (not enough free pages) or 2 (a sequence out of range or named against these
+// rules, a length out of range). fork_count == 0 is a no-op success. Caches are
+// 16-byte aligned.
+hipError_t gemma4_kv_cache_fork_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cache_v,
+                                     Gemma4KvCacheConfig config, int32_t *d_page_table,
+                                     int32_t *d_page_refs, int32_t *d_seq_lengths,
+                                     const int32_t *d_parents, const int32_t *d_children,
+                                     int32_t fork_count, int32_t *d_status, hipStream_t stream);
+
+// Closes up kept tokens: for request i < sequence_count, the rows of sequence
+// d_sequences[i] at positions d_kept_positions[d_kept_offsets[i] ..
+// d_kept_offsets[i + 1]) move to d_first_positions[i], + 1, + 2, ..., in place,
+// in every layer, K and V (the accepted tokens of a verified draft; a prompt
+// thinned out). Rows move as they are: a key keeps the rotation of its old
+// position. A request's positions ascend strictly, none lies before its new
+// place, and for a sliding cache all lie within the ring's slots of the first
+// position. d_page_refs may be null where no page is shared; otherwise a request
+// that would write to a page with more than one reference is refused.
+// d_status[i]: 0, or with the sequence's rows unchanged 1 (a list, sequence or
+// position against these rules, two requests for one sequence), 2 (a page is
+// unmapped) or 3 (a destination page is shared). total_kept is the length of
+// d_kept_positions. The table, the counts and the lengths stay as they are.
+// sequence_count == 0 is a no-op success; sequence_count <= batch_size.
+hipError_t gemma4_kv_cache_compact_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cache_v,
+                                        Gemma4KvCacheConfig config, const int32_t *d_page_table,
+                                        const int32_t *d_page_refs, const int32_t *d_sequences,
+                                        const int32_t *d_first_positions,
+                                        const int32_t *d_kept_offsets,
+                                        const int32_t *d_kept_positions, int32_t sequence_count,
+                                        int32_t total_kept, int32_t *d_status,
+                                        hipStream_t stream);
+
 #ifdef __cplusplus
 }  // extern "C"
 #endif
