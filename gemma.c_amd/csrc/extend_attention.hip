@@ -2,6 +2,7 @@
 // plan that shares the work out, the merge of split row blocks and the entry
 // points. No counterpart in the reference.
 #include "extend_common.hpp"
+#include "extend_rows.hpp"
 
 #include <math.h>
 
@@ -197,79 +198,6 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
   }
 }
 
-// ---- the rows' attention --------------------------------------------------------
-// A wave per (row, query head), one key at a time.
-template <int kHeads, int kDim>
-__global__ __launch_bounds__(256) void extend_rows_kernel(ExtendParams p, ExtendGeometry g) {
-  if (!extend_plan_fits(p)) return;
-  constexpr int kGroup = kQueryHeads / kHeads, kPer = kDim / kWave;
-  const auto *h = reinterpret_cast<const ExtendHeader *>(p.plan);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int head = blockIdx.x % kHeads, share = blockIdx.x / kHeads;
-  const auto *share_first = reinterpret_cast<const int32_t *>(p.plan + p.share_first);
-  const auto *segments = reinterpret_cast<const ExtendSegment *>(p.plan + p.segments);
-  const int64_t layer = (int64_t)p.layer * p.c.num_pages * p.c.page_size;
-  for (int32_t i = share_first[share]; i < share_first[share + 1]; ++i) {
-    const ExtendSegment s = segments[i];
-    const int32_t first = s.prior + s.row0;
-    const ExtendTiles tiles =
-        extend_tiles(first, first + s.rows - 1, h->window, h->sinks, g.tile);
-    for (int32_t w = wave; w < s.rows * kGroup; w += 4) {
-      const int32_t r = w / kGroup, qh = head * kGroup + w % kGroup;
-      const int32_t at = first + r;
-      const int64_t row = s.base + s.row0 + r;
-      float q[kPer], o[kPer], m = -INFINITY, l = 0.0f;
-      for (int e = 0; e < kPer; ++e) {
-        q[e] = bf16_lo(p.q[row * p.q_stride + qh * kDim + lane + kWave * e]) * p.q_scale;
-        o[e] = 0.0f;
-      }
-      for (int32_t tile = s.tile_lo; tile < s.tile_hi; ++tile) {
-        const int32_t k0 =
-            (tile < tiles.sink_tiles ? tile : tile - tiles.sink_tiles + tiles.window_tile) * g.tile;
-        for (int32_t key = k0; key < k0 + g.tile && key <= at; ++key) {
-          if (h->window > 0 && key <= at - h->window && key >= h->sinks) continue;
-          const uint16_t *k, *v;
-          if (key >= s.prior) {
-            const int64_t from = (s.base + key - s.prior) * p.kv_stride + head * kDim;
-            k = p.k + from;
-            v = p.v + from;
-          } else {
-            const uint32_t logical = fast_div(key, p.page_div);
-            if (p.c.window_size == 0 && logical >= (uint32_t)p.c.max_pages_per_seq) continue;
-            const int32_t page = p.page_table[(int64_t)s.sequence * p.c.max_pages_per_seq +
-                                              fast_mod(logical, p.slot_div)];
-            if (page < 0 || page >= p.c.num_pages) continue;
-            const int64_t from = ((layer + (int64_t)page * p.c.page_size + key -
-                                   (int64_t)logical * p.c.page_size) * kHeads + head) * kDim;
-            k = p.cache_k + from;
-            v = p.cache_v + from;
-          }
-          float x = 0.0f;
-          for (int e = 0; e < kPer; ++e) x += q[e] * bf16_lo(k[lane + kWave * e]);
-          for (int d = 1; d < kWave; d <<= 1) x += __shfl_xor(x, d);
-          const float top = fmaxf(m, x), a = exp2f(m - top), w1 = exp2f(x - top);
-          l = l * a + w1;
-          for (int e = 0; e < kPer; ++e) o[e] = o[e] * a + w1 * bf16_lo(v[lane + kWave * e]);
-          m = top;
-        }
-      }
-      if (s.partial < 0) {
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        for (int e = 0; e < kPer; ++e)
-          p.out[(row * kQueryHeads + qh) * kDim + lane + kWave * e] =
-              (uint16_t)f32_to_bf16_bits(o[e] * inv);
-      } else {
-        const int64_t part = (int64_t)(s.partial + r) * kQueryHeads + qh;
-        for (int e = 0; e < kPer; ++e) p.partial[part * kDim + lane + kWave * e] = o[e];
-        if (lane == 0) {
-          p.stats[2 * part] = m;
-          p.stats[2 * part + 1] = l;
-        }
-      }
-    }
-  }
-}
-
 // ---- merge ----------------------------------------------------------------------
 // Workgroup (merged row, query head, 256 dims), four waves: lane l holds dims
 // 4 l .. + 3, the waves take the parts in turn.
@@ -458,13 +386,11 @@ extern "C" hipError_t gemma4_flash_attention_extend_paged_bf16(
                                       extend_stats_offset(l, config.head_dim));
   const uint32_t merge_grid = (uint32_t)std::min<int64_t>(
       kMergeGrid, std::max<int64_t>(l.max_merges, 1) * kQueryHeads * (config.head_dim / 256));
+  launch_extend_rows(p, stream);
   if (config.num_heads == 1) {
-    hipLaunchKernelGGL((extend_rows_kernel<1, 512>), dim3(g.shares), dim3(256), 0, stream, p, g);
     hipLaunchKernelGGL(extend_merge_kernel<512>, dim3(merge_grid), dim3(kMergeThreads), 0, stream,
                        p);
   } else {
-    hipLaunchKernelGGL((extend_rows_kernel<8, 256>), dim3(8 * g.shares), dim3(256), 0, stream, p,
-                       g);
     hipLaunchKernelGGL(extend_merge_kernel<256>, dim3(merge_grid), dim3(kMergeThreads), 0, stream,
                        p);
   }

@@ -16,7 +16,7 @@ struct ExtendGeometry {
   int32_t tile;     // keys of a tile
   int32_t shares;   // workgroups per KV head: heads x shares fill the chip
 };
-constexpr ExtendGeometry kExtend256 = {64, 64, 32};
+constexpr ExtendGeometry kExtend256 = {64, 32, 32};
 constexpr ExtendGeometry kExtend512 = {8, 32, 256};
 constexpr int kExtendBatch = 4096;  // sequences at most
 

@@ -34,9 +34,11 @@ HIP_FLAGS = [
 # Per-source additions. The prefill kernels rescale their MFMA accumulators with
 # VALU multiplies on a rarely taken path; in the AGPR form the register
 # allocator copies all 128 accumulators between AGPRs and VGPRs on every tile
-# to serve that path, so their MFMAs are selected in the VGPR form.
+# to serve that path, so their MFMAs are selected in the VGPR form. extend_rows
+# holds its accumulators in AGPRs by inline asm; the form keeps its scores in VGPRs.
 EXTRA_FLAGS = {
     "decode_d512": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "extend_rows": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "prefill_attention": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "prefill_norm_rope": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
 }
