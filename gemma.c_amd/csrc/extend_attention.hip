@@ -109,7 +109,12 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
       if (s_blocks[mid] <= j) lo = mid; else hi = mid;
     }
     r.sequence = lo;
-    r.row0 = (j - s_blocks[lo]) * p.g.rows;
+    // Causal work grows along a sequence: its blocks are laid out first, last, second,
+    // last but one, .. so that every pair costs the same. Where two shares serve a
+    // pair, every other cut falls between blocks, and the shares of one parity walk
+    // the same keys at about the same time, which L2 notices.
+    const int32_t at = j - s_blocks[lo], blocks = s_blocks[lo + 1] - s_blocks[lo];
+    r.row0 = (at % 2 == 0 ? at / 2 : blocks - 1 - at / 2) * p.g.rows;
     r.rows = min(s_begin[lo + 1] - s_begin[lo] - r.row0, p.g.rows);
     r.prior = min(max(p.prior_lengths[lo], 0), p.max_prior);
     const int32_t first = r.prior + r.row0;
@@ -199,60 +204,90 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
 }
 
 // ---- merge ----------------------------------------------------------------------
-// Workgroup (merged row, query head, 256 dims), four waves: lane l holds dims
-// 4 l .. + 3, the waves take the parts in turn.
+// Item: (merged row, query head, 256 dims), lane l holding dims 4 l .. + 3. A row of
+// few parts is one wave's, kMergeBatch parts' loads at a time; of many, the four
+// waves' of a workgroup, each a quarter of the parts. Parts are folded in a fixed
+// order either way.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeWaves = kMergeThreads / kWave;
 constexpr int kMergeGrid = 2048;
+constexpr int kMergeBatch = 8;
+constexpr int kMergeFew = 16;  // parts a single wave folds
+
+struct MergeState {
+  float m = -INFINITY, l = 0.0f;
+  float4 acc = {0, 0, 0, 0};
+  __device__ __forceinline__ void fold(float mi, float li, const float4 &a) {
+    const float top = fmaxf(m, mi);
+    const float fa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    const float fb = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - top);
+    l = l * fa + li * fb;
+    // A part without a visible key has nothing to add, whatever its sums are.
+    acc.x = acc.x * fa + (mi == -INFINITY ? 0.0f : a.x * fb);
+    acc.y = acc.y * fa + (mi == -INFINITY ? 0.0f : a.y * fb);
+    acc.z = acc.z * fa + (mi == -INFINITY ? 0.0f : a.z * fb);
+    acc.w = acc.w * fa + (mi == -INFINITY ? 0.0f : a.w * fb);
+    m = top;
+  }
+};
+
 template <int kDim>
 __global__ __launch_bounds__(kMergeThreads) void extend_merge_kernel(ExtendParams p) {
   if (!extend_plan_fits(p)) return;
   __shared__ float4 s_acc[kMergeWaves][kWave];
   __shared__ float2 s_stats[kMergeWaves];
-  constexpr int kSlices = kDim / 256;
+  constexpr int kSlices = kDim / 256, kRowItems = kQueryHeads * kSlices;
   const auto *h = reinterpret_cast<const ExtendHeader *>(p.plan);
   const auto *merges = reinterpret_cast<const ExtendMerge *>(p.plan + p.merges);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int32_t items = h->merges * kQueryHeads * kSlices;
-  for (int32_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const ExtendMerge r = merges[i / (kQueryHeads * kSlices)];
-    const int qh = i / kSlices % kQueryHeads, d0 = i % kSlices * 256 + 4 * lane;
-    float m = -INFINITY, l = 0.0f;
-    float4 acc = {0, 0, 0, 0};
-    for (int32_t part = wave; part < r.parts; part += kMergeWaves) {
-      const int64_t at = ((int64_t)r.partial + (int64_t)part * r.stride) * kQueryHeads + qh;
-      const float2 s = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
-      const float4 a = *reinterpret_cast<const float4 *>(p.partial + at * kDim + d0);
-      if (s.x == -INFINITY) continue;
-      const float top = fmaxf(m, s.x);
-      const float fa = __builtin_amdgcn_exp2f(m - top), fb = __builtin_amdgcn_exp2f(s.x - top);
-      l = l * fa + s.y * fb;
-      acc.x = acc.x * fa + a.x * fb;
-      acc.y = acc.y * fa + a.y * fb;
-      acc.z = acc.z * fa + a.z * fb;
-      acc.w = acc.w * fa + a.w * fb;
-      m = top;
+  const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
+  const int32_t items = h->merges * kRowItems;
+  // Parts first, first + step, .. of an item.
+  auto gather = [&](const ExtendMerge &r, int32_t item, int32_t first, int32_t step) {
+    const int qh = item / kSlices % kQueryHeads, d0 = item % kSlices * 256 + 4 * lane;
+    MergeState s;
+    for (int32_t i0 = first; i0 < r.parts; i0 += step * kMergeBatch) {
+      float2 stats[kMergeBatch];
+      float4 a[kMergeBatch];
+#pragma unroll
+      for (int i = 0; i < kMergeBatch; ++i) {
+        const int32_t part = i0 + i * step;
+        if (part >= r.parts) break;
+        const int64_t at = ((int64_t)r.partial + (int64_t)part * r.stride) * kQueryHeads + qh;
+        stats[i] = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
+        a[i] = *reinterpret_cast<const float4 *>(p.partial + at * kDim + d0);
+      }
+#pragma unroll
+      for (int i = 0; i < kMergeBatch; ++i) {
+        if (i0 + i * step >= r.parts) break;
+        s.fold(stats[i].x, stats[i].y, a[i]);
+      }
     }
-    s_acc[wave][lane] = acc;
-    if (lane == 0) s_stats[wave] = make_float2(m, l);
+    return s;
+  };
+  auto store = [&](const ExtendMerge &r, int32_t item, const MergeState &s) {
+    const int qh = item / kSlices % kQueryHeads, d0 = item % kSlices * 256 + 4 * lane;
+    const float inv = s.l > 0.0f ? 1.0f / s.l : 0.0f;
+    *reinterpret_cast<uint2 *>(p.out + ((int64_t)r.row * kQueryHeads + qh) * kDim + d0) =
+        make_uint2(cvt_pk_bf16(s.acc.x * inv, s.acc.y * inv),
+                   cvt_pk_bf16(s.acc.z * inv, s.acc.w * inv));
+  };
+  // Rows of few parts.
+  for (int32_t i = blockIdx.x * kMergeWaves + wave; i < items; i += gridDim.x * kMergeWaves) {
+    const ExtendMerge r = merges[i / kRowItems];
+    if (r.parts > kMergeFew) continue;
+    store(r, i, gather(r, i, 0, 1));
+  }
+  // Rows of many.
+  for (int32_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const ExtendMerge r = merges[i / kRowItems];
+    if (r.parts <= kMergeFew) continue;
+    MergeState s = gather(r, i, wave, kMergeWaves);
+    s_acc[wave][lane] = s.acc;
+    if (lane == 0) s_stats[wave] = make_float2(s.m, s.l);
     __syncthreads();
     if (wave == 0) {
-      for (int w = 1; w < kMergeWaves; ++w) {
-        const float2 s = s_stats[w];
-        const float4 a = s_acc[w][lane];
-        if (s.x == -INFINITY) continue;
-        const float top = fmaxf(m, s.x);
-        const float fa = __builtin_amdgcn_exp2f(m - top), fb = __builtin_amdgcn_exp2f(s.x - top);
-        l = l * fa + s.y * fb;
-        acc.x = acc.x * fa + a.x * fb;
-        acc.y = acc.y * fa + a.y * fb;
-        acc.z = acc.z * fa + a.z * fb;
-        acc.w = acc.w * fa + a.w * fb;
-        m = top;
-      }
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      *reinterpret_cast<uint2 *>(p.out + ((int64_t)r.row * kQueryHeads + qh) * kDim + d0) =
-          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+      for (int w = 1; w < kMergeWaves; ++w) s.fold(s_stats[w].x, s_stats[w].y, s_acc[w][lane]);
+      store(r, i, s);
     }
     __syncthreads();
   }

@@ -51,6 +51,8 @@ __device__ uint4 g_zero_row[64];
 constexpr int kTile = 32;              // keys per LDS stage: one MFMA block
 constexpr int kCopyKeys = kTile / kWaves;  // keys a wave copies
 
+constexpr int kRunTiles = kWave / kCopyKeys;  // tiles whose keys a wave resolves at once
+
 template <int kDim>
 struct Shape {
   static constexpr int kHeads = kDim == 256 ? 8 : 1;
@@ -123,8 +125,12 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
   struct Lds {
     uint4 k[kStages][kStageBytes / 16];
     uint4 v[kStages][kStageBytes / 16];
-    uint32_t valid[kStages][kWaves];        // bit j: key kCopyKeys w + j of the tile is readable
-    int32_t pages[kStages][kWaves][kWave];  // page-table entries of a tile's keys
+    // Of the current and the next run of kRunTiles tiles, by parity: the addresses
+    // of the keys that a wave copies, and which keys can be read.
+    uint64_t k_rows[2][kWaves][kWave];
+    uint64_t v_rows[2][kWaves][kWave];
+    uint8_t valid[2][kRunTiles][kWaves];  // bit j: key kCopyKeys w + j of the tile
+    int32_t pages[kWaves][kWave];         // the next run's page-table entries
   };
   __shared__ __attribute__((aligned(1024))) Lds lds;
 
@@ -177,12 +183,10 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
   auto v_chunk = [&](int l) __attribute__((always_inline)) -> uint32_t {
     return (G::kRowBytes == 1024 ? l : (l & 31) ^ ((l >> 5) << 2)) << 4;
   };
-  const int key_lane = kCopyKeys * wave + (lane & (kCopyKeys - 1));
   const uint32_t copy_row0 = kCopyKeys * wave * G::kRowBytes;
   const uint32_t k_dst = wave_uniform(lds_address(&lds.k[0][0]) + copy_row0);
   const uint32_t v_dst = wave_uniform(lds_address(&lds.v[0][0]) + copy_row0);
-  const uint32_t page_dst = wave_uniform(lds_address(&lds.pages[0][wave][0]));
-  constexpr uint32_t kPageStage = kWaves * kWave * 4;
+  const uint32_t page_dst = wave_uniform(lds_address(&lds.pages[wave][0]));
 
   for (; segment < segment_end; ++segment) {
     // ---- the segment ---------------------------------------------------------
@@ -205,26 +209,25 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     const int32_t wave_qmax = min(wave_qmin + G::kWaveRows - 1, last);
 
     // ---- key rows ----------------------------------------------------------------
+    // A wave resolves its keys of kRunTiles tiles at once: lane l key kCopyKeys w + l %
+    // 8 of the run's tile l / 8.
     const int32_t *table = p.page_table + (int64_t)seg.sequence * max_pages;
     const uint64_t chunk_off = (uint64_t)base * kv_bytes + head * G::kRowBytes;
     const uint64_t chunk_k = reinterpret_cast<uint64_t>(p.k) + chunk_off;
     const uint64_t chunk_v = reinterpret_cast<uint64_t>(p.v) + chunk_off;
-    // Table entry of this lane's key of tile it; any readable one for a new key.
-    auto page_entry = [&](int it) __attribute__((always_inline)) -> const int32_t * {
-      const uint32_t at = (uint32_t)max(min(tile_key(it) + key_lane, prior - 1), 0);
+    auto run_key = [&](int run, int l) __attribute__((always_inline)) -> int32_t {
+      return tile_key(run * kRunTiles + l / kCopyKeys) + kCopyKeys * wave + l % kCopyKeys;
+    };
+    // Table entry of this lane's key; any readable one for a new key.
+    auto page_entry = [&](int run, int l) __attribute__((always_inline)) -> const int32_t * {
+      const uint32_t at = (uint32_t)max(min(run_key(run, l), prior - 1), 0);
       return table + fast_mod(fast_div(at, p.page_div), p.slot_div);
     };
-    // Addresses of this lane's key's K and V rows in tile it; the ballot says which
-    // of the wave's keys can be read.
-    struct Rows {
-      uint64_t k, v;
-      uint32_t valid;
-    };
-    auto resolve = [&](int it, int32_t page) __attribute__((always_inline)) -> Rows {
-      const int32_t key = tile_key(it) + key_lane;
+    auto resolve = [&](int run, int l, int32_t page) __attribute__((always_inline)) {
+      const int32_t key = run_key(run, l);
       const bool fresh = key >= prior;
       const uint32_t logical = fast_div((uint32_t)key, p.page_div);
-      const bool seen = (key <= last) & (it < n_tiles) &
+      const bool seen = (key <= last) & (run * kRunTiles + l / kCopyKeys < n_tiles) &
                         ((window == 0) | (key > first - window) | (key < sinks));
       const bool mapped = ((uint32_t)page < (uint32_t)p.c.num_pages) &
                           (ring | (logical < (uint32_t)max_pages));
@@ -233,50 +236,40 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
           (uint32_t)page * p.page_div.d + ((uint32_t)key - logical * p.page_div.d);
       const uint64_t off = pick(fresh, (uint64_t)(uint32_t)(key - prior) * kv_bytes,
                                 (uint64_t)cached * G::kTokenBytes);
-      Rows r;
-      r.k = pick(ok, pick(fresh, chunk_k, cache_k) + off, zero_row);
-      r.v = pick(ok, pick(fresh, chunk_v, cache_v) + off, zero_row);
-      r.valid = (uint32_t)__builtin_amdgcn_ballot_w64(ok) & ((1u << kCopyKeys) - 1);
-      return r;
+      lds.k_rows[run & 1][wave][l] = pick(ok, pick(fresh, chunk_k, cache_k) + off, zero_row);
+      lds.v_rows[run & 1][wave][l] = pick(ok, pick(fresh, chunk_v, cache_v) + off, zero_row);
+      const uint64_t valid = __builtin_amdgcn_ballot_w64(ok);
+      if (l < kRunTiles) lds.valid[run & 1][l][wave] = (uint8_t)(valid >> (kCopyKeys * l));
     };
-    // Copy a of a wave: keys kCopyKeys w + 2 a and + 1 (lanes 0..31, 32..63) at 8 x
-    // 256, key kCopyKeys w + a at 1 x 512.
-    auto key_value = [&](uint64_t x, int a) __attribute__((always_inline)) -> uint64_t {
-      auto lane_value = [&](int j) __attribute__((always_inline)) -> uint64_t {
-        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, j);
-        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(x >> 32), j);
-        return (uint64_t)hi << 32 | lo;
-      };
-      if constexpr (G::kRowBytes == 1024) {
-        return lane_value(a);
-      } else {
-        const uint64_t even = lane_value(2 * a), odd = lane_value(2 * a + 1);
-        return half ? odd : even;
-      }
+    // This lane's row address for copy a of a tile: keys kCopyKeys w + 2 a and + 1
+    // (lanes 0 .. 31, 32 .. 63) at 8 x 256, key kCopyKeys w + a at 1 x 512.
+    auto row_slot = [&](int tile, int a, int l) __attribute__((always_inline)) -> int {
+      return tile % kRunTiles * kCopyKeys + (G::kRowBytes == 1024 ? a : 2 * a + (l >> 5));
+    };
+    auto k_row = [&](int tile, int a, int l) __attribute__((always_inline)) -> uint64_t {
+      return lds.k_rows[tile / kRunTiles & 1][wave][row_slot(tile, a, l)];
+    };
+    auto v_row = [&](int tile, int a, int l) __attribute__((always_inline)) -> uint64_t {
+      return lds.v_rows[tile / kRunTiles & 1][wave][row_slot(tile, a, l)];
     };
     // Lane l of a copy fills chunk l (or l % 32) of its key's row with the chunk that
     // the swizzle puts there: k_chunk and v_chunk with the key's a-dependent bits.
-    auto copy_k = [&](uint64_t rows_k, uint32_t chunk, int a, int stage)
+    auto copy_k = [&](uint64_t row, uint32_t chunk, int a, int stage)
         __attribute__((always_inline)) {
       const int key = G::kRowBytes == 1024 ? a : 2 * a;
-      copy_row_pair(key_value(rows_k, a) + (chunk ^ ((key & 15) << 4)),
-                    k_dst + stage * kStageBytes + a * 1024);
+      copy_row_pair(row + (chunk ^ ((key & 15) << 4)), k_dst + stage * kStageBytes + a * 1024);
     };
-    auto copy_v = [&](uint64_t rows_v, uint32_t chunk, int a, int stage)
+    auto copy_v = [&](uint64_t row, uint32_t chunk, int a, int stage)
         __attribute__((always_inline)) {
       const int key = G::kRowBytes == 1024 ? a : 2 * a;
-      copy_row_pair(key_value(rows_v, a) + (chunk ^ ((key & 3) << 6)),
-                    v_dst + stage * kStageBytes + a * 1024);
+      copy_row_pair(row + (chunk ^ ((key & 3) << 6)), v_dst + stage * kStageBytes + a * 1024);
     };
 
     // ---- before the first tile ------------------------------------------------------
-    // Copies go out in groups: group g is K of tile g, V of tile g - 1 and the table
-    // entries of tile g + kStages. Groups 0 .. kStages - 2 go out here, group t +
-    // kStages - 1 in iteration t, which needs groups 0 .. t; its tile's rows were
-    // resolved in the iteration before.
-    int32_t page[kStages];
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) page[i] = *page_entry(i);
+    // Iteration t copies K of tile t + kStages - 1 and V of t + kStages - 2; what tile 0
+    // .. kStages - 2 need goes out here. A run's table entries are copied to LDS in the
+    // first iteration of the run before, and resolved in its fifth.
+    int32_t page = *page_entry(0, lane);
     // Q^T operand: lane holds Q[row][16 s + 8 half .. + 8] of every k-step.
     u32x4v_t q[G::kSteps];
     {
@@ -289,23 +282,17 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     }
     // All of these are asked for before anything waits, and waited for before the
     // first copy: a later wait for them would wait for the copies too.
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) asm volatile("" : "+v"(page[i]));
+    asm volatile("" : "+v"(page));
 #pragma unroll
     for (int s = 0; s < G::kSteps; ++s) asm volatile("" : "+v"(q[s]));
-    Rows next = resolve(0, page[0]);  // of the next group's K
-    uint64_t next_v = 0;              // and V, a tile behind
+    resolve(0, lane, page);
 #pragma unroll
     for (int g = 0; g < kStages - 1; ++g) {
 #pragma unroll
       for (int a = 0; a < G::kCopies; ++a) {
-        copy_k(next.k, k_chunk(lane), a, g);
-        if (g > 0) copy_v(next_v, v_chunk(lane), a, g - 1);
+        copy_k(k_row(g, a, lane), k_chunk(lane), a, g);
+        if (g > 0) copy_v(v_row(g - 1, a, lane), v_chunk(lane), a, g - 1);
       }
-      copy_dwords(page_entry(g + kStages), page_dst + g * kPageStage);
-      lds.valid[g][wave] = next.valid;
-      next_v = next.v;
-      next = resolve(g + 1, page[g + 1]);
     }
 
     float m_run = -INFINITY, l_run = 0.0f;
@@ -343,24 +330,25 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
       const int stage = it & (kStages - 1);
       const int k_stage = (it + kStages - 1) & (kStages - 1);  // of tile it - 1, too
       const int v_stage = (it + kStages - 2) & (kStages - 1);
-      wait_vector<(kStages - 2) * (2 * G::kCopies + 1)>();
-      lds_barrier();  // groups 0 .. it are there; every wave is done with iteration it - 1
-      const int32_t entry = lds.pages[stage][wave][lane];
-      const uint4 vw = *reinterpret_cast<const uint4 *>(lds.valid[stage]);
-      lds.valid[k_stage][wave] = next.valid;
-      const uint32_t valid = wave_uniform(vw.x | vw.y << 8 | vw.z << 16 | vw.w << 24);
+      // Needed: K of tile it, V of the tile before. Of what was issued in the last
+      // kStages - 2 iterations nothing is, and right after a run's first iteration its
+      // entries' copy is the newest.
+      constexpr int kInFlight = (kStages - 2) * 2 * G::kCopies;
+      const int run = it / kRunTiles, run_tile = it % kRunTiles;
+      if (run_tile == 1) {
+        wait_vector<kInFlight + 1>();
+      } else {
+        wait_vector<kInFlight>();
+      }
+      lds_barrier();  // all waves' copies are there; every wave is done with iteration it - 1
+      const uint32_t valid =
+          wave_uniform(*reinterpret_cast<const int32_t *>(lds.valid[run & 1][run_tile]));
       const int32_t key0 = tile_key(it), key1 = key0 + kTile - 1;
       const bool live = wave_has_rows && it < n_tiles && key0 <= wave_qmax &&
                         (window == 0 || key1 > wave_qmin - window || key0 < sinks);
       const int copy_lane = fresh_lane();
       const uint32_t kc = k_chunk(copy_lane), vc = v_chunk(copy_lane);
-      auto copy = [&](int i) __attribute__((always_inline)) {
-        if (i % 2 == 0) {
-          copy_k(next.k, kc, i / 2, k_stage);
-        } else {
-          copy_v(next_v, vc, i / 2, v_stage);
-        }
-      };
+      const int k_tile = it + kStages - 1, v_tile = it + kStages - 2;
       f32x16_t score = f32x16_t{};
       if (live) {
         const uint32_t k_at = k_lane + stage * kStageBytes;
@@ -370,24 +358,42 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
         u32x4v_t kf[G::kWindow];
 #pragma unroll
         for (int s = 0; s < G::kWindow; ++s) kf[s] = read_k(s);
+        // Copy a of K and of V ride on products 4 a + 1 and 4 a + 3, their row addresses
+        // are read four products ahead.
+        uint64_t kr = k_row(k_tile, 0, copy_lane), vr = v_row(v_tile, 0, copy_lane);
+        uint64_t kr_next = 0, vr_next = 0;
         __builtin_amdgcn_sched_barrier(0);
         static_for<0, G::kSteps>([&](auto sc) __attribute__((always_inline)) {
-          constexpr int s = decltype(sc)::value;
+          constexpr int s = decltype(sc)::value, a = s / 4;
           score = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               __builtin_bit_cast(bf16x8_t, kf[s % G::kWindow]), __builtin_bit_cast(bf16x8_t, q[s]),
               score, 0, 0, 0);
           if constexpr (s + G::kWindow < G::kSteps) kf[s % G::kWindow] = read_k(s + G::kWindow);
-          if constexpr (s % 2 == 0) copy(s / 2);
+          if constexpr (s % 4 == 0 && a + 1 < G::kCopies) {
+            kr_next = k_row(k_tile, a + 1, copy_lane);
+            vr_next = v_row(v_tile, a + 1, copy_lane);
+          } else if constexpr (s % 4 == 1) {
+            copy_k(kr, kc, a, k_stage);
+          } else if constexpr (s % 4 == 3) {
+            copy_v(vr, vc, a, v_stage);
+            kr = kr_next;
+            vr = vr_next;
+          }
           __builtin_amdgcn_sched_barrier(0);
         });
         static_assert(G::kSteps == 4 * G::kCopies);
       } else {
 #pragma unroll
-        for (int i = 0; i < 2 * G::kCopies; ++i) copy(i);
+        for (int a = 0; a < G::kCopies; ++a) {
+          copy_k(k_row(k_tile, a, copy_lane), kc, a, k_stage);
+          copy_v(v_row(v_tile, a, copy_lane), vc, a, v_stage);
+        }
       }
-      copy_dwords(page_entry(it + 2 * kStages - 1), page_dst + k_stage * kPageStage);
-      next_v = next.v;
-      next = resolve(it + kStages, entry);
+      if (run_tile == 0) {
+        copy_dwords(page_entry(run + 1, copy_lane), page_dst);
+      } else if (run_tile == 4) {
+        resolve(run + 1, copy_lane, lds.pages[wave][copy_lane]);
+      }
       if (!live && !pending) continue;
       const bool full = live && wave_rows_full && valid == 0xFFFFFFFFu && key1 <= wave_qmin &&
                         (window == 0 || key0 > wave_qmax - window || key1 < sinks);
