@@ -62,7 +62,7 @@ struct Shape {
   static constexpr int kRowBytes = kDim * 2;
   static constexpr int kStages = kDim == 256 ? 4 : 2;
   static constexpr int kSteps = kDim / 16;              // of S^T
-  static constexpr int kDims = kDim / 32;               // 32-dim blocks of O^T
+  static constexpr int kDims = kDim / 32 / kWaves;      // 32-dim blocks of O^T per wave
   static constexpr int kCopies = kCopyKeys * kRowBytes / 1024;  // of K, and of V
   static constexpr int kTokenBytes = kHeads * kRowBytes;        // a cached token's rows
   static constexpr int kWindow = kDim == 256 ? 16 : 8;  // K fragments read ahead
@@ -80,20 +80,18 @@ __device__ __forceinline__ void static_for(F &&f) {
 
 typedef unsigned u32x4v_t __attribute__((ext_vector_type(4)));
 
-// acc += V^T P^T with the accumulators in AGPRs. The wait states cover operands
-// that a VALU instruction wrote right before (the compiler does not see into asm).
+// acc += V^T P^T with the accumulators in AGPRs. No VALU instruction writes an
+// operand within two issues before (both come from LDS reads): the compiler does not
+// see into asm and adds no wait states.
 __device__ __forceinline__ void mfma_pv(f32x16_t &acc, u32x4v_t v, u32x4v_t p) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(v), "v"(p));
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(v), "v"(p));
 }
 // Every product above has written its accumulators (16 passes and the write).
 template <int kCount>
 __device__ __forceinline__ void mfma_pv_done(f32x16_t (&acc)[kCount]) {
 #pragma unroll
-  for (int d = 0; d < kCount; d += 8) {
-    asm volatile("s_nop 15\n\ts_nop 7"
-                 : "+a"(acc[d]), "+a"(acc[d + 1]), "+a"(acc[d + 2]), "+a"(acc[d + 3]),
-                   "+a"(acc[d + 4]), "+a"(acc[d + 5]), "+a"(acc[d + 6]), "+a"(acc[d + 7]));
-  }
+  for (int d = 0; d < kCount; d += 2)
+    asm volatile("s_nop 15\n\ts_nop 7" : "+a"(acc[d]), "+a"(acc[d + 1]));
 }
 
 typedef __attribute__((address_space(3))) const u32x4v_t lds_u32x4;
@@ -104,6 +102,22 @@ __device__ __forceinline__ u32x4v_t lds_read128(uint32_t at) {
 __device__ __forceinline__ uint2 lds_read_tr(uint32_t at) {
   return __builtin_bit_cast(
       uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4 *>(at)));
+}
+
+// Two 1 KiB LDS copies (16 bytes per lane) into consecutive KiB: the second's
+// offset applies to both of its addresses and is taken back from the source.
+__device__ __forceinline__ void copy_rows2(uint64_t src0, uint64_t src1, uint32_t lds_addr) {
+  uint32_t m0_saved;
+  src1 -= 1024;
+  asm volatile(
+      "s_mov_b32 %[m0s], m0\n\t"
+      "s_mov_b32 m0, %[lds]\n\t"
+      "s_nop 0\n\t"  // SALU write of M0 -> LDS DMA reading it: one wait state (gfx9)
+      "global_load_lds_dwordx4 %[s0], off\n\t"
+      "global_load_lds_dwordx4 %[s1], off offset:1024\n\t"
+      "s_mov_b32 m0, %[m0s]"
+      : [m0s] "=&s"(m0_saved)
+      : [lds] "s"(lds_addr), [s0] "v"(src0), [s1] "v"(src1));
 }
 
 // By value: a ternary of captured variables would be a choice of addresses, and
@@ -131,6 +145,12 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     uint64_t v_rows[2][kWaves][kWave];
     uint8_t valid[2][kRunTiles][kWaves];  // bit j: key kCopyKeys w + j of the tile
     int32_t pages[kWaves][kWave];         // the next run's page-table entries
+    // What the waves trade, by the parity of the tile: their columns' weights as B
+    // operands, and the factor of the columns' sums where a maximum moved.
+    u32x4v_t weights[2][kWaves][2][kWave];
+    float alpha[2][kWaves][32];
+    uint8_t moved[2][kWaves];
+    float sums[kWaves][32];
   };
   __shared__ __attribute__((aligned(1024))) Lds lds;
 
@@ -156,23 +176,27 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
   const uint64_t zero_row = reinterpret_cast<uint64_t>(&g_zero_row[0]);
   const uint32_t kv_bytes = (uint32_t)(p.kv_stride * 2);
 
-  // Row of column n among the workgroup's, and its query head.
-  auto column_row = [&](int column) __attribute__((always_inline)) {
-    return G::kWaveRows * wave + (G::kGroup == 2 ? column % 16 : column / 16);
+  // Row, among the workgroup's, of a column of wave w, and its query head.
+  auto column_row = [&](int w, int column) __attribute__((always_inline)) {
+    return G::kWaveRows * w + (G::kGroup == 2 ? column % 16 : column / 16);
   };
   auto column_head = [&](int column) __attribute__((always_inline)) {
     return head * G::kGroup + (G::kGroup == 2 ? column / 16 : column % 16);
   };
 
-  // LDS read addresses within stage 0. K of k-step s: key n, chunk (2 s + half) ^ (n
-  // & 15): bits 1 to 3 of the chunk by XOR, the rest by offset. V^T of dim block d:
-  // lane i of 16-lane group vg reads keys 4 half + j (+ 8 r + 16 s2), dims 32 d + 16
-  // vg + 4 q (j = (lane % 16) / 4, q = lane % 4).
-  const uint32_t k_lane = lds_address(&lds.k[0][0]) + n * G::kRowBytes + ((half ^ (n & 15)) << 4);
-  const int vj = (lane & 15) >> 2, vq = lane & 3, vg = (lane >> 4) & 1;
-  const uint32_t v_lane = lds_address(&lds.v[0][0]) + (4 * half + vj) * G::kRowBytes +
-                          (((4 * vj + 2 * vg + (vq >> 1)) << 4) | ((vq & 1) << 3));  // d = 0
-
+  // LDS read addresses of lane l within stage 0. K of k-step s: key l % 32, chunk (2 s +
+  // l / 32) ^ (l & 15): bits 1 to 3 of the chunk by XOR, the rest by offset. V^T of the
+  // wave's first dim block: lane i of 16-lane group vg reads keys 4 (l / 32) + j (+ 8 r +
+  // 16 s2), dims 16 vg + 4 q (j = (l % 16) / 4, q = l % 4).
+  auto k_address = [&](int l) __attribute__((always_inline)) -> uint32_t {
+    return lds_address(&lds.k[0][0]) + (l & 31) * G::kRowBytes + (((l >> 5) ^ (l & 15)) << 4);
+  };
+  auto v_address = [&](int l) __attribute__((always_inline)) -> uint32_t {
+    const int block = G::kDims * wave, j = (l & 15) >> 2, q = l & 3, vg = (l >> 4) & 1;
+    return lds_address(&lds.v[0][0]) + (4 * (l >> 5) + j) * G::kRowBytes +
+           (((4 * ((block & 3) ^ j) + 2 * vg + (q >> 1)) << 4) | ((q & 1) << 3)) +
+           (block >> 2) * 256;
+  };
   // Source byte offsets of a copying lane before the copy's own bits: key 8 w (+ 1
   // in lanes 32 .. 63 of a copy of two keys).
   static_assert(kCopyKeys == 8);
@@ -187,6 +211,12 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
   const uint32_t k_dst = wave_uniform(lds_address(&lds.k[0][0]) + copy_row0);
   const uint32_t v_dst = wave_uniform(lds_address(&lds.v[0][0]) + copy_row0);
   const uint32_t page_dst = wave_uniform(lds_address(&lds.pages[wave][0]));
+
+  // Registers are short at 1 x 512 only.
+  auto lane_now = [&]() __attribute__((always_inline)) -> int {
+    if constexpr (kDim == 512) return fresh_lane();
+    return lane;
+  };
 
   for (; segment < segment_end; ++segment) {
     // ---- the segment ---------------------------------------------------------
@@ -254,15 +284,18 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     };
     // Lane l of a copy fills chunk l (or l % 32) of its key's row with the chunk that
     // the swizzle puts there: k_chunk and v_chunk with the key's a-dependent bits.
-    auto copy_k = [&](uint64_t row, uint32_t chunk, int a, int stage)
+    // Copies a and a + 1 go out together, from rows r0 and r1.
+    auto copy_k = [&](uint64_t r0, uint64_t r1, uint32_t chunk, int a, int stage)
         __attribute__((always_inline)) {
-      const int key = G::kRowBytes == 1024 ? a : 2 * a;
-      copy_row_pair(row + (chunk ^ ((key & 15) << 4)), k_dst + stage * kStageBytes + a * 1024);
+      const int key = G::kRowBytes == 1024 ? a : 2 * a, step = G::kRowBytes == 1024 ? 1 : 2;
+      copy_rows2(r0 + (chunk ^ ((key & 15) << 4)), r1 + (chunk ^ (((key + step) & 15) << 4)),
+                 k_dst + stage * kStageBytes + a * 1024);
     };
-    auto copy_v = [&](uint64_t row, uint32_t chunk, int a, int stage)
+    auto copy_v = [&](uint64_t r0, uint64_t r1, uint32_t chunk, int a, int stage)
         __attribute__((always_inline)) {
-      const int key = G::kRowBytes == 1024 ? a : 2 * a;
-      copy_row_pair(row + (chunk ^ ((key & 3) << 6)), v_dst + stage * kStageBytes + a * 1024);
+      const int key = G::kRowBytes == 1024 ? a : 2 * a, step = G::kRowBytes == 1024 ? 1 : 2;
+      copy_rows2(r0 + (chunk ^ ((key & 3) << 6)), r1 + (chunk ^ (((key + step) & 3) << 6)),
+                 v_dst + stage * kStageBytes + a * 1024);
     };
 
     // ---- before the first tile ------------------------------------------------------
@@ -273,7 +306,7 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     // Q^T operand: lane holds Q[row][16 s + 8 half .. + 8] of every k-step.
     u32x4v_t q[G::kSteps];
     {
-      const int row = column_row(n);  // past the last one: any row, not stored
+      const int row = column_row(wave, n);  // past the last one: any row, not stored
       const int64_t from = (int64_t)base + row0 + (row < rows ? row : 0);
       const uint16_t *q_row = p.q + from * p.q_stride + column_head(n) * kDim + 8 * half;
 #pragma unroll
@@ -286,115 +319,135 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
 #pragma unroll
     for (int s = 0; s < G::kSteps; ++s) asm volatile("" : "+v"(q[s]));
     resolve(0, lane, page);
+    // Iteration 0 multiplies a tile -1 of zero weights and zero rows.
+    lds.weights[1][wave][0][lane] = lds.weights[1][wave][1][lane] = u32x4v_t{0, 0, 0, 0};
+#pragma unroll
+    for (int a = 0; a < G::kCopies; a += 2) copy_v(zero_row, zero_row, v_chunk(lane), a, kStages - 1);
 #pragma unroll
     for (int g = 0; g < kStages - 1; ++g) {
 #pragma unroll
-      for (int a = 0; a < G::kCopies; ++a) {
-        copy_k(k_row(g, a, lane), k_chunk(lane), a, g);
-        if (g > 0) copy_v(v_row(g - 1, a, lane), v_chunk(lane), a, g - 1);
+      for (int a = 0; a < G::kCopies; a += 2) {
+        copy_k(k_row(g, a, lane), k_row(g, a + 1, lane), k_chunk(lane), a, g);
+        if (g > 0)
+          copy_v(v_row(g - 1, a, lane), v_row(g - 1, a + 1, lane), v_chunk(lane), a, g - 1);
       }
     }
 
+    // The segment with its columns in kGroups groups: all four waves' of them, or one
+    // wave's where its rows are that few; then only the first wave scores, and all four
+    // still share the second product by dims.
+    auto attend = [&](auto groups) __attribute__((always_inline)) {
+    constexpr int kGroups = decltype(groups)::value;
     float m_run = -INFINITY, l_run = 0.0f;
-    f32x16_t acc[G::kDims];
+    bool started = false;  // whether this wave's columns have had weights
+    // O^T of the wave's dims for all columns: group c, the columns of wave c.
+    f32x16_t acc[kGroups * G::kDims];
 #pragma unroll
-    for (int d = 0; d < G::kDims; ++d) acc[d] = f32x16_t{};
-    u32x4v_t weights[2];    // P^T of the tile before, 16 keys each
-    bool pending = false;   // whether it still has to meet V
-    bool started = false;   // whether the accumulators hold anything
+    for (int i = 0; i < kGroups * G::kDims; ++i) acc[i] = f32x16_t{};
 
-    // The second product of a tile in `stage`; beside(j) rides on product j.
-    auto multiply_v = [&](int stage, auto &&beside) __attribute__((always_inline)) {
-      uint32_t base_at = v_lane + stage * kStageBytes;
-      asm volatile("" : "+v"(base_at));  // the four offsets below are not kept either
-      auto read_v = [&](int j) __attribute__((always_inline)) -> u32x4v_t {
-        const int d = j % G::kDims, s2 = j / G::kDims;
-        const uint32_t at = (base_at ^ ((d & 3) << 6)) + 16 * s2 * G::kRowBytes + (d >> 2) * 256;
-        const uint2 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * G::kRowBytes);
-        return u32x4v_t{lo.x, lo.y, hi.x, hi.y};
-      };
-      constexpr int kProducts = 2 * G::kDims, kAhead = 4;
-      u32x4v_t v[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) v[j] = read_v(j);
-      static_for<0, kProducts>([&](auto jc) __attribute__((always_inline)) {
-        constexpr int j = decltype(jc)::value;
-        mfma_pv(acc[j % G::kDims], v[j % kAhead], weights[j / G::kDims]);
-        if constexpr (j + kAhead < kProducts) v[j % kAhead] = read_v(j + kAhead);
-        beside(jc);
-        __builtin_amdgcn_sched_barrier(0);
-      });
+    // V^T operand i = kDims s2 + d of the tile at v_at; weights of group c, 16 keys s2.
+    constexpr int kOperands = 2 * G::kDims, kRing = 3;
+    u32x4v_t v[kRing], w[kGroups];
+    auto read_v = [&](uint32_t v_at, int i) __attribute__((always_inline)) {
+      const int d = i % G::kDims, s2 = i / G::kDims;
+      const uint32_t at = (v_at ^ (d << 6)) + 16 * s2 * G::kRowBytes;
+      const uint2 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * G::kRowBytes);
+      v[i % kRing] = u32x4v_t{lo.x, lo.y, hi.x, hi.y};
     };
+    auto read_w = [&](int from, int c, int s2, int l) __attribute__((always_inline)) {
+      w[c] = lds.weights[from][c][s2][l];
+    };
+
+    // Before iteration it: K of its tile, V of the tile before. Of what was issued in
+    // the last kStages - 2 iterations nothing is needed, and right after a run's first
+    // iteration its entries' copy is the newest.
+    constexpr int kInFlight = (kStages - 2) * 2 * G::kCopies;
+    wait_vector<kInFlight>();
+    lds_barrier();
+    // The first K fragments of a tile are asked for right behind its barrier, with
+    // the word that says which of its keys can be read.
+    u32x4v_t kf[G::kWindow];
+    int32_t valid_word;
+    auto read_k = [&](uint32_t k_at, int s) __attribute__((always_inline)) {
+      kf[s % G::kWindow] = lds_read128((k_at ^ ((s & 7) << 5)) + (s >> 3) * 256);
+    };
+    auto read_first = [&](int tile, uint32_t k_at) __attribute__((always_inline)) {
+      valid_word = *reinterpret_cast<const int32_t *>(
+          lds.valid[tile / kRunTiles & 1][tile % kRunTiles]);
+#pragma unroll
+      for (int s = 0; s < G::kWindow; ++s) read_k(k_at, s);
+    };
+    uint32_t k_at = k_address(lane_now());  // of the tile's stage
+    read_first(0, k_at);
     // One iteration more than tiles, for the last tile's second product.
     for (int it = 0; it <= n_tiles; ++it) {
-      const int stage = it & (kStages - 1);
       const int k_stage = (it + kStages - 1) & (kStages - 1);  // of tile it - 1, too
       const int v_stage = (it + kStages - 2) & (kStages - 1);
-      // Needed: K of tile it, V of the tile before. Of what was issued in the last
-      // kStages - 2 iterations nothing is, and right after a run's first iteration its
-      // entries' copy is the newest.
-      constexpr int kInFlight = (kStages - 2) * 2 * G::kCopies;
       const int run = it / kRunTiles, run_tile = it % kRunTiles;
-      if (run_tile == 1) {
-        wait_vector<kInFlight + 1>();
-      } else {
-        wait_vector<kInFlight>();
-      }
-      lds_barrier();  // all waves' copies are there; every wave is done with iteration it - 1
-      const uint32_t valid =
-          wave_uniform(*reinterpret_cast<const int32_t *>(lds.valid[run & 1][run_tile]));
       const int32_t key0 = tile_key(it), key1 = key0 + kTile - 1;
       const bool live = wave_has_rows && it < n_tiles && key0 <= wave_qmax &&
                         (window == 0 || key1 > wave_qmin - window || key0 < sinks);
-      const int copy_lane = fresh_lane();
-      const uint32_t kc = k_chunk(copy_lane), vc = v_chunk(copy_lane);
       const int k_tile = it + kStages - 1, v_tile = it + kStages - 2;
+      const int parity = it & 1;
       f32x16_t score = f32x16_t{};
       if (live) {
-        const uint32_t k_at = k_lane + stage * kStageBytes;
-        auto read_k = [&](int s) __attribute__((always_inline)) {
-          return lds_read128((k_at ^ ((s & 7) << 5)) + (s >> 3) * 256);
-        };
-        u32x4v_t kf[G::kWindow];
-#pragma unroll
-        for (int s = 0; s < G::kWindow; ++s) kf[s] = read_k(s);
-        // Copy a of K and of V ride on products 4 a + 1 and 4 a + 3, their row addresses
-        // are read four products ahead.
-        uint64_t kr = k_row(k_tile, 0, copy_lane), vr = v_row(v_tile, 0, copy_lane);
-        uint64_t kr_next = 0, vr_next = 0;
-        __builtin_amdgcn_sched_barrier(0);
+        // Copies a and a + 1 of K ride on product 4 a + 3, of V on 4 a + 7; their row
+        // addresses are read three products ahead.
+        uint64_t r0 = 0, r1 = 0;
+        int l = 0;
+        uint32_t kc = 0, vc = 0, v_at = 0;
         static_for<0, G::kSteps>([&](auto sc) __attribute__((always_inline)) {
           constexpr int s = decltype(sc)::value, a = s / 4;
           score = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               __builtin_bit_cast(bf16x8_t, kf[s % G::kWindow]), __builtin_bit_cast(bf16x8_t, q[s]),
               score, 0, 0, 0);
-          if constexpr (s + G::kWindow < G::kSteps) kf[s % G::kWindow] = read_k(s + G::kWindow);
-          if constexpr (s % 4 == 0 && a + 1 < G::kCopies) {
-            kr_next = k_row(k_tile, a + 1, copy_lane);
-            vr_next = v_row(v_tile, a + 1, copy_lane);
-          } else if constexpr (s % 4 == 1) {
-            copy_k(kr, kc, a, k_stage);
-          } else if constexpr (s % 4 == 3) {
-            copy_v(vr, vc, a, v_stage);
-            kr = kr_next;
-            vr = vr_next;
+          if constexpr (s + G::kWindow < G::kSteps) read_k(k_at, s + G::kWindow);
+          if constexpr (s == 0) l = lane_now();
+          if constexpr (s == 1) kc = k_chunk(l);
+          if constexpr (s == 5) vc = v_chunk(l);
+          if constexpr (s == 6) v_at = v_address(l) + k_stage * kStageBytes;  // V of tile it - 1
+          // The first operands of the second product that follows.
+          constexpr int ahead = s - (G::kSteps - kGroups - kRing + 1);
+          if constexpr (ahead >= 0 && ahead < kGroups) {
+            read_w(parity ^ 1, ahead, 0, l);
+          } else if constexpr (ahead >= kGroups) {
+            read_v(v_at, ahead - kGroups);
+          }
+          if constexpr (s % 8 == 0) {
+            r0 = k_row(k_tile, a, l);
+            r1 = k_row(k_tile, a + 1, l);
+          } else if constexpr (s % 8 == 3) {
+            copy_k(r0, r1, kc, a, k_stage);
+          } else if constexpr (s % 8 == 4) {
+            r0 = v_row(v_tile, a - 1, l);
+            r1 = v_row(v_tile, a, l);
+          } else if constexpr (s % 8 == 7) {
+            copy_v(r0, r1, vc, a - 1, v_stage);
           }
           __builtin_amdgcn_sched_barrier(0);
         });
         static_assert(G::kSteps == 4 * G::kCopies);
       } else {
+        const int l = lane_now();
 #pragma unroll
-        for (int a = 0; a < G::kCopies; ++a) {
-          copy_k(k_row(k_tile, a, copy_lane), kc, a, k_stage);
-          copy_v(v_row(v_tile, a, copy_lane), vc, a, v_stage);
+        for (int a = 0; a < G::kCopies; a += 2) {
+          copy_k(k_row(k_tile, a, l), k_row(k_tile, a + 1, l), k_chunk(l), a, k_stage);
+          copy_v(v_row(v_tile, a, l), v_row(v_tile, a + 1, l), v_chunk(l), a, v_stage);
         }
+#pragma unroll
+        for (int c = 0; c < kGroups; ++c) read_w(parity ^ 1, c, 0, l);
+#pragma unroll
+        for (int i = 0; i < kRing - 1; ++i) read_v(v_address(l) + k_stage * kStageBytes, i);
       }
+      const int copy_lane = lane_now();
+      const uint32_t v_at = v_address(copy_lane) + k_stage * kStageBytes;
       if (run_tile == 0) {
         copy_dwords(page_entry(run + 1, copy_lane), page_dst);
       } else if (run_tile == 4) {
         resolve(run + 1, copy_lane, lds.pages[wave][copy_lane]);
       }
-      if (!live && !pending) continue;
+
+      const uint32_t valid = wave_uniform(valid_word);
       const bool full = live && wave_rows_full && valid == 0xFFFFFFFFu && key1 <= wave_qmin &&
                         (window == 0 || key0 > wave_qmax - window || key1 < sinks);
       // Lane holds keys (i / 4) * 8 + 4 half + i % 4 of column n.
@@ -402,7 +455,7 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
         auto below = [](int32_t count) -> uint32_t {  // keys 0 .. count - 1 of the block
           return count <= 0 ? 0u : (count >= 32 ? 0xFFFFFFFFu : (1u << count) - 1u);
         };
-        const int lane2 = fresh_lane(), row = column_row(lane2 & 31);
+        const int lane2 = lane_now(), row = column_row(wave, lane2 & 31);
         const int32_t qpos = first + row;
         uint32_t seen = below(qpos - key0 + 1);
         if (window > 0) seen &= ~below(qpos - window + 1 - key0) | below(sinks - key0);
@@ -412,9 +465,9 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
           score[i] = (seen >> ((i / 4) * 8 + i % 4)) & 1u ? score[i] : -INFINITY;
       }
 
-      // ---- softmax, under the second product of the tile before ------------------------
+      // ---- sums of tile it - 1, and under them the softmax of tile it -------------------
       float top, alpha, m_use;
-      bool moved;
+      bool moved = false;
       uint32_t pw[8];
       auto softmax = [&](auto uc) __attribute__((always_inline)) {
         constexpr int u = decltype(uc)::value;
@@ -444,54 +497,113 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
           l_run += p0 + p1;
           // P is the product's operand: bf16, half a step (2^-8) of each weight.
           pw[i / 2] = cvt_pk_bf16(p0, p1);
+        } else if constexpr (u == 12) {
+          if (kGroups == kWaves || wave == 0) {
+            lds.weights[parity][wave][0][copy_lane] = u32x4v_t{pw[0], pw[1], pw[2], pw[3]};
+            lds.weights[parity][wave][1][copy_lane] = u32x4v_t{pw[4], pw[5], pw[6], pw[7]};
+            lds.alpha[parity][wave][copy_lane & 31] = alpha;
+          }
+          // The first weights meet sums that are zero: no factor.
+          lds.moved[parity][wave] = moved && started ? 1 : 0;
+          started = started || moved;
+          asm volatile("" : "+v"(l_run));  // its additions stay under the products
         }
       };
-      if (pending) {
-        multiply_v(k_stage, [&](auto jc) __attribute__((always_inline)) {
-          constexpr int j = decltype(jc)::value, kPer = G::kDims / 8;
-          if constexpr (j % kPer == 0) softmax(std::integral_constant<int, j / kPer>{});
-        });
-        started = true;
+      // Product j: operand i = j / kGroups, group j % kGroups.
+      constexpr int kUnits = 13, kProducts = kGroups * kOperands;
+      constexpr int kPerUnit = kProducts >= 16 ? kProducts / 16 : 1;
+      static_for<0, kProducts>([&](auto jc) __attribute__((always_inline)) {
+        constexpr int j = decltype(jc)::value, i = j / kGroups, c = j % kGroups;
+        mfma_pv(acc[c * G::kDims + i % G::kDims], v[i % kRing], w[c]);
+        if constexpr (c == 0 && i + kRing - 1 < kOperands) read_v(v_at, i + kRing - 1);
+        if constexpr (i == G::kDims - 1) read_w(parity ^ 1, c, 1, copy_lane);
+        if constexpr (j % kPerUnit == 0 && j / kPerUnit < kUnits)
+          softmax(std::integral_constant<int, j / kPerUnit>{});
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      static_for<(kProducts + kPerUnit - 1) / kPerUnit, kUnits>(softmax);
+
+      k_at = k_address(copy_lane) + ((it + 1) & (kStages - 1)) * kStageBytes;
+      if (run_tile == 0) {
+        wait_vector<kInFlight + 1>();
       } else {
-        static_for<0, 12>(softmax);
+        wait_vector<kInFlight>();
       }
-      if (moved && started) {
+      lds_barrier();  // all waves' copies and weights are there; all are done with iteration it
+      const int32_t moved_word = *reinterpret_cast<const int32_t *>(lds.moved[parity]);
+      read_first(it + 1, k_at);
+      const uint32_t moves = wave_uniform(moved_word);
+      if (moves != 0) {
         mfma_pv_done(acc);
+        static_for<0, kGroups>([&](auto cc) __attribute__((always_inline)) {
+          constexpr int c = decltype(cc)::value;
+          const float own = lds.alpha[parity][c][lane_now() & 31];
+          const float factor = moves >> (8 * c) & 1 ? own : 1.0f;
 #pragma unroll
-        for (int d = 0; d < G::kDims; ++d) acc[d] *= alpha;
+          for (int d = 0; d < G::kDims; ++d) {
+            acc[c * G::kDims + d] *= factor;
+            asm volatile("" : "+a"(acc[c * G::kDims + d]));  // one at a time through VGPRs
+          }
+        });
+        mfma_pv_done(acc);
       }
-      weights[0] = u32x4v_t{pw[0], pw[1], pw[2], pw[3]};
-      weights[1] = u32x4v_t{pw[4], pw[5], pw[6], pw[7]};
-      pending = live;
+      // Pinned to AGPRs here too: the register allocator otherwise moves all sums to
+      // VGPRs and back in every iteration, for the sake of the path above.
+#pragma unroll
+      for (int i = 0; i < kGroups * G::kDims; ++i) asm volatile("" : "+a"(acc[i]));
     }
     wait_copies();
     mfma_pv_done(acc);
 
     // ---- the rows' end ---------------------------------------------------------------
+    const int end_lane = fresh_lane(), column = end_lane & 31, end_half = end_lane >> 5;
     l_run = xor_sum<32>(l_run);
-    const int end_lane = fresh_lane(), end_half = end_lane >> 5;
-    const int row = column_row(end_lane & 31), qh = column_head(end_lane & 31);
-    // Lane holds dims 32 d + 8 i + 4 half .. + 3 of its column in accumulators 4 i .. + 3.
-    if (row < rows && partial < 0) {
-      const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-      uint16_t *o = p.out + (((int64_t)base + row0 + row) * kQueryHeads + qh) * kDim + 4 * end_half;
+    if (end_half == 0) {
+      lds.sums[wave][column] = l_run;
+      const int row = column_row(wave, column);
+      if (partial >= 0 && row < rows) {
+        const int64_t at = (int64_t)(partial + row) * kQueryHeads + column_head(column);
+        *reinterpret_cast<float2 *>(p.stats + 2 * at) = make_float2(m_run, l_run);
+      }
+    }
+    __syncthreads();
+    // Lane holds dims 32 (kDims w + d) + 8 i + 4 half .. + 3 of group c's column in
+    // accumulators 4 i .. + 3.
+    const int dim0 = 32 * G::kDims * wave + 4 * end_half, qh = column_head(column);
+    static_for<0, kGroups>([&](auto cc) __attribute__((always_inline)) {
+      constexpr int c = decltype(cc)::value;
+      const int row = column_row(c, column);
+      if (row >= rows) return;
+      if (partial < 0) {
+        const float sum = lds.sums[c][column];
+        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        uint16_t *o = p.out + (((int64_t)base + row0 + row) * kQueryHeads + qh) * kDim + dim0;
 #pragma unroll
-      for (int d = 0; d < G::kDims; ++d)
+        for (int d = 0; d < G::kDims; ++d) {
+          const f32x16_t &x = acc[c * G::kDims + d];
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *reinterpret_cast<uint2 *>(o + 32 * d + 2 * i) =
-              make_uint2(cvt_pk_bf16(acc[d][i] * inv, acc[d][i + 1] * inv),
-                         cvt_pk_bf16(acc[d][i + 2] * inv, acc[d][i + 3] * inv));
-    } else if (row < rows) {
-      const int64_t at = (int64_t)(partial + row) * kQueryHeads + qh;
-      float *o = p.partial + at * kDim + 4 * end_half;
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint2 *>(o + 32 * d + 2 * i) =
+                make_uint2(cvt_pk_bf16(x[i] * inv, x[i + 1] * inv),
+                           cvt_pk_bf16(x[i + 2] * inv, x[i + 3] * inv));
+        }
+      } else {
+        float *o = p.partial + ((int64_t)(partial + row) * kQueryHeads + qh) * kDim + dim0;
 #pragma unroll
-      for (int d = 0; d < G::kDims; ++d)
+        for (int d = 0; d < G::kDims; ++d) {
+          const f32x16_t &x = acc[c * G::kDims + d];
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *reinterpret_cast<float4 *>(o + 32 * d + 2 * i) =
-              make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
-      if (end_half == 0) *reinterpret_cast<float2 *>(p.stats + 2 * at) = make_float2(m_run, l_run);
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4 *>(o + 32 * d + 2 * i) =
+                make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        }
+      }
+    });
+    };
+    if (rows <= G::kWaveRows) {
+      attend(std::integral_constant<int, 1>{});
+    } else {
+      attend(std::integral_constant<int, kWaves>{});
     }
     __syncthreads();  // the next segment's copies overwrite the stages
   }
