@@ -16,7 +16,7 @@ constexpr int kPlanWaves = kPlanThreads / kWave;
 
 struct PlanParams {
   char *plan;
-  int32_t share_first, segments, merges;
+  int32_t shares, segments, merges;
   const int32_t *row_offsets;
   const int32_t *prior_lengths;
   ExtendGeometry g;
@@ -53,7 +53,8 @@ __device__ __forceinline__ T block_prefix(T x, T &total, T *waves, F f) {
   return wave > 0 ? f(head, x) : x;
 }
 
-constexpr int kBlockCost = 1;  // of a row block besides its tiles: queries, end of the rows
+constexpr int kPlanShares = 256;
+constexpr int kBlockCost = 3;  // of a row block besides its tiles: the first keys' way, queries, the rows' end
 constexpr int kShareCost = 2;  // least cost worth a workgroup
 
 // One workgroup. The row blocks laid end to end, each at the cost of its tiles
@@ -63,10 +64,11 @@ constexpr int kShareCost = 2;  // least cost worth a workgroup
 __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p) {
   __shared__ int32_t s_begin[kExtendBatch + 1];   // first row of a sequence
   __shared__ int32_t s_blocks[kExtendBatch + 1];  // row blocks before it
+  __shared__ int32_t s_share[kPlanShares + 1];    // first segment of a share
   __shared__ int64_t s_waves[kPlanWaves];
   __shared__ int32_t s_waves32[kPlanWaves];
   const int t = threadIdx.x;
-  auto *share_first = reinterpret_cast<int32_t *>(p.plan + p.share_first);
+  auto *shares_at = reinterpret_cast<ExtendShare *>(p.plan + p.shares);
   auto *segments = reinterpret_cast<ExtendSegment *>(p.plan + p.segments);
   auto *merges = reinterpret_cast<ExtendMerge *>(p.plan + p.merges);
 
@@ -164,9 +166,10 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
         last = tile;
       }
     });
+    const int32_t stride = extend_partial_rows(p.g, r.rows);
     // Three counts in one word: partial rows stay below 2^16, merged ones too.
     const int64_t own = (int64_t)parts << 32 |
-                        (parts > 1 ? (int64_t)(parts * r.rows) << 16 | r.rows : (int64_t)0);
+                        (parts > 1 ? (int64_t)(parts * stride) << 16 | stride : (int64_t)0);
     int64_t sums;
     const int64_t at = counts + block_prefix(own, sums, s_waves, Sum()) - own;
     counts += sums;
@@ -176,7 +179,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     last = 0;
     auto emit = [&](int32_t lo, int32_t hi) {
       segments[segment + part] = {r.row0, r.rows, s_begin[r.sequence], r.prior, r.sequence, lo, hi,
-                                  parts > 1 ? partial + part * r.rows : -1};
+                                  parts > 1 ? partial + part * stride : -1};
     };
     for_cuts([&](int32_t k, int32_t tile) {
       if (tile > last && tile < r.tiles) {
@@ -184,18 +187,24 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
         ++part;
         last = tile;
       }
-      share_first[k] = segment + part + (tile >= r.tiles ? 1 : 0);
+      s_share[k] = segment + part + (tile >= r.tiles ? 1 : 0);
     });
     if (r.rows > 0) emit(last, r.tiles);
     if (parts > 1) {
-      for (int32_t i = 0; i < r.rows; ++i)
-        merges[merge + i] = {s_begin[r.sequence] + r.row0 + i, partial + i, parts, r.rows};
+      for (int32_t i = 0; i < stride; ++i)
+        merges[merge + i] = {s_begin[r.sequence] + r.row0, r.rows, partial, parts, stride, i, {}};
     }
   }
   const int32_t n_segments = (int32_t)(counts >> 32);
-  if (t == 0) share_first[0] = 0;
-  for (int32_t k = max(shares, 1) + t; k <= p.g.shares; k += kPlanThreads)
-    share_first[k] = n_segments;
+  if (t == 0) s_share[0] = 0;
+  for (int32_t k = max(shares, 1) + t; k <= p.g.shares; k += kPlanThreads) s_share[k] = n_segments;
+  __threadfence_block();
+  __syncthreads();
+  for (int32_t k = t; k < p.g.shares; k += kPlanThreads) {
+    ExtendShare s = {s_share[k], s_share[k + 1], {}, {}};
+    if (s.first < s.end) s.segment = segments[s.first];
+    shares_at[k] = s;
+  }
   if (t == 0) {
     *reinterpret_cast<ExtendHeader *>(p.plan) = {
         kExtendMagic, p.batch, p.total_rows, p.heads, p.window, p.sinks, p.page_size, n_segments,
@@ -204,10 +213,10 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
 }
 
 // ---- merge ----------------------------------------------------------------------
-// Item: (merged row, query head, 256 dims), lane l holding dims 4 l .. + 3. A row of
-// few parts is one wave's, kMergeBatch parts' loads at a time; of many, the four
-// waves' of a workgroup, each a quarter of the parts. Parts are folded in a fixed
-// order either way.
+// Item: 1 KiB of partial sums (256 fp32, four to a lane) and the parts of a split row
+// block that have them. A block of few parts is one wave's, kMergeBatch parts' loads
+// at a time; of many, the four waves' of a workgroup, each a quarter of the parts.
+// Parts are folded in a fixed order either way.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeWaves = kMergeThreads / kWave;
 constexpr int kMergeGrid = 2048;
@@ -233,61 +242,99 @@ struct MergeState {
 
 template <int kDim>
 __global__ __launch_bounds__(kMergeThreads) void extend_merge_kernel(ExtendParams p) {
-  if (!extend_plan_fits(p)) return;
   __shared__ float4 s_acc[kMergeWaves][kWave];
-  __shared__ float2 s_stats[kMergeWaves];
-  constexpr int kSlices = kDim / 256, kRowItems = kQueryHeads * kSlices;
-  const auto *h = reinterpret_cast<const ExtendHeader *>(p.plan);
-  const auto *merges = reinterpret_cast<const ExtendMerge *>(p.plan + p.merges);
+  __shared__ float2 s_stats[kMergeWaves][kWave];
+  constexpr ExtendGeometry kG = kDim == 256 ? kExtend256 : kExtend512;
+  constexpr int kHeads = kDim == 256 ? 8 : 1, kGroup = kQueryHeads / kHeads;
+  constexpr int kRowItems = kQueryHeads * kDim / 256;  // items of a partial row
+  constexpr int kWaveDims = kDim / 4;                  // dims of a wave in the rows' kernel
   const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
-  const int32_t items = h->merges * kRowItems;
+  auto merge_of = [&](int32_t item) {
+    return plan_read<ExtendMerge>(p.plan + p.merges + (int64_t)(item / kRowItems) * sizeof(ExtendMerge));
+  };
+  const int32_t first_item = wave_uniform(blockIdx.x * kMergeWaves + wave);
+  // Asked for together with the header: within the plan whatever that says.
+  ExtendMerge r = merge_of(min(first_item, max(p.max_merges, 1) * kRowItems - 1));
+  const ExtendHeader h = plan_read<ExtendHeader>(p.plan);
+  if (!extend_plan_fits(p, h)) return;
+  const int32_t items = h.merges * kRowItems;
+
+  // Where an item's values are: this lane's in the first part's sums and stats, and in
+  // the output (row -1: a column without a row).
+  struct Place {
+    int64_t sum, stat, out;
+  };
+  auto place = [&](const ExtendMerge &m, int32_t item) {
+    const int32_t chunk = m.index * kRowItems + item % kRowItems;
+    Place at;
+    int32_t row, head, dim;
+    if (m.rows <= kG.wave_rows) {
+      row = m.index;
+      head = chunk % kRowItems / (kDim / 256);
+      dim = chunk % (kDim / 256) * 256 + 4 * lane;
+      at.stat = (int64_t)(m.partial + row) * kQueryHeads + head;
+    } else {
+      // [KV head][group of 32 columns][wave][32 dims][8 dims][lane]
+      const int32_t per_head = m.stride * kGroup * kDim / 256;
+      const int32_t kv = chunk / per_head, i = chunk - kv * per_head;
+      const int32_t group = i / (kDim / 8), j = i % (kDim / 8), n = lane & 31;
+      row = group * kG.wave_rows + (kGroup == 2 ? n % 16 : n / 16);
+      head = kv * kGroup + (kGroup == 2 ? n / 16 : n % 16);
+      dim = j / (kWaveDims / 8) * kWaveDims + j % (kWaveDims / 8) * 8 + 4 * (lane >> 5);
+      at.stat = (int64_t)m.partial * kQueryHeads + kv * m.stride * kGroup + group * 32 + n;
+    }
+    at.sum = ((int64_t)m.partial * kRowItems + chunk) * 256 + 4 * lane;
+    at.out = row < m.rows ? ((int64_t)(m.row + row) * kQueryHeads + head) * kDim + dim : -1;
+    return at;
+  };
   // Parts first, first + step, .. of an item.
-  auto gather = [&](const ExtendMerge &r, int32_t item, int32_t first, int32_t step) {
-    const int qh = item / kSlices % kQueryHeads, d0 = item % kSlices * 256 + 4 * lane;
+  auto gather = [&](const ExtendMerge &m, const Place &at, int32_t first, int32_t step) {
     MergeState s;
-    for (int32_t i0 = first; i0 < r.parts; i0 += step * kMergeBatch) {
+    const int64_t part_stats = (int64_t)m.stride * kQueryHeads;
+    for (int32_t i0 = first; i0 < m.parts; i0 += step * kMergeBatch) {
       float2 stats[kMergeBatch];
       float4 a[kMergeBatch];
 #pragma unroll
       for (int i = 0; i < kMergeBatch; ++i) {
         const int32_t part = i0 + i * step;
-        if (part >= r.parts) break;
-        const int64_t at = ((int64_t)r.partial + (int64_t)part * r.stride) * kQueryHeads + qh;
-        stats[i] = *reinterpret_cast<const float2 *>(p.stats + 2 * at);
-        a[i] = *reinterpret_cast<const float4 *>(p.partial + at * kDim + d0);
+        if (part >= m.parts) break;
+        stats[i] = *reinterpret_cast<const float2 *>(p.stats + 2 * (at.stat + part * part_stats));
+        a[i] = *reinterpret_cast<const float4 *>(p.partial + at.sum + part * part_stats * kDim);
       }
 #pragma unroll
       for (int i = 0; i < kMergeBatch; ++i) {
-        if (i0 + i * step >= r.parts) break;
+        if (i0 + i * step >= m.parts) break;
         s.fold(stats[i].x, stats[i].y, a[i]);
       }
     }
     return s;
   };
-  auto store = [&](const ExtendMerge &r, int32_t item, const MergeState &s) {
-    const int qh = item / kSlices % kQueryHeads, d0 = item % kSlices * 256 + 4 * lane;
+  auto store = [&](const Place &at, const MergeState &s) {
+    if (at.out < 0) return;
     const float inv = s.l > 0.0f ? 1.0f / s.l : 0.0f;
-    *reinterpret_cast<uint2 *>(p.out + ((int64_t)r.row * kQueryHeads + qh) * kDim + d0) =
-        make_uint2(cvt_pk_bf16(s.acc.x * inv, s.acc.y * inv),
-                   cvt_pk_bf16(s.acc.z * inv, s.acc.w * inv));
+    *reinterpret_cast<uint2 *>(p.out + at.out) = make_uint2(
+        cvt_pk_bf16(s.acc.x * inv, s.acc.y * inv), cvt_pk_bf16(s.acc.z * inv, s.acc.w * inv));
   };
-  // Rows of few parts.
-  for (int32_t i = blockIdx.x * kMergeWaves + wave; i < items; i += gridDim.x * kMergeWaves) {
-    const ExtendMerge r = merges[i / kRowItems];
+  // Blocks of few parts.
+  for (int32_t i = first_item; i < items; i += gridDim.x * kMergeWaves) {
+    if (i != first_item) r = merge_of(i);
     if (r.parts > kMergeFew) continue;
-    store(r, i, gather(r, i, 0, 1));
+    const Place at = place(r, i);
+    store(at, gather(r, at, 0, 1));
   }
-  // Rows of many.
+  // Blocks of many.
   for (int32_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const ExtendMerge r = merges[i / kRowItems];
+    r = merge_of(i);
     if (r.parts <= kMergeFew) continue;
-    MergeState s = gather(r, i, wave, kMergeWaves);
+    const Place at = place(r, i);
+    MergeState s = gather(r, at, wave, kMergeWaves);
     s_acc[wave][lane] = s.acc;
-    if (lane == 0) s_stats[wave] = make_float2(s.m, s.l);
+    s_stats[wave][lane] = make_float2(s.m, s.l);
     __syncthreads();
     if (wave == 0) {
-      for (int w = 1; w < kMergeWaves; ++w) s.fold(s_stats[w].x, s_stats[w].y, s_acc[w][lane]);
-      store(r, i, s);
+      for (int w = 1; w < kMergeWaves; ++w)
+        s.fold(s_stats[w][lane].x, s_stats[w][lane].y, s_acc[w][lane]);
+      store(at, s);
     }
     __syncthreads();
   }
@@ -344,7 +391,7 @@ extern "C" hipError_t gemma4_flash_attention_extend_plan(
   if (plan_bytes < (size_t)l.bytes) return hipErrorInvalidValue;
   PlanParams p{};
   p.plan = static_cast<char *>(d_plan);
-  p.share_first = (int32_t)l.share_first;
+  p.shares = (int32_t)l.shares;
   p.segments = (int32_t)l.segments;
   p.merges = (int32_t)l.merges;
   p.row_offsets = d_row_offsets;
@@ -404,9 +451,10 @@ extern "C" hipError_t gemma4_flash_attention_extend_paged_bf16(
   p.cache_v = reinterpret_cast<const uint16_t *>(d_cache_v);
   p.page_table = d_page_table;
   p.plan = static_cast<const char *>(d_plan);
-  p.share_first = (int32_t)l.share_first;
+  p.shares = (int32_t)l.shares;
   p.segments = (int32_t)l.segments;
   p.merges = (int32_t)l.merges;
+  p.max_merges = (int32_t)l.max_merges;
   p.c = config;
   p.page_div = make_fast_div(config.page_size);
   p.slot_div = make_fast_div(config.max_pages_per_seq);

@@ -12,12 +12,13 @@ namespace gemma4 {
 // attends together; its keys come in tiles. A share (one workgroup's work) is a
 // run of segments, each a row block's tiles [tile_lo, tile_hi).
 struct ExtendGeometry {
-  int32_t rows;     // rows of a row block
-  int32_t tile;     // keys of a tile
-  int32_t shares;   // workgroups per KV head: heads x shares fill the chip
+  int32_t rows;      // rows of a row block
+  int32_t wave_rows; // of a wave's columns
+  int32_t tile;      // keys of a tile
+  int32_t shares;    // workgroups per KV head: heads x shares fill the chip
 };
-constexpr ExtendGeometry kExtend256 = {64, 32, 32};
-constexpr ExtendGeometry kExtend512 = {8, 32, 256};
+constexpr ExtendGeometry kExtend256 = {64, 16, 32, 32};
+constexpr ExtendGeometry kExtend512 = {8, 2, 32, 256};
 constexpr int kExtendBatch = 4096;  // sequences at most
 
 struct ExtendSegment {
@@ -31,13 +32,30 @@ struct ExtendSegment {
 };
 static_assert(sizeof(ExtendSegment) == 32, "two 16-byte loads");
 
-// One row of a row block that several segments share.
-struct ExtendMerge {
-  int32_t row;      // of the packed batch
-  int32_t partial;  // its row among the first segment's partial rows
-  int32_t parts;
-  int32_t stride;   // partial rows from one segment's to the next's
+// A share: its segments [first, end), and the first of them here, so that a
+// workgroup has it with one load.
+struct ExtendShare {
+  int32_t first, end, pad[2];
+  ExtendSegment segment;
 };
+
+// Partial sums of a row block that several segments share. One segment's are
+// `stride` partial rows of [16][dim] fp32. Blocks of one wave's rows at most: row,
+// query head, dim. Longer ones, as they leave the registers (rows rounded up to a
+// wave's): KV head, wave's columns, chunks of 32 columns x 8 dims.
+__host__ __device__ inline int32_t extend_partial_rows(const ExtendGeometry &g, int32_t rows) {
+  return rows <= g.wave_rows ? rows : (rows + g.wave_rows - 1) / g.wave_rows * g.wave_rows;
+}
+// One partial row of a split row block.
+struct ExtendMerge {
+  int32_t row, rows;  // the block's, of the packed batch
+  int32_t partial;    // its first segment's partial rows
+  int32_t parts;      // segments
+  int32_t stride;     // partial rows from one segment's to the next's
+  int32_t index;      // this one among them
+  int32_t pad[2];
+};
+static_assert(sizeof(ExtendMerge) == 32, "two 16-byte loads");
 
 struct ExtendHeader {
   uint32_t magic;
@@ -49,7 +67,7 @@ constexpr uint32_t kExtendMagic = 0x67345850;
 
 // Sections of the plan, by byte offset; all sizes follow from what the host knows.
 struct ExtendPlanLayout {
-  int64_t share_first, segments, merges, bytes;
+  int64_t shares, segments, merges, bytes;
   int64_t max_segments, max_merges, max_partials;
 };
 inline int64_t extend_round(int64_t n) { return (n + 255) & ~(int64_t)255; }
@@ -57,13 +75,12 @@ inline ExtendPlanLayout extend_layout(const ExtendGeometry &g, int32_t batch, in
   ExtendPlanLayout l;
   const int64_t blocks = total_rows / g.rows + (batch < total_rows ? batch : total_rows);
   l.max_segments = blocks + g.shares;
-  const int64_t block_rows = g.rows < total_rows ? g.rows : total_rows;
+  const int64_t block_rows = extend_partial_rows(g, g.rows < total_rows ? g.rows : total_rows);
   // A cut splits one row block; a block of p segments has p - 1 cuts.
   l.max_merges = (int64_t)(g.shares - 1) * block_rows;
-  if (l.max_merges > total_rows) l.max_merges = total_rows;
   l.max_partials = 2 * (int64_t)(g.shares - 1) * block_rows;
-  l.share_first = extend_round(sizeof(ExtendHeader));
-  l.segments = extend_round(l.share_first + (g.shares + 1) * 4);
+  l.shares = extend_round(sizeof(ExtendHeader));
+  l.segments = extend_round(l.shares + g.shares * (int64_t)sizeof(ExtendShare));
   l.merges = extend_round(l.segments + l.max_segments * (int64_t)sizeof(ExtendSegment));
   l.bytes = extend_round(l.merges + l.max_merges * (int64_t)sizeof(ExtendMerge));
   return l;
@@ -71,8 +88,8 @@ inline ExtendPlanLayout extend_layout(const ExtendGeometry &g, int32_t batch, in
 inline const ExtendGeometry &extend_geometry(const Gemma4KvCacheConfig &c) {
   return c.num_heads == 1 ? kExtend512 : kExtend256;
 }
-// Workspace: partial sums [partial row][16][dim] fp32, then {maximum, sum}
-// [partial row][16].
+// Workspace: the partial rows' sums, [16][dim] fp32 each, then their {maximum, sum},
+// [16] each in the same order.
 inline int64_t extend_stats_offset(const ExtendPlanLayout &l, int32_t dim) {
   return extend_round(l.max_partials * kQueryHeads * (int64_t)dim * 4);
 }
@@ -102,7 +119,8 @@ struct ExtendParams {
   const uint16_t *cache_v;
   const int32_t *page_table;
   const char *plan;
-  int32_t share_first, segments, merges;  // byte offsets in the plan
+  int32_t shares, segments, merges;  // byte offsets in the plan
+  int32_t max_merges;
   Gemma4KvCacheConfig c;
   FastDiv page_div, slot_div;
   int32_t layer, batch, total_rows;
@@ -112,11 +130,24 @@ struct ExtendParams {
   float *stats;
 };
 
+// The plan is the same for every workgroup and read through the scalar cache.
+template <class T>
+__device__ __forceinline__ T plan_read(const char *at) {
+  static_assert(sizeof(T) % 4 == 0);
+  constexpr int kWords = sizeof(T) / 4;
+  const auto *from = (const __attribute__((address_space(4))) uint32_t *)(uintptr_t)at;
+  uint32_t words[kWords];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) words[i] = from[i];
+  T x;
+  __builtin_memcpy(&x, words, sizeof(T));
+  return x;
+}
+
 // Whether the plan was made for this call's sizes.
-__device__ __forceinline__ bool extend_plan_fits(const ExtendParams &p) {
-  const auto *h = reinterpret_cast<const ExtendHeader *>(p.plan);
-  return h->magic == kExtendMagic && h->batch == p.batch && h->total_rows == p.total_rows &&
-         h->heads == p.c.num_heads && h->page_size == p.c.page_size;
+__device__ __forceinline__ bool extend_plan_fits(const ExtendParams &p, const ExtendHeader &h) {
+  return h.magic == kExtendMagic && h.batch == p.batch && h.total_rows == p.total_rows &&
+         h.heads == p.c.num_heads && h.page_size == p.c.page_size;
 }
 
 }  // namespace gemma4

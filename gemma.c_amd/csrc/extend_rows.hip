@@ -67,8 +67,10 @@ struct Shape {
   static constexpr int kTokenBytes = kHeads * kRowBytes;        // a cached token's rows
   static constexpr int kWindow = kDim == 256 ? 16 : 8;  // K fragments read ahead
 };
-static_assert(Shape<256>::kRows == kExtend256.rows && kTile == kExtend256.tile);
-static_assert(Shape<512>::kRows == kExtend512.rows && kTile == kExtend512.tile);
+static_assert(Shape<256>::kRows == kExtend256.rows && kTile == kExtend256.tile &&
+              Shape<256>::kWaveRows == kExtend256.wave_rows);
+static_assert(Shape<512>::kRows == kExtend512.rows && kTile == kExtend512.tile &&
+              Shape<512>::kWaveRows == kExtend512.wave_rows);
 
 template <int kBegin, int kEnd, class F>
 __device__ __forceinline__ void static_for(F &&f) {
@@ -157,15 +159,18 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
   const int t = threadIdx.x, lane = t & 63;
   const int wave = wave_uniform(t >> 6);
   const int half = lane >> 5, n = lane & 31;
-  const int head = blockIdx.x % G::kHeads, share = blockIdx.x / G::kHeads;
+  // Workgroups go to the eight XCDs in turn. At 8 x 256 an XCD gets a KV head; at 1 x
+  // 512 the shares in eight runs, so that a sequence's keys are read through the L2s
+  // of few XCDs (a step of ten mixed sequences 202 -> 188 us).
+  const int head = blockIdx.x % G::kHeads;
+  const int share = G::kHeads == 1 ? blockIdx.x % 8 * (kExtend512.shares / 8) + blockIdx.x / 8
+                                   : blockIdx.x / G::kHeads;
 
-  const auto *header = reinterpret_cast<const ExtendHeader *>(p.plan);
-  const auto *share_first = reinterpret_cast<const int32_t *>(p.plan + p.share_first);
-  const auto *segments = reinterpret_cast<const ExtendSegment *>(p.plan + p.segments);
-  const int32_t segment_end = share_first[share + 1];
-  int32_t segment = share_first[share];
-  const int32_t window = header->window, sinks = header->sinks;
-  if (!extend_plan_fits(p)) return;
+  const ExtendShare mine =
+      plan_read<ExtendShare>(p.plan + p.shares + (int64_t)share * sizeof(ExtendShare));
+  const ExtendHeader header = plan_read<ExtendHeader>(p.plan);
+  if (!extend_plan_fits(p, header)) return;
+  const int32_t window = header.window, sinks = header.sinks;
 
   const bool ring = p.c.window_size > 0;
   const int32_t max_pages = p.c.max_pages_per_seq;
@@ -218,9 +223,11 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     return lane;
   };
 
-  for (; segment < segment_end; ++segment) {
+  for (int32_t segment = mine.first; segment < mine.end; ++segment) {
     // ---- the segment ---------------------------------------------------------
-    const ExtendSegment seg = segments[segment];
+    ExtendSegment seg = mine.segment;
+    if (segment != mine.first)
+      seg = plan_read<ExtendSegment>(p.plan + p.segments + (int64_t)segment * sizeof(ExtendSegment));
     const int32_t row0 = seg.row0, rows = seg.rows, base = seg.base, prior = seg.prior;
     const int32_t partial = seg.partial, tile_lo = seg.tile_lo;
     const int n_tiles = seg.tile_hi - tile_lo;
@@ -302,22 +309,7 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     // Iteration t copies K of tile t + kStages - 1 and V of t + kStages - 2; what tile 0
     // .. kStages - 2 need goes out here. A run's table entries are copied to LDS in the
     // first iteration of the run before, and resolved in its fifth.
-    int32_t page = *page_entry(0, lane);
-    // Q^T operand: lane holds Q[row][16 s + 8 half .. + 8] of every k-step.
-    u32x4v_t q[G::kSteps];
-    {
-      const int row = column_row(wave, n);  // past the last one: any row, not stored
-      const int64_t from = (int64_t)base + row0 + (row < rows ? row : 0);
-      const uint16_t *q_row = p.q + from * p.q_stride + column_head(n) * kDim + 8 * half;
-#pragma unroll
-      for (int s = 0; s < G::kSteps; ++s)
-        q[s] = *reinterpret_cast<const u32x4v_t *>(q_row + 16 * s);
-    }
-    // All of these are asked for before anything waits, and waited for before the
-    // first copy: a later wait for them would wait for the copies too.
-    asm volatile("" : "+v"(page));
-#pragma unroll
-    for (int s = 0; s < G::kSteps; ++s) asm volatile("" : "+v"(q[s]));
+    const int32_t page = *page_entry(0, lane);
     resolve(0, lane, page);
     // Iteration 0 multiplies a tile -1 of zero weights and zero rows.
     lds.weights[1][wave][0][lane] = lds.weights[1][wave][1][lane] = u32x4v_t{0, 0, 0, 0};
@@ -332,6 +324,24 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
           copy_v(v_row(g - 1, a, lane), v_row(g - 1, a + 1, lane), v_chunk(lane), a, g - 1);
       }
     }
+
+    // Q^T operand: lane holds Q[row][16 s + 8 half .. + 8] of every k-step. Asked for
+    // behind the first copies, and waited for (with them) here: a wait in the loop
+    // would be one for the loop's copies.
+    u32x4v_t q[G::kSteps];
+    if (wave_has_rows) {
+      const int row = column_row(wave, n);  // past the last one: any row, not stored
+      const int64_t from = (int64_t)base + row0 + (row < rows ? row : 0);
+      const uint16_t *q_row = p.q + from * p.q_stride + column_head(n) * kDim + 8 * half;
+#pragma unroll
+      for (int s = 0; s < G::kSteps; ++s)
+        q[s] = *reinterpret_cast<const u32x4v_t *>(q_row + 16 * s);
+    } else {
+#pragma unroll
+      for (int s = 0; s < G::kSteps; ++s) q[s] = u32x4v_t{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int s = 0; s < G::kSteps; ++s) asm volatile("" : "+v"(q[s]));
 
     // The segment with its columns in kGroups groups: all four waves' of them, or one
     // wave's where its rows are that few; then only the first wave scores, and all four
@@ -558,11 +568,17 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     // ---- the rows' end ---------------------------------------------------------------
     const int end_lane = fresh_lane(), column = end_lane & 31, end_half = end_lane >> 5;
     l_run = xor_sum<32>(l_run);
+    // First of the KV head's columns in the segment's partial rows, where rows of
+    // several waves are stored as they are.
+    const int64_t wide_column =
+        (int64_t)partial * kQueryHeads +
+        head * G::kGroup * ((rows + G::kWaveRows - 1) / G::kWaveRows * G::kWaveRows);
     if (end_half == 0) {
       lds.sums[wave][column] = l_run;
       const int row = column_row(wave, column);
       if (partial >= 0 && row < rows) {
-        const int64_t at = (int64_t)(partial + row) * kQueryHeads + column_head(column);
+        const int64_t at = kGroups == 1 ? (int64_t)(partial + row) * kQueryHeads + column_head(column)
+                                        : wide_column + wave * 32 + column;
         *reinterpret_cast<float2 *>(p.stats + 2 * at) = make_float2(m_run, l_run);
       }
     }
@@ -573,8 +589,8 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     static_for<0, kGroups>([&](auto cc) __attribute__((always_inline)) {
       constexpr int c = decltype(cc)::value;
       const int row = column_row(c, column);
-      if (row >= rows) return;
       if (partial < 0) {
+        if (row >= rows) return;
         const float sum = lds.sums[c][column];
         const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
         uint16_t *o = p.out + (((int64_t)base + row0 + row) * kQueryHeads + qh) * kDim + dim0;
@@ -588,13 +604,18 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
                            cvt_pk_bf16(x[i + 2] * inv, x[i + 3] * inv));
         }
       } else {
-        float *o = p.partial + ((int64_t)(partial + row) * kQueryHeads + qh) * kDim + dim0;
+        // One wave's rows go to their places; more leave as they are, 1 KiB a store.
+        if (kGroups == 1 ? row >= rows : c * G::kWaveRows >= rows) return;
+        float *o = kGroups == 1
+                       ? p.partial + ((int64_t)(partial + row) * kQueryHeads + qh) * kDim + dim0
+                       : p.partial + wide_column * kDim +
+                             (c * kWaves + wave) * (G::kDims * 1024) + 4 * end_lane;
 #pragma unroll
         for (int d = 0; d < G::kDims; ++d) {
           const f32x16_t &x = acc[c * G::kDims + d];
 #pragma unroll
           for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4 *>(o + 32 * d + 2 * i) =
+            *reinterpret_cast<float4 *>(o + (kGroups == 1 ? 32 * d + 2 * i : 1024 * d + 64 * i)) =
                 make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
         }
       }
