@@ -54,11 +54,15 @@ __device__ __forceinline__ T block_prefix(T x, T &total, T *waves, F f) {
 }
 
 constexpr int kPlanShares = 256;
-constexpr int kBlockCost = 3;  // of a row block besides its tiles: the first keys' way, queries, the rows' end
-constexpr int kShareCost = 2;  // least cost worth a workgroup
+constexpr int kShareTiles = 2;  // least cost worth a workgroup
+// Besides its tiles a row block costs the way to its first keys, its queries and its
+// rows' end: about four tiles' time where it holds several waves' rows, three where
+// one's.
+__device__ __forceinline__ int32_t block_cost(const ExtendGeometry &g, int32_t rows) {
+  return rows > g.wave_rows ? 4 : 3;
+}
 
-// One workgroup. The row blocks laid end to end, each at the cost of its tiles
-// and kBlockCost, are cut into shares of equal cost. A cut near a block's end moves
+// One workgroup. The row blocks laid end to end are cut into shares of equal cost. A cut near a block's end moves
 // there: a split block costs its partial sums, written, read and merged (64 rows
 // about four tiles' time, few rows less).
 __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p) {
@@ -121,7 +125,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     r.prior = min(max(p.prior_lengths[lo], 0), p.max_prior);
     const int32_t first = r.prior + r.row0;
     r.tiles = extend_tiles(first, first + r.rows - 1, p.window, p.sinks, p.g.tile).count;
-    r.cost = (int64_t)r.tiles + kBlockCost;
+    r.cost = (int64_t)r.tiles + block_cost(p.g, r.rows);
     return r;
   };
   int64_t cost = 0;
@@ -131,7 +135,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     cost += all;
   }
   const int32_t shares =
-      (int32_t)min((int64_t)p.g.shares, max(cost / kShareCost, (int64_t)1));
+      (int32_t)min((int64_t)p.g.shares, max(cost / kShareTiles, (int64_t)1));
   // Cut k of 1 .. shares - 1 lies at this cost. Every thread evaluates the same
   // expression, so the blocks agree on it.
   const double step = (double)cost / (double)shares;
@@ -146,6 +150,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     const int64_t begin = end - r.cost;
     before += all;
     const int32_t snap = 1 + r.rows * 3 / p.g.rows;
+    const int32_t ahead = block_cost(p.g, r.rows);
     // f(cut k, the tile it lies at: 0 and r.tiles are no cuts of the block)
     auto for_cuts = [&](auto &&f) {
       if (r.rows == 0) return;
@@ -153,7 +158,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
       while (k > 1 && cut_at(k - 1) >= begin) --k;
       while (k < shares && cut_at(k) < begin) ++k;
       for (; k < shares && cut_at(k) < end; ++k) {
-        int32_t tile = (int32_t)max(cut_at(k) - begin - kBlockCost, (int64_t)0);
+        int32_t tile = (int32_t)max(cut_at(k) - begin - ahead, (int64_t)0);
         if (tile < snap) tile = 0;
         if (r.tiles - tile < snap) tile = r.tiles;
         f(k, tile);

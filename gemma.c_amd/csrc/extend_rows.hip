@@ -241,7 +241,6 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
 
     const int32_t wave_row0 = G::kWaveRows * wave;
     const bool wave_has_rows = wave_row0 < rows;
-    const bool wave_rows_full = wave_row0 + G::kWaveRows <= rows;
     const int32_t wave_qmin = first + wave_row0;
     const int32_t wave_qmax = min(wave_qmin + G::kWaveRows - 1, last);
 
@@ -458,7 +457,8 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
       }
 
       const uint32_t valid = wave_uniform(valid_word);
-      const bool full = live && wave_rows_full && valid == 0xFFFFFFFFu && key1 <= wave_qmin &&
+      // Columns without a row have some row's query; what they come to is not stored.
+      const bool full = live && valid == 0xFFFFFFFFu && key1 <= wave_qmin &&
                         (window == 0 || key0 > wave_qmax - window || key1 < sinks);
       // Lane holds keys (i / 4) * 8 + 4 half + i % 4 of column n.
       if (!full) {
