@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     if (r.rows > 0) emit(last, r.tiles);
     if (parts > 1) {
       for (int32_t i = 0; i < stride; ++i)
-        merges[merge + i] = {s_begin[r.sequence] + r.row0, r.rows, partial, parts, stride, i, {}};
+        merges[merge + i] = {s_begin[r.sequence] + r.row0, r.rows, partial, parts, stride, i, segment, {}};
     }
   }
   const int32_t n_segments = (int32_t)(counts >> 32);
@@ -231,6 +231,7 @@ constexpr int kMergeFew = 16;  // parts a single wave folds
 struct MergeState {
   float m = -INFINITY, l = 0.0f;
   float4 acc = {0, 0, 0, 0};
+  uint32_t odd = 0;  // of the item's 32 columns, those with sums that are not finite
   __device__ __forceinline__ void fold(float mi, float li, const float4 &a) {
     const float top = fmaxf(m, mi);
     const float fa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
@@ -245,10 +246,94 @@ struct MergeState {
   }
 };
 
+// A (row, query head) from the keys that it sees alone, by one wave, kAgainKeys at a
+// time: for columns that an infinity or NaN of V got into, which may be of a key that
+// they do not see. For those only: a wave reads about 10 GB/s.
+constexpr int kAgainKeys = 4;
 template <int kDim>
-__global__ __launch_bounds__(kMergeThreads) void extend_merge_kernel(ExtendParams p) {
+__device__ __forceinline__ void extend_again(int32_t segment, int32_t row, int32_t qh) {
+  // The kernel's argument, read here: what only this needs takes no registers elsewhere.
+  uint64_t argument = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(argument));
+  const ExtendParams p = plan_read<ExtendParams>(reinterpret_cast<const char *>(argument));
+  const ExtendHeader h = plan_read<ExtendHeader>(p.plan);
+  const ExtendSegment s =
+      plan_read<ExtendSegment>(p.plan + p.segments + (int64_t)segment * sizeof(ExtendSegment));
+  constexpr int kHeads = kDim == 256 ? 8 : 1, kPer = kDim / kWave;
+  const int lane = threadIdx.x & 63, head = qh / (kQueryHeads / kHeads);
+  const int32_t position = s.prior + row - s.base;
+  const int64_t layer = (int64_t)p.layer * p.c.num_pages * p.c.page_size;
+  typedef uint32_t Words __attribute__((ext_vector_type(kPer / 2)));  // this lane's dims
+  auto load = [&](const uint16_t *row0) {
+    return *reinterpret_cast<const Words *>(row0 + kPer * lane);
+  };
+  const Words q_words = load(p.q + row * p.q_stride + qh * kDim);
+  float o[kPer] = {}, m = -INFINITY, l = 0.0f;
+  const int32_t low = h.window > 0 ? max(position - h.window + 1, 0) : 0;
+  const int32_t sinks = min(h.sinks, low);
+  // Key i of the count = sinks + position - low + 1 that the row sees.
+  const int32_t count = sinks + position - low + 1;
+  for (int32_t i0 = 0; i0 < count; i0 += kAgainKeys) {
+    Words k[kAgainKeys], v[kAgainKeys];
+    bool ok[kAgainKeys];
+#pragma unroll
+    for (int j = 0; j < kAgainKeys; ++j) {
+      const int32_t i = min(i0 + j, count - 1), key = i < sinks ? i : low + i - sinks;
+      const uint16_t *from_k = p.k, *from_v = p.v;
+      int64_t from = 0;
+      ok[j] = i0 + j < count;
+      if (key >= s.prior) {
+        from = ((int64_t)s.base + key - s.prior) * p.kv_stride + head * kDim;
+      } else {
+        const uint32_t logical = fast_div((uint32_t)key, p.page_div);
+        const int32_t page = p.page_table[(int64_t)s.sequence * p.c.max_pages_per_seq +
+                                          fast_mod(logical, p.slot_div)];
+        if (page >= 0 && page < p.c.num_pages &&
+            (p.c.window_size > 0 || logical < (uint32_t)p.c.max_pages_per_seq)) {
+          from = ((layer + (int64_t)page * p.c.page_size + key -
+                   (int64_t)logical * p.c.page_size) * kHeads + head) * kDim;
+          from_k = p.cache_k;
+          from_v = p.cache_v;
+        } else {
+          ok[j] = false;
+        }
+      }
+      k[j] = load(from_k + from);
+      v[j] = load(from_v + from);
+    }
+#pragma unroll
+    for (int j = 0; j < kAgainKeys; ++j) {
+      if (!ok[j]) continue;
+      float x = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kPer / 2; ++e)
+        x = fmaf(bf16_lo(q_words[e]), bf16_lo(k[j][e]), fmaf(bf16_hi(q_words[e]), bf16_hi(k[j][e]), x));
+      for (int d = 1; d < kWave; d <<= 1) x += __shfl_xor(x, d);
+      x *= p.q_scale;
+      const float top = fmaxf(m, x), base = top == -INFINITY ? 0.0f : top;
+      const float a = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - base);
+      const float w = __builtin_amdgcn_exp2f(x - base);
+      l = l * a + w;
+#pragma unroll
+      for (int e = 0; e < kPer / 2; ++e) {
+        o[2 * e] = o[2 * e] * a + w * bf16_lo(v[j][e]);
+        o[2 * e + 1] = o[2 * e + 1] * a + w * bf16_hi(v[j][e]);
+      }
+      m = top;
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  Words words;
+#pragma unroll
+  for (int e = 0; e < kPer / 2; ++e) words[e] = cvt_pk_bf16(o[2 * e] * inv, o[2 * e + 1] * inv);
+  *reinterpret_cast<Words *>(p.out + ((int64_t)row * kQueryHeads + qh) * kDim + kPer * lane) = words;
+}
+
+template <int kDim>
+__global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendParams p) {
   __shared__ float4 s_acc[kMergeWaves][kWave];
   __shared__ float2 s_stats[kMergeWaves][kWave];
+  __shared__ uint32_t s_odd[kMergeWaves];
   constexpr ExtendGeometry kG = kDim == 256 ? kExtend256 : kExtend512;
   constexpr int kHeads = kDim == 256 ? 8 : 1, kGroup = kQueryHeads / kHeads;
   constexpr int kRowItems = kQueryHeads * kDim / 256;  // items of a partial row
@@ -260,14 +345,30 @@ __global__ __launch_bounds__(kMergeThreads) void extend_merge_kernel(ExtendParam
   const int32_t first_item = wave_uniform(blockIdx.x * kMergeWaves + wave);
   // Asked for together with the header: within the plan whatever that says.
   ExtendMerge r = merge_of(min(first_item, max(p.max_merges, 1) * kRowItems - 1));
+  // Marks in row blocks of one segment: a unit is a row's, four to a query head.
+  auto segment_of = [&](int32_t unit) {
+    return plan_read<ExtendSegment>(p.plan + p.segments +
+                                    (int64_t)(unit / kG.rows) * sizeof(ExtendSegment));
+  };
+  auto marks_of = [&](const ExtendSegment &s, int32_t unit) -> uint16_t {
+    if (s.partial >= 0 || unit % kG.rows >= s.rows) return 0;
+    const int64_t row = s.base + s.row0 + unit % kG.rows;
+    return p.out[(row * kQueryHeads + lane / 4) * kDim + lane % 4 * (kDim / 4)];
+  };
+  ExtendSegment seg = segment_of(min(first_item, p.max_segments * kG.rows - 1));
   const ExtendHeader h = plan_read<ExtendHeader>(p.plan);
   if (!extend_plan_fits(p, h)) return;
-  const int32_t items = h.merges * kRowItems;
+  const int32_t items = h.merges * kRowItems, units = h.segments * kG.rows;
+  uint16_t mark = first_item < units ? marks_of(seg, first_item) : 0;
 
   // Where an item's values are: this lane's in the first part's sums and stats, and in
   // the output (row -1: a column without a row).
   struct Place {
     int64_t sum, stat, out;
+    int32_t odd;   // the first part's words (all lanes' the same)
+    int32_t row, head;
+    uint32_t bit;  // this lane's column in them
+    bool again;    // this lane's item works the column out again, if need be
   };
   auto place = [&](const ExtendMerge &m, int32_t item) {
     const int32_t chunk = m.index * kRowItems + item % kRowItems;
@@ -278,6 +379,9 @@ __global__ __launch_bounds__(kMergeThreads) void extend_merge_kernel(ExtendParam
       head = chunk % kRowItems / (kDim / 256);
       dim = chunk % (kDim / 256) * 256 + 4 * lane;
       at.stat = (int64_t)(m.partial + row) * kQueryHeads + head;
+      at.odd = (m.partial * kHeads + head / kGroup) * 4;
+      at.bit = 1u << (kGroup == 2 ? head % 2 * 16 + row : row * 16 + head);
+      at.again = dim == 0;
     } else {
       // [KV head][group of 32 columns][wave][32 dims][8 dims][lane]
       const int32_t per_head = m.stride * kGroup * kDim / 256;
@@ -287,14 +391,24 @@ __global__ __launch_bounds__(kMergeThreads) void extend_merge_kernel(ExtendParam
       head = kv * kGroup + (kGroup == 2 ? n / 16 : n % 16);
       dim = j / (kWaveDims / 8) * kWaveDims + j % (kWaveDims / 8) * 8 + 4 * (lane >> 5);
       at.stat = (int64_t)m.partial * kQueryHeads + kv * m.stride * kGroup + group * 32 + n;
+      at.odd = ((m.partial + group * kG.wave_rows) * kHeads + kv) * 4;
+      at.bit = 1u << n;
+      at.again = lane == j && j < 32;
     }
     at.sum = ((int64_t)m.partial * kRowItems + chunk) * 256 + 4 * lane;
     at.out = row < m.rows ? ((int64_t)(m.row + row) * kQueryHeads + head) * kDim + dim : -1;
+    at.row = m.row + row;
+    at.head = head;
     return at;
   };
   // Parts first, first + step, .. of an item.
   auto gather = [&](const ExtendMerge &m, const Place &at, int32_t first, int32_t step) {
     MergeState s;
+    // The words of the first 16 parts, asked for with the first sums.
+    auto odd_of = [&](int32_t part) -> uint32_t {
+      return p.odd[at.odd + min(part, m.parts - 1) * m.stride * kHeads * 4 + lane % 4];
+    };
+    const uint32_t odd = odd_of(first + lane / 4 * step);
     const int64_t part_stats = (int64_t)m.stride * kQueryHeads;
     for (int32_t i0 = first; i0 < m.parts; i0 += step * kMergeBatch) {
       float2 stats[kMergeBatch];
@@ -312,20 +426,30 @@ __global__ __launch_bounds__(kMergeThreads) void extend_merge_kernel(ExtendParam
         s.fold(stats[i].x, stats[i].y, a[i]);
       }
     }
+    s.odd = odd;
+    for (int32_t part = first + (16 + lane / 4) * step; part < m.parts; part += 16 * step)
+      s.odd |= odd_of(part);
+    if (__builtin_expect(__ballot(s.odd != 0) != 0, 0))
+      for (int d = 1; d < kWave; d <<= 1) s.odd |= __shfl_xor(s.odd, d);
     return s;
   };
-  auto store = [&](const Place &at, const MergeState &s) {
-    if (at.out < 0) return;
+  auto store = [&](const Place &at, const ExtendMerge &m, const MergeState &s) {
     const float inv = s.l > 0.0f ? 1.0f / s.l : 0.0f;
-    *reinterpret_cast<uint2 *>(p.out + at.out) = make_uint2(
-        cvt_pk_bf16(s.acc.x * inv, s.acc.y * inv), cvt_pk_bf16(s.acc.z * inv, s.acc.w * inv));
+    if (at.out >= 0 && (s.odd & at.bit) == 0)
+      *reinterpret_cast<uint2 *>(p.out + at.out) = make_uint2(
+          cvt_pk_bf16(s.acc.x * inv, s.acc.y * inv), cvt_pk_bf16(s.acc.z * inv, s.acc.w * inv));
+    uint64_t again = __ballot((s.odd & at.bit) != 0 && at.out >= 0 && at.again);
+    for (; __builtin_expect(again != 0, 0); again &= again - 1) {
+      const int from = __builtin_ctzll(again);
+      extend_again<kDim>(m.segment, __shfl(at.row, from), __shfl(at.head, from));
+    }
   };
   // Blocks of few parts.
   for (int32_t i = first_item; i < items; i += gridDim.x * kMergeWaves) {
     if (i != first_item) r = merge_of(i);
     if (r.parts > kMergeFew) continue;
     const Place at = place(r, i);
-    store(at, gather(r, at, 0, 1));
+    store(at, r, gather(r, at, 0, 1));
   }
   // Blocks of many.
   for (int32_t i = blockIdx.x; i < items; i += gridDim.x) {
@@ -335,13 +459,29 @@ __global__ __launch_bounds__(kMergeThreads) void extend_merge_kernel(ExtendParam
     MergeState s = gather(r, at, wave, kMergeWaves);
     s_acc[wave][lane] = s.acc;
     s_stats[wave][lane] = make_float2(s.m, s.l);
+    if (lane == 0) s_odd[wave] = s.odd;
     __syncthreads();
     if (wave == 0) {
-      for (int w = 1; w < kMergeWaves; ++w)
+      for (int w = 1; w < kMergeWaves; ++w) {
         s.fold(s_stats[w][lane].x, s_stats[w][lane].y, s_acc[w][lane]);
-      store(at, s);
+        s.odd |= s_odd[w];
+      }
+      store(at, r, s);
     }
     __syncthreads();
+  }
+  for (int32_t i = first_item; i < units;) {
+    uint64_t marks = __ballot(mark == kExtendOdd);
+    while (__builtin_expect(marks != 0, 0)) {
+      const int qh = __builtin_ctzll(marks) / 4;
+      marks &= ~(15ull << (4 * qh));
+      extend_again<kDim>(i / kG.rows, seg.base + seg.row0 + i % kG.rows, qh);
+    }
+    i += gridDim.x * kMergeWaves;
+    if (i < units) {
+      seg = segment_of(i);
+      mark = marks_of(seg, i);
+    }
   }
 }
 
@@ -373,8 +513,8 @@ extern "C" size_t gemma4_flash_attention_extend_workspace_bytes(Gemma4KvCacheCon
                                                                 int32_t total_rows) {
   if (!valid_extend(config, batch_size, total_rows)) return 0;
   const ExtendPlanLayout l = extend_layout(extend_geometry(config), batch_size, total_rows);
-  return (size_t)(extend_stats_offset(l, config.head_dim) +
-                  extend_round(l.max_partials * kQueryHeads * 8));
+  return (size_t)(extend_odd_offset(l, config.head_dim) +
+                  extend_round(l.max_partials * config.num_heads * 16));
 }
 
 extern "C" hipError_t gemma4_flash_attention_extend_plan(
@@ -433,7 +573,7 @@ extern "C" hipError_t gemma4_flash_attention_extend_paged_bf16(
   const int64_t kv_width = (int64_t)config.num_heads * config.head_dim;
   if (q_stride == 0) q_stride = q_width;
   if (kv_stride == 0) kv_stride = kv_width;
-  const int64_t most = (int64_t)1 << 31;
+  const int64_t most = (int64_t)1 << 30;
   if (q_stride < q_width || kv_stride < kv_width || q_stride % kPackElems != 0 ||
       kv_stride % kPackElems != 0 || q_stride > most || kv_stride > most || !aligned(d_out, 16) ||
       !aligned(d_q, 16) || !aligned(d_k, 16) || !aligned(d_v, 16) || !aligned(d_cache_k, 16) ||
@@ -460,6 +600,7 @@ extern "C" hipError_t gemma4_flash_attention_extend_paged_bf16(
   p.segments = (int32_t)l.segments;
   p.merges = (int32_t)l.merges;
   p.max_merges = (int32_t)l.max_merges;
+  p.max_segments = (int32_t)l.max_segments;
   p.c = config;
   p.page_div = make_fast_div(config.page_size);
   p.slot_div = make_fast_div(config.max_pages_per_seq);
@@ -470,8 +611,9 @@ extern "C" hipError_t gemma4_flash_attention_extend_paged_bf16(
   p.kv_stride = kv_stride;
   p.q_scale = softmax_scale * kLog2e;
   p.partial = static_cast<float *>(d_workspace);
-  p.stats = reinterpret_cast<float *>(static_cast<char *>(d_workspace) +
-                                      extend_stats_offset(l, config.head_dim));
+  char *workspace = static_cast<char *>(d_workspace);
+  p.stats = reinterpret_cast<float *>(workspace + extend_stats_offset(l, config.head_dim));
+  p.odd = reinterpret_cast<uint32_t *>(workspace + extend_odd_offset(l, config.head_dim));
   const uint32_t merge_grid = (uint32_t)std::min<int64_t>(
       kMergeGrid, std::max<int64_t>(l.max_merges, 1) * kQueryHeads * (config.head_dim / 256));
   launch_extend_rows(p, stream);

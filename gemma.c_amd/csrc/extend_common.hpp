@@ -53,7 +53,8 @@ struct ExtendMerge {
   int32_t parts;      // segments
   int32_t stride;     // partial rows from one segment's to the next's
   int32_t index;      // this one among them
-  int32_t pad[2];
+  int32_t segment;    // the block's first
+  int32_t pad;
 };
 static_assert(sizeof(ExtendMerge) == 32, "two 16-byte loads");
 
@@ -63,6 +64,9 @@ struct ExtendHeader {
   int32_t segments;
   int32_t merges;
 };
+// In a (row, query head) that has to be worked out again, the first element of one of
+// its quarters: a signalling NaN, which no arithmetic gives.
+constexpr uint16_t kExtendOdd = 0x7FA5;
 constexpr uint32_t kExtendMagic = 0x67345850;
 
 // Sections of the plan, by byte offset; all sizes follow from what the host knows.
@@ -89,9 +93,14 @@ inline const ExtendGeometry &extend_geometry(const Gemma4KvCacheConfig &c) {
   return c.num_heads == 1 ? kExtend512 : kExtend256;
 }
 // Workspace: the partial rows' sums, [16][dim] fp32 each, then their {maximum, sum},
-// [16] each in the same order.
+// [16] each in the same order, then the words that tell which sums are not finite: at
+// [first partial row of a wave's columns][KV head] a bit per column from each of the
+// four waves, which have a quarter of the dims each.
 inline int64_t extend_stats_offset(const ExtendPlanLayout &l, int32_t dim) {
   return extend_round(l.max_partials * kQueryHeads * (int64_t)dim * 4);
+}
+inline int64_t extend_odd_offset(const ExtendPlanLayout &l, int32_t dim) {
+  return extend_stats_offset(l, dim) + extend_round(l.max_partials * kQueryHeads * 8);
 }
 
 // Key tiles of a row block whose rows sit at positions [first, last]: those of
@@ -120,7 +129,7 @@ struct ExtendParams {
   const int32_t *page_table;
   const char *plan;
   int32_t shares, segments, merges;  // byte offsets in the plan
-  int32_t max_merges;
+  int32_t max_merges, max_segments;
   Gemma4KvCacheConfig c;
   FastDiv page_div, slot_div;
   int32_t layer, batch, total_rows;
@@ -128,6 +137,7 @@ struct ExtendParams {
   float q_scale;          // softmax_scale * log2(e)
   float *partial;
   float *stats;
+  uint32_t *odd;
 };
 
 // The plan is the same for every workgroup and read through the scalar cache.

@@ -568,56 +568,70 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     // ---- the rows' end ---------------------------------------------------------------
     const int end_lane = fresh_lane(), column = end_lane & 31, end_half = end_lane >> 5;
     l_run = xor_sum<32>(l_run);
-    // First of the KV head's columns in the segment's partial rows, where rows of
-    // several waves are stored as they are.
-    const int64_t wide_column =
-        (int64_t)partial * kQueryHeads +
-        head * G::kGroup * ((rows + G::kWaveRows - 1) / G::kWaveRows * G::kWaveRows);
-    if (end_half == 0) {
-      lds.sums[wave][column] = l_run;
-      const int row = column_row(wave, column);
-      if (partial >= 0 && row < rows) {
-        const int64_t at = kGroups == 1 ? (int64_t)(partial + row) * kQueryHeads + column_head(column)
-                                        : wide_column + wave * 32 + column;
-        *reinterpret_cast<float2 *>(p.stats + 2 * at) = make_float2(m_run, l_run);
-      }
-    }
+    if (end_half == 0) lds.sums[wave][column] = l_run;
     __syncthreads();
     // Lane holds dims 32 (kDims w + d) + 8 i + 4 half .. + 3 of group c's column in
-    // accumulators 4 i .. + 3.
-    const int dim0 = 32 * G::kDims * wave + 4 * end_half, qh = column_head(column);
+    // accumulators 4 i .. + 3. An infinity or NaN of V meets weight 0 too in the
+    // products, in columns that do not see its key: a column whose sums are not all
+    // finite is marked by each wave that has such sums, and the merge launch works it
+    // out again from the keys that it sees.
+    const int dim0 = 32 * G::kDims * wave, qh = column_head(column);
     static_for<0, kGroups>([&](auto cc) __attribute__((always_inline)) {
       constexpr int c = decltype(cc)::value;
+      if (c * G::kWaveRows >= rows) return;
       const int row = column_row(c, column);
+      float zero = 0.0f;  // stays that if all sums are finite
       if (partial < 0) {
-        if (row >= rows) return;
         const float sum = lds.sums[c][column];
         const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
         uint16_t *o = p.out + (((int64_t)base + row0 + row) * kQueryHeads + qh) * kDim + dim0;
 #pragma unroll
         for (int d = 0; d < G::kDims; ++d) {
           const f32x16_t &x = acc[c * G::kDims + d];
+          uint2 words[4];
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<uint2 *>(o + 32 * d + 2 * i) =
-                make_uint2(cvt_pk_bf16(x[i] * inv, x[i + 1] * inv),
-                           cvt_pk_bf16(x[i + 2] * inv, x[i + 3] * inv));
+          for (int i = 0; i < 16; i += 4) {
+            words[i / 4] = make_uint2(cvt_pk_bf16(x[i] * inv, x[i + 1] * inv),
+                                      cvt_pk_bf16(x[i + 2] * inv, x[i + 3] * inv));
+            zero = fmaf(x[i], 0.0f, fmaf(x[i + 1], 0.0f, zero));
+            zero = fmaf(x[i + 2], 0.0f, fmaf(x[i + 3], 0.0f, zero));
+          }
+          if (row < rows) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint2 *>(o + 4 * end_half + 32 * d + 8 * i) = words[i];
+          }
         }
+        // The same lane stored this element above.
+        if (xor_sum<32>(zero) != 0.0f && end_half == 0 && row < rows) *o = kExtendOdd;
       } else {
         // One wave's rows go to their places; more leave as they are, 1 KiB a store.
-        if (kGroups == 1 ? row >= rows : c * G::kWaveRows >= rows) return;
+        const int64_t at =
+            (int64_t)partial * kQueryHeads +
+            (kGroups == 1 ? row * kQueryHeads + qh
+                          : head * G::kGroup * ((rows + G::kWaveRows - 1) / G::kWaveRows *
+                                                G::kWaveRows) + c * 32 + column);
         float *o = kGroups == 1
-                       ? p.partial + ((int64_t)(partial + row) * kQueryHeads + qh) * kDim + dim0
-                       : p.partial + wide_column * kDim +
-                             (c * kWaves + wave) * (G::kDims * 1024) + 4 * end_lane;
+                       ? p.partial + at * kDim + dim0 + 4 * end_half
+                       : p.partial + (at - column) * kDim + wave * (G::kDims * 1024) + 4 * end_lane;
 #pragma unroll
         for (int d = 0; d < G::kDims; ++d) {
           const f32x16_t &x = acc[c * G::kDims + d];
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4 *>(o + (kGroups == 1 ? 32 * d + 2 * i : 1024 * d + 64 * i)) =
-                make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+          for (int i = 0; i < 16; i += 4) {
+            if (kGroups > 1 || row < rows)
+              *reinterpret_cast<float4 *>(o + (kGroups == 1 ? 32 * d + 2 * i : 1024 * d + 64 * i)) =
+                  make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+            zero = fmaf(x[i], 0.0f, fmaf(x[i + 1], 0.0f, zero));
+            zero = fmaf(x[i + 2], 0.0f, fmaf(x[i + 3], 0.0f, zero));
+          }
         }
+        if (wave == c && end_half == 0 && row < rows)
+          *reinterpret_cast<float2 *>(p.stats + 2 * at) = make_float2(m_run, l_run);
+        const uint64_t odd = __builtin_amdgcn_ballot_w64(zero != 0.0f);
+        if (end_lane == 0)
+          p.odd[((int64_t)(partial + c * G::kWaveRows) * G::kHeads + head) * kWaves + wave] =
+              (uint32_t)odd | (uint32_t)(odd >> 32);
       }
     });
     };

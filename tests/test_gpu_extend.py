@@ -232,6 +232,44 @@ def test_small_and_large_values(dev, heads, dim, spread):
 
 
 @pytest.mark.parametrize("heads,dim", GEOMETRIES)
+@pytest.mark.parametrize("rows,prior", [([40], [0]), ([2], [3000]), ([12, 30, 1], [3000, 40, 7]), ([300], [100])])
+@pytest.mark.parametrize("window", [0, 9])
+def test_what_a_row_does_not_see_is_not_in_it(dev, heads, dim, rows, prior, window):
+    """Infinities and NaN in keys and values of new tokens, and of cached ones that the
+    window has passed for some rows: in the rows that see them, and nowhere else."""
+    import torch
+    b = Batch(dev, heads, dim, rows, prior, window=window, seed=window)
+    clean = b.expected()
+    b.expected = lambda layer=0: clean
+    n, p = rows[0], prior[0]
+    at = torch.arange(b.total, device=dev)[:, None, None] + p
+    own = (at < p + n)
+    sees = lambda key: own & (key <= at) & ((key > at - window) if window else own)  # noqa: E731
+    of_head = torch.arange(16, device=dev)[None, :, None] * heads // 16
+    dims = torch.arange(dim, device=dev)[None, None, :]
+    token, cached, last = p + n // 2, max(p - window // 2, 0), heads - 1
+    odd = torch.zeros(b.total, 16, dim, dtype=torch.bool, device=dev)
+    b.v[n // 2, 0, 3], b.v[n // 2, 0, dim - 1] = math.inf, NAN
+    odd |= sees(token) & (of_head == 0) & ((dims == 3) | (dims == dim - 1))
+    b.v[n - 1, last] = -math.inf
+    odd |= sees(p + n - 1) & (of_head == last)
+    if cached < p:
+        held = int(b.table[0, cached // 16])
+        b.cv[0, held, cached % 16, last, dim // 2] = math.inf
+        odd |= sees(cached) & (of_head == last) & (dims == dim // 2)
+    outs = [b.run(), b.run()]
+    assert torch.equal(outs[0].isfinite(), ~odd)
+    for out in outs:
+        b.check(torch.where(odd, clean[0].bfloat16(), out))
+    # Keys: a row that sees one has no finite weights.
+    b.k[n // 2, 0, 5] = NAN
+    odd |= sees(token) & (of_head == 0)
+    out = b.run()
+    assert torch.equal(out.isfinite(), ~odd)
+    b.check(torch.where(odd, clean[0].bfloat16(), out))
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
 def test_rising_scores(dev, heads, dim):
     """Each tile's scores above the last's: the running maximum moves every time."""
     import torch
