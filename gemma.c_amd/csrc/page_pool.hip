@@ -113,26 +113,38 @@ __device__ __forceinline__ int32_t round_ranks(const bool (&flag)[kPoolUnroll],
   return total;
 }
 
+// Counts of this thread's pages of a round; 1 behind the last page.
+struct RefRound {
+  int32_t refs[kPoolUnroll];
+};
+__device__ __forceinline__ RefRound load_refs(const PoolParams &p, uint32_t base) {
+  RefRound r;
+#pragma unroll
+  for (int u = 0; u < kPoolUnroll; ++u) {
+    const uint32_t page = base + u * kPoolThreads + threadIdx.x;
+    r.refs[u] = page < (uint32_t)p.c.num_pages ? p.refs[page] : 1;
+  }
+  return r;
+}
+
 // Free pages with ranks [from, from + kPoolList) into `list`, in page order.
 // Looks no further than to the one with rank wanted - 1; returns how many free
-// pages it has seen.
+// pages it has seen. `next` holds the first round's counts.
 __device__ __forceinline__ int32_t find_free(const PoolParams &p, int32_t from, int32_t wanted,
-                                             int32_t *list, RankScratch &scratch) {
+                                             RefRound next, int32_t *list, RankScratch &scratch) {
   int32_t seen = 0;
-  for (int32_t base = 0; base < p.c.num_pages && seen < wanted; base += kPoolRound) {
+  for (uint32_t base = 0; base < (uint32_t)p.c.num_pages && seen < wanted; base += kPoolRound) {
     bool flag[kPoolUnroll];
     int32_t rank[kPoolUnroll];
 #pragma unroll
-    for (int u = 0; u < kPoolUnroll; ++u) {
-      const int32_t page = base + u * kPoolThreads + (int32_t)threadIdx.x;
-      flag[u] = page < p.c.num_pages && p.refs[page] <= 0;
-    }
+    for (int u = 0; u < kPoolUnroll; ++u) flag[u] = next.refs[u] <= 0;
+    next = load_refs(p, base + kPoolRound);
     const int32_t found = round_ranks(flag, rank, scratch);
 #pragma unroll
     for (int u = 0; u < kPoolUnroll; ++u) {
       const int32_t at = seen + rank[u] - from;
       if (flag[u] && at >= 0 && at < kPoolList)
-        list[at] = base + u * kPoolThreads + (int32_t)threadIdx.x;
+        list[at] = (int32_t)(base + u * kPoolThreads + threadIdx.x);
     }
     seen += found;
   }
@@ -214,14 +226,14 @@ __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
   // how many are missing.
   auto for_missing = [&](auto &&f) -> int32_t {
     int32_t missing = 0;
-    for (int32_t base = 0; base < items; base += kPoolRound) {
+    for (uint32_t base = 0; base < (uint32_t)items; base += kPoolRound) {
       int64_t at[kPoolUnroll];
       bool flag[kPoolUnroll];
       int32_t rank[kPoolUnroll];
 #pragma unroll
       for (int u = 0; u < kPoolUnroll; ++u) {
-        const int32_t item = base + u * kPoolThreads + t;
-        at[u] = item < items ? entry_of(item) : -1;
+        const uint32_t item = base + u * kPoolThreads + t;
+        at[u] = item < (uint32_t)items ? entry_of((int32_t)item) : -1;
         flag[u] = at[u] >= 0 && p.page_table[at[u]] < 0;
       }
       const int32_t found = round_ranks(flag, rank, lds.scratch);
@@ -233,7 +245,7 @@ __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
     return missing;
   };
   const int32_t wanted = for_missing([](int64_t, int32_t) {});
-  int32_t seen = find_free(p, 0, wanted, lds.list, lds.scratch);
+  const int32_t seen = find_free(p, 0, wanted, load_refs(p, 0), lds.list, lds.scratch);
   if (seen < wanted) {
     if (t == 0) *status = kStatusPages;
     return;
@@ -242,7 +254,7 @@ __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
   // A window of the list at a time. What an earlier window filled is no longer
   // missing: the ranks of what is left start at the window's own first.
   for (int32_t from = 0; from < wanted; from += kPoolList) {
-    if (from > 0) find_free(p, 0, wanted - from, lds.list, lds.scratch);
+    if (from > 0) find_free(p, 0, wanted - from, load_refs(p, 0), lds.list, lds.scratch);
     for_missing([&](int64_t at, int32_t rank) {
       if (rank >= kPoolList) return;
       const int32_t page = lds.list[rank];
@@ -274,17 +286,31 @@ __device__ __forceinline__ Share fork_share(const PoolParams &p, int32_t length,
   return slot == whole && length > whole * p.c.page_size ? Share::kCopy : Share::kNone;
 }
 
+// Slots of a branch that may need a page of its own: all of a ring's, the begun page's
+// of a full-length cache.
+__device__ __forceinline__ int32_t fork_slot(const PoolParams &p, int32_t length, int32_t i) {
+  return p.c.window_size > 0 ? i : (int32_t)fast_div((uint32_t)length, p.page_div);
+}
+
+// One workgroup checks the request, hands out the pages of what is copied and tells
+// in `status` whether the launch behind it copies and shares: the way is a chain of
+// dependent loads (requests, lengths, table, counts), which is the time. What is
+// known early is asked for early and a branch's parent, child and length are kept in
+// LDS (18 branches of a 1 x 512 cache, tables of 129 pages: 12.1 -> 6.0 us).
 struct ForkLds {
   int32_t role[kPoolBatch];  // bit 0: a parent, bit 1: a child
+  int32_t parent[kPoolBatch], child[kPoolBatch], length[kPoolBatch];  // of a branch
   int32_t list[kPoolList];
   RankScratch scratch;
   int32_t bad;
 };
-__global__ __launch_bounds__(kPoolThreads) void fork_tables_kernel(ForkParams f) {
+__global__ __launch_bounds__(kPoolThreads) void fork_tables_kernel(ForkParams f, int32_t slots,
+                                                                   FastDiv by_slots) {
   __shared__ ForkLds lds;
   const PoolParams &p = f.pool;
   const int t = threadIdx.x;
   const int32_t batch = p.c.batch_size, pages = p.c.max_pages_per_seq;
+  const RefRound ahead = load_refs(p, 0);
   for (int32_t b = t; b < batch; b += kPoolThreads) lds.role[b] = 0;
   if (t == 0) lds.bad = 0;
   __syncthreads();
@@ -293,6 +319,9 @@ __global__ __launch_bounds__(kPoolThreads) void fork_tables_kernel(ForkParams f)
     bool ok = parent >= 0 && parent < batch && child >= 0 && child < batch;
     if (ok) {
       const int32_t length = f.seq_lengths[parent];
+      lds.parent[r] = parent;
+      lds.child[r] = child;
+      lds.length[r] = length;
       ok = length >= 0 && (p.c.window_size > 0 || length <= (int64_t)pages * p.c.page_size);
       atomicOr(&lds.role[parent], 1);
       if (atomicOr(&lds.role[child], 2) & 2) ok = false;  // a child of two
@@ -307,74 +336,83 @@ __global__ __launch_bounds__(kPoolThreads) void fork_tables_kernel(ForkParams f)
     if (t == 0) *f.status = kStatusArguments;
     return;
   }
-  // Entry (request r, slot s) of the list at r * pages + s.
-  const int32_t items = f.count * pages;
-  // visit(share, child's table index, parent's page, rank among the copies).
-  auto for_entries = [&](auto &&visit) -> int32_t {
+  // Entry i of branch r, of those that may be copied, at r * slots + i of a list.
+  const uint32_t items = (uint32_t)(f.count * slots);
+  struct Round {
+    int64_t to[kPoolUnroll];      // child's table entry
+    int32_t rank[kPoolUnroll];
+    bool copy[kPoolUnroll];
+  };
+  auto load_round = [&](uint32_t base, Round &e) -> int32_t {
+    int32_t physical[kPoolUnroll];
+    int32_t slot[kPoolUnroll], length[kPoolUnroll];
+#pragma unroll
+    for (int u = 0; u < kPoolUnroll; ++u) {
+      const uint32_t item = base + u * kPoolThreads + t;
+      e.to[u] = -1;
+      physical[u] = -1;
+      if (item < items) {
+        const int32_t r = (int32_t)fast_div(item, by_slots);
+        length[u] = lds.length[r];
+        slot[u] = fork_slot(p, length[u], (int32_t)item - r * slots);
+        if (slot[u] < pages) {
+          e.to[u] = (int64_t)lds.child[r] * pages + slot[u];
+          physical[u] = p.page_table[(int64_t)lds.parent[r] * pages + slot[u]];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kPoolUnroll; ++u)
+      e.copy[u] = e.to[u] >= 0 && fork_share(p, length[u], slot[u], physical[u]) == Share::kCopy;
+    return round_ranks(e.copy, e.rank, lds.scratch);
+  };
+  Round first;
+  int32_t wanted = load_round(0, first);
+  for (uint32_t base = kPoolRound; base < items; base += kPoolRound) {
+    Round e;
+    wanted += load_round(base, e);
+  }
+  // A child holds nothing yet.
+  const uint32_t entries = (uint32_t)(f.count * pages);
+  bool held = false;
+  for (uint32_t base = 0; base < entries; base += kPoolRound) {
+#pragma unroll
+    for (int u = 0; u < kPoolUnroll; ++u) {
+      const uint32_t entry = base + u * kPoolThreads + t;
+      if (entry >= entries) continue;
+      const int32_t r = (int32_t)fast_div(entry, p.slot_div);
+      held |= p.page_table[(int64_t)lds.child[r] * pages + ((int32_t)entry - r * pages)] >= 0;
+    }
+  }
+  if (held) lds.bad = 1;
+  const int32_t seen = find_free(p, 0, wanted, ahead, lds.list, lds.scratch);
+  if (lds.bad || seen < wanted) {
+    if (t == 0) *f.status = lds.bad ? kStatusArguments : kStatusPages;
+    return;
+  }
+  // A page handed out is free no more, so the list of the next window starts with its
+  // own first page.
+  for (int32_t from = 0; from < wanted; from += kPoolList) {
+    if (from > 0) find_free(p, 0, wanted - from, load_refs(p, 0), lds.list, lds.scratch);
     int32_t copies = 0;
-    for (int32_t base = 0; base < items; base += kPoolRound) {
-      int64_t to[kPoolUnroll];
-      int32_t physical[kPoolUnroll], rank[kPoolUnroll];
-      Share share[kPoolUnroll];
-      bool flag[kPoolUnroll];
+    for (uint32_t base = 0; base < items; base += kPoolRound) {
+      Round e = first;
+      int32_t found = 0;
+      if (items > kPoolRound) found = load_round(base, e);
 #pragma unroll
       for (int u = 0; u < kPoolUnroll; ++u) {
-        const int32_t item = base + u * kPoolThreads + t;
-        to[u] = -1;
-        physical[u] = -1;
-        share[u] = Share::kNone;
-        if (item < items) {
-          const int32_t r = (int32_t)fast_div((uint32_t)item, p.slot_div);
-          const int32_t slot = item - r * pages;
-          const int32_t parent = f.parents[r];
-          to[u] = (int64_t)f.children[r] * pages + slot;
-          physical[u] = p.page_table[(int64_t)parent * pages + slot];
-          share[u] = fork_share(p, f.seq_lengths[parent], slot, physical[u]);
-        }
-        flag[u] = share[u] == Share::kCopy;
-      }
-      const int32_t found = round_ranks(flag, rank, lds.scratch);
-#pragma unroll
-      for (int u = 0; u < kPoolUnroll; ++u)
-        if (to[u] >= 0) visit(share[u], to[u], physical[u], copies + rank[u]);
-      copies += found;
-    }
-    return copies;
-  };
-  // A child holds nothing yet.
-  const int32_t wanted = for_entries([&](Share, int64_t to, int32_t, int32_t) {
-    if (p.page_table[to] >= 0) lds.bad = 1;
-  });
-  __syncthreads();
-  if (lds.bad) {
-    if (t == 0) *f.status = kStatusArguments;
-    return;
-  }
-  const int32_t seen = find_free(p, 0, wanted, lds.list, lds.scratch);
-  if (seen < wanted) {
-    if (t == 0) *f.status = kStatusPages;
-    return;
-  }
-  // The first window also shares; later ones only hand out their pages. A page
-  // handed out is free no more, so the list of the next window starts with its
-  // own first page.
-  for (int32_t from = 0; from == 0 || from < wanted; from += kPoolList) {
-    if (from > 0) find_free(p, 0, wanted - from, lds.list, lds.scratch);
-    for_entries([&](Share share, int64_t to, int32_t physical, int32_t rank) {
-      if (share == Share::kSame && from == 0) {
-        p.page_table[to] = physical;
-        atomicAdd(&p.refs[physical], 1);
-      } else if (share == Share::kCopy && rank >= from && rank - from < kPoolList) {
-        const int32_t page = lds.list[rank - from];
-        p.page_table[to] = page;
+        const int32_t rank = copies + e.rank[u] - from;
+        if (!e.copy[u] || rank < 0 || rank >= kPoolList) continue;
+        const int32_t page = lds.list[rank];
+        p.page_table[e.to[u]] = page;
         p.refs[page] = 1;
       }
-    });
+      copies += found;
+    }
     __threadfence_block();
     __syncthreads();
   }
-  for (int32_t r = t; r < f.count; r += kPoolThreads)
-    f.seq_lengths[f.children[r]] = f.seq_lengths[f.parents[r]];
+  for (int32_t r = t; r < f.count; r += kPoolThreads) f.seq_lengths[lds.child[r]] = lds.length[r];
   if (t == 0) *f.status = kStatusOk;
 }
 
@@ -384,7 +422,9 @@ constexpr int kCopyPacks = kCopyThreads * kCopyUnroll;  // 16-byte packs per wor
 
 // Workgroup (piece of a page, copied page of a branch, layer x {K, V}): the
 // branch's table says where to, what the parent's length leaves in a begun page
-// how much. All loads of a piece are in flight before its first store.
+// how much. All loads of a piece are in flight before its first store. In a
+// full-length cache the first layer's workgroups of a branch also share its
+// parent's whole pages.
 __global__ __launch_bounds__(kCopyThreads) void fork_copy_kernel(ForkParams f, uint16_t *cache_k,
                                                                  uint16_t *cache_v, int32_t pieces,
                                                                  int32_t slots) {
@@ -395,9 +435,17 @@ __global__ __launch_bounds__(kCopyThreads) void fork_copy_kernel(ForkParams f, u
   const int32_t r = which / slots;
   const int32_t parent = f.parents[r], child = f.children[r];
   const int32_t length = f.seq_lengths[parent];
-  int32_t slot = which - r * slots, rows = p.c.page_size;
+  const int32_t slot = fork_slot(p, length, which - r * slots);
+  int32_t rows = p.c.page_size;
   if (p.c.window_size == 0) {
-    slot = (int32_t)fast_div((uint32_t)length, p.page_div);
+    if (blockIdx.y == 0) {
+      for (int32_t s = piece * kCopyThreads + threadIdx.x; s < slot; s += pieces * kCopyThreads) {
+        const int32_t physical = p.page_table[(int64_t)parent * pages + s];
+        if (fork_share(p, length, s, physical) != Share::kSame) continue;
+        p.page_table[(int64_t)child * pages + s] = physical;
+        atomicAdd(&p.refs[physical], 1);
+      }
+    }
     rows = length - slot * p.c.page_size;
     if (rows == 0) return;
   }
@@ -632,7 +680,8 @@ hipError_t gemma4_kv_cache_fork_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cach
   const int64_t pieces = (page_packs + kCopyPacks - 1) / kCopyPacks;
   const int64_t blocks = pieces * slots * fork_count;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(fork_tables_kernel, dim3(1), dim3(kPoolThreads), 0, stream, f);
+  hipLaunchKernelGGL(fork_tables_kernel, dim3(1), dim3(kPoolThreads), 0, stream, f, slots,
+                     make_fast_div(slots));
   hipLaunchKernelGGL(fork_copy_kernel, dim3((uint32_t)blocks, 2 * config.num_layers),
                      dim3(kCopyThreads), 0, stream, f, reinterpret_cast<uint16_t *>(d_cache_k),
                      reinterpret_cast<uint16_t *>(d_cache_v), (int32_t)pieces, slots);
