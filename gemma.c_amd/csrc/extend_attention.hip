@@ -71,6 +71,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
   __shared__ int32_t s_share[kPlanShares + 1];    // first segment of a share
   __shared__ int64_t s_waves[kPlanWaves];
   __shared__ int32_t s_waves32[kPlanWaves];
+  __shared__ int32_t s_parts;
   const int t = threadIdx.x;
   auto *shares_at = reinterpret_cast<ExtendShare *>(p.plan + p.shares);
   auto *segments = reinterpret_cast<ExtendSegment *>(p.plan + p.segments);
@@ -78,6 +79,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
 
   // Offsets within the batch and, by a running maximum, ascending: whatever they
   // say, no row belongs to two sequences and the sections above hold the plan.
+  if (t == 0) s_parts = 0;
   int32_t reach = 0;
   for (int32_t b0 = 0; b0 <= p.batch; b0 += kPlanThreads) {
     const int32_t b = b0 + t;
@@ -196,6 +198,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     });
     if (r.rows > 0) emit(last, r.tiles);
     if (parts > 1) {
+      atomicMax(&s_parts, parts);
       for (int32_t i = 0; i < stride; ++i)
         merges[merge + i] = {s_begin[r.sequence] + r.row0, r.rows, partial, parts, stride, i, segment, {}};
     }
@@ -213,7 +216,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
   if (t == 0) {
     *reinterpret_cast<ExtendHeader *>(p.plan) = {
         kExtendMagic, p.batch, p.total_rows, p.heads, p.window, p.sinks, p.page_size, n_segments,
-        (int32_t)counts & 0xFFFF};
+        (int32_t)counts & 0xFFFF, s_parts};
   }
 }
 
@@ -225,7 +228,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
 constexpr int kMergeThreads = 256;
 constexpr int kMergeWaves = kMergeThreads / kWave;
 constexpr int kMergeGrid = 2048;
-constexpr int kMergeBatch = 8;
+constexpr int kMergeBatch = 4;
 constexpr int kMergeFew = 16;  // parts a single wave folds
 
 struct MergeState {
@@ -445,14 +448,18 @@ __global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendPa
     }
   };
   // Blocks of few parts.
-  for (int32_t i = first_item; i < items; i += gridDim.x * kMergeWaves) {
-    if (i != first_item) r = merge_of(i);
-    if (r.parts > kMergeFew) continue;
-    const Place at = place(r, i);
-    store(at, r, gather(r, at, 0, 1));
+  for (int32_t i = first_item; i < items;) {
+    const int32_t ahead = i + gridDim.x * kMergeWaves;
+    const ExtendMerge next = merge_of(min(ahead, items - 1));
+    if (r.parts <= kMergeFew) {
+      const Place at = place(r, i);
+      store(at, r, gather(r, at, 0, 1));
+    }
+    i = ahead;
+    r = next;
   }
   // Blocks of many.
-  for (int32_t i = blockIdx.x; i < items; i += gridDim.x) {
+  for (int32_t i = blockIdx.x; h.most_parts > kMergeFew && i < items; i += gridDim.x) {
     r = merge_of(i);
     if (r.parts <= kMergeFew) continue;
     const Place at = place(r, i);

@@ -63,6 +63,7 @@ struct ExtendHeader {
   int32_t batch, total_rows, heads, window, sinks, page_size;
   int32_t segments;
   int32_t merges;
+  int32_t most_parts;  // of a split row block
 };
 // In a (row, query head) that has to be worked out again, the first element of one of
 // its quarters: a signalling NaN, which no arithmetic gives.

@@ -476,7 +476,7 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
       }
 
       // ---- sums of tile it - 1, and under them the softmax of tile it -------------------
-      float top, alpha, m_use;
+      float top, alpha, m_use, even;
       bool moved = false;
       uint32_t pw[8];
       auto softmax = [&](auto uc) __attribute__((always_inline)) {
@@ -484,14 +484,16 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
         if constexpr (u == 0) {
           top = fmaxf(fmaxf(score[0], score[1]), score[2]);
           top = fmaxf(fmaxf(top, score[3]), score[4]);
-          top = fmaxf(fmaxf(top, score[5]), score[6]);
-          top = fmaxf(fmaxf(top, score[7]), score[8]);
-        } else if constexpr (u == 1) {
-          top = fmaxf(fmaxf(top, score[9]), score[10]);
-          top = fmaxf(fmaxf(top, score[11]), score[12]);
-          top = fmaxf(fmaxf(top, score[13]), score[14]);
-          top = xor_max<32>(fmaxf(top, score[15])) * p.q_scale;
-        } else if constexpr (u == 2) {
+        } else if constexpr (u < 4) {
+          top = fmaxf(fmaxf(top, score[4 * u + 1]), score[4 * u + 2]);
+          if constexpr (u < 3) {
+            top = fmaxf(fmaxf(top, score[4 * u + 3]), score[4 * u + 4]);
+          } else {
+            top = fmaxf(top, score[15]);
+          }
+        } else if constexpr (u == 4) {
+          top = xor_max<32>(top) * p.q_scale;
+        } else if constexpr (u == 5) {
           // The maximum moves (and the sums are rescaled) only when a column outgrows
           // it by more than the slack: exp2's arguments stay below that.
           moved = __builtin_amdgcn_ballot_w64(top > m_run + kRescaleSlack) != 0;
@@ -500,14 +502,17 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
           m_run = m_new;
           m_use = m_new == -INFINITY ? 0.0f : m_new;
           l_run *= alpha;
-        } else if constexpr (u >= 4 && u < 12) {
-          constexpr int i = 2 * (u - 4);
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(score[i], p.q_scale, -m_use));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(score[i + 1], p.q_scale, -m_use));
-          l_run += p0 + p1;
+        } else if constexpr (u >= 7 && u < 23) {
+          constexpr int i = u - 7;
+          const float w = __builtin_amdgcn_exp2f(fmaf(score[i], p.q_scale, -m_use));
           // P is the product's operand: bf16, half a step (2^-8) of each weight.
-          pw[i / 2] = cvt_pk_bf16(p0, p1);
-        } else if constexpr (u == 12) {
+          if constexpr (i % 2 == 0) {
+            even = w;
+          } else {
+            l_run += even + w;
+            pw[i / 2] = cvt_pk_bf16(even, w);
+          }
+        } else if constexpr (u == 23) {
           if (kGroups == kWaves || wave == 0) {
             lds.weights[parity][wave][0][copy_lane] = u32x4v_t{pw[0], pw[1], pw[2], pw[3]};
             lds.weights[parity][wave][1][copy_lane] = u32x4v_t{pw[4], pw[5], pw[6], pw[7]};
@@ -520,18 +525,15 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
         }
       };
       // Product j: operand i = j / kGroups, group j % kGroups.
-      constexpr int kUnits = 13, kProducts = kGroups * kOperands;
-      constexpr int kPerUnit = kProducts >= 16 ? kProducts / 16 : 1;
+      constexpr int kUnits = 24, kProducts = kGroups * kOperands;
       static_for<0, kProducts>([&](auto jc) __attribute__((always_inline)) {
         constexpr int j = decltype(jc)::value, i = j / kGroups, c = j % kGroups;
         mfma_pv(acc[c * G::kDims + i % G::kDims], v[i % kRing], w[c]);
         if constexpr (c == 0 && i + kRing - 1 < kOperands) read_v(v_at, i + kRing - 1);
         if constexpr (i == G::kDims - 1) read_w(parity ^ 1, c, 1, copy_lane);
-        if constexpr (j % kPerUnit == 0 && j / kPerUnit < kUnits)
-          softmax(std::integral_constant<int, j / kPerUnit>{});
+        static_for<j * kUnits / kProducts, (j + 1) * kUnits / kProducts>(softmax);
         __builtin_amdgcn_sched_barrier(0);
       });
-      static_for<(kProducts + kPerUnit - 1) / kPerUnit, kUnits>(softmax);
 
       k_at = k_address(copy_lane) + ((it + 1) & (kStages - 1)) * kStageBytes;
       if (run_tile == 0) {
