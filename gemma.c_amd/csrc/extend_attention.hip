@@ -56,15 +56,17 @@ __device__ __forceinline__ T block_prefix(T x, T &total, T *waves, F f) {
 constexpr int kPlanShares = 256;
 constexpr int kShareTiles = 2;  // least cost worth a workgroup
 // Besides its tiles a row block costs the way to its first keys, its queries and its
-// rows' end: about four tiles' time where it holds several waves' rows, three where
-// one's.
+// rows' end, in tiles' times: at 8 x 256 7.8 us, of 1.3 us a tile, where it holds several
+// waves' rows, 4.5 where one's; at 1 x 512 12 and 7, of 2.1. Batches of 1 x 512 are
+// shared out best (by a few percent) with somewhat less.
 __device__ __forceinline__ int32_t block_cost(const ExtendGeometry &g, int32_t rows) {
-  return rows > g.wave_rows ? 4 : 3;
+  return rows <= g.wave_rows ? 3 : (g.rows == kExtend256.rows ? 6 : 4);
 }
 
-// One workgroup. The row blocks laid end to end are cut into shares of equal cost. A cut near a block's end moves
-// there: a split block costs its partial sums, written, read and merged (64 rows
-// about four tiles' time, few rows less).
+// One workgroup. The row blocks laid end to end are cut into shares of equal cost,
+// wherever the cuts fall: cuts that kept a tile or four away from a block's ends, to
+// save partial sums, left shares of twice the mean where blocks are short (geometric
+// mean of 32 batches of 1 to 30 sequences 38 -> 34 us without).
 __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p) {
   __shared__ int32_t s_begin[kExtendBatch + 1];   // first row of a sequence
   __shared__ int32_t s_blocks[kExtendBatch + 1];  // row blocks before it
@@ -151,24 +153,20 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     const int64_t end = before + block_prefix(r.cost, all, s_waves, Sum());
     const int64_t begin = end - r.cost;
     before += all;
-    const int32_t snap = 1 + r.rows * 3 / p.g.rows;
     const int32_t ahead = block_cost(p.g, r.rows);
-    // f(cut k, the tile it lies at: 0 and r.tiles are no cuts of the block)
+    // f(cut k, the tile it lies at: 0 is no cut of the block)
     auto for_cuts = [&](auto &&f) {
       if (r.rows == 0) return;
       int32_t k = max((int32_t)((double)begin / step), 1);
       while (k > 1 && cut_at(k - 1) >= begin) --k;
       while (k < shares && cut_at(k) < begin) ++k;
       for (; k < shares && cut_at(k) < end; ++k) {
-        int32_t tile = (int32_t)max(cut_at(k) - begin - ahead, (int64_t)0);
-        if (tile < snap) tile = 0;
-        if (r.tiles - tile < snap) tile = r.tiles;
-        f(k, tile);
+        f(k, (int32_t)max(cut_at(k) - begin - ahead, (int64_t)0));
       }
     };
     int32_t parts = r.rows > 0 ? 1 : 0, last = 0;
     for_cuts([&](int32_t, int32_t tile) {
-      if (tile > last && tile < r.tiles) {
+      if (tile > last) {
         ++parts;
         last = tile;
       }
@@ -189,12 +187,12 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
                                   parts > 1 ? partial + part * stride : -1};
     };
     for_cuts([&](int32_t k, int32_t tile) {
-      if (tile > last && tile < r.tiles) {
+      if (tile > last) {
         emit(last, tile);
         ++part;
         last = tile;
       }
-      s_share[k] = segment + part + (tile >= r.tiles ? 1 : 0);
+      s_share[k] = segment + part;
     });
     if (r.rows > 0) emit(last, r.tiles);
     if (parts > 1) {
