@@ -571,7 +571,7 @@ extern "C" hipError_t gemma4_flash_attention_extend_paged_bf16(
   if (!valid_extend(config, batch_size, total_rows) || d_out == nullptr || d_q == nullptr ||
       d_k == nullptr || d_v == nullptr || d_cache_k == nullptr || d_cache_v == nullptr ||
       d_page_table == nullptr || d_plan == nullptr || d_workspace == nullptr || layer < 0 ||
-      layer >= config.num_layers || !(softmax_scale > 0.0f) || !isfinite(softmax_scale)) {
+      layer >= config.num_layers || !(softmax_scale > 0.0f) || !isfinite(softmax_scale * kLog2e)) {
     return hipErrorInvalidValue;
   }
   const int64_t q_width = (int64_t)kQueryHeads * config.head_dim;

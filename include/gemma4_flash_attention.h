@@ -215,7 +215,10 @@ hipError_t gemma4_flash_attention_prefill_chunk_paged_bf16_ws(
 // may be read by several. Offsets that do not ascend or pass total_rows are
 // clamped to it, a negative prior length counts as 0: such a plan attends to the
 // wrong keys but reads and writes within the tensors. Rows that no sequence
-// holds (total_rows past the last offset) are left as they were.
+// holds (total_rows past the last offset) are left as they were. batch_size is at
+// most 4096 and config.batch_size, total_rows 2^24, num_pages * page_size below
+// 2^31 (sizes outside: 0 bytes). A key that a row does not see has no part in it,
+// whatever its K and V hold; every row sees at least itself.
 size_t gemma4_flash_attention_extend_plan_bytes(Gemma4KvCacheConfig config, int32_t batch_size,
                                                 int32_t total_rows);
 size_t gemma4_flash_attention_extend_workspace_bytes(Gemma4KvCacheConfig config,
@@ -231,8 +234,9 @@ hipError_t gemma4_flash_attention_extend_plan(void *d_plan, size_t plan_bytes,
 // batch_size and total_rows (a plan of other sizes writes nothing).
 // q_stride, kv_stride: elements from one row of q, and of k and v, to the next
 // (slices of a wider projection), multiples of 8; 0 for packed rows, 16 * head_dim
-// and num_heads * head_dim. out [total_rows][16][head_dim] is packed. q, k, v, out
-// and the caches are 16-byte aligned. total_rows == 0 is a no-op success.
+// and num_heads * head_dim, at most 2^30. out [total_rows][16][head_dim] is packed
+// and overlaps no input. q, k, v, out and the caches are 16-byte aligned.
+// total_rows == 0 is a no-op success.
 hipError_t gemma4_flash_attention_extend_paged_bf16(
     gemma4_bf16 *d_out, const gemma4_bf16 *d_q, const gemma4_bf16 *d_k, const gemma4_bf16 *d_v,
     const gemma4_bf16 *d_cache_k, const gemma4_bf16 *d_cache_v, const int32_t *d_page_table,

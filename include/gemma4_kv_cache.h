@@ -183,7 +183,8 @@ hipError_t gemma4_kv_cache_fork_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cach
 // d_kept_offsets[i + 1]) move to d_first_positions[i], + 1, + 2, ..., in place,
 // in every layer, K and V (the accepted tokens of a verified draft; a prompt
 // thinned out). Rows move as they are: a key keeps the rotation of its old
-// position. A request's positions ascend strictly, none lies before its new
+// position. (A ring has lost the keys that rejected tokens overwrote: one that
+// verifies n drafts needs n slots more than its window.) A request's positions ascend strictly, none lies before its new
 // place, and for a sliding cache all lie within the ring's slots of the first
 // position. d_page_refs may be null where no page is shared; otherwise a request
 // that would write to a page with more than one reference is refused.

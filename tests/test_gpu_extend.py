@@ -471,3 +471,88 @@ def test_a_server_s_steps(dev, heads, dim, ring):
         gk.check(gk.kv_cache_release_pages(table, refs, cfg, i32([0] * 4), i32([max(0, n - window) for n in lens])))
     step([1, 1, 1, 1])
     step([40, 1, 2, 3])
+
+
+@pytest.mark.parametrize("heads,dim,pages", [(8, 256, 21000), (1, 512, 84000)])
+def test_a_cache_of_more_than_four_gigabytes(dev, heads, dim, pages):
+    """The same pages at the far end of a cache past 2^32 bytes, in its second layer."""
+    import torch
+    b = Batch(dev, heads, dim, [1, 40, 0, 3], [900, 333, 7, 64], page=64)
+    out = b.run()
+    b.check(out)
+    large = torch.empty((2, 2, pages, 64, heads, dim), dtype=torch.bfloat16, device=dev)
+    assert large[0, 0].numel() * 2 > 2**32 and b.pages < 100
+    for i, small in enumerate((b.ck, b.cv)):
+        large[i, 1, pages - b.pages:] = small[0]
+    b.ck, b.cv = large[0], large[1]
+    b.table = torch.where(b.table >= 0, b.table + pages - b.pages, b.table)
+    b.config = gk.make_config(2, pages, 64, b.max_pages, b.batch, heads, dim, 0)
+    assert torch.equal(b.run(1), out)
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+def test_every_run_gives_the_same(dev, heads, dim):
+    import torch
+    b = Batch(dev, heads, dim, [1, 30, 3, 200], [5000, 700, 2049, 100])
+    b.v[20, 0, 3] = math.inf  # some rows are worked out again
+    out = b.run()
+    assert not bool(out.isfinite().all())
+    for _ in range(6):
+        b.ws.fill_(0xFF)
+        assert torch.equal(b.run().view(torch.int16), out.view(torch.int16))
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+def test_two_streams_at_once(dev, heads, dim):
+    """Two batches, each with its buffers, on streams that overlap; layers of one batch
+    on two streams by one plan, each with its workspace."""
+    import torch
+    b = Batch(dev, heads, dim, [1, 30, 3], [5000, 700, 2049], layers=2)
+    c = Batch(dev, heads, dim, [150, 1], [900, 3000], layers=2, seed=4)
+    want = [b.run(0), b.run(1), c.run(0)]
+    ws = torch.empty_like(b.ws)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    b.make_plan()
+    torch.cuda.synchronize()
+    outs = [[torch.full_like(w, 7.0) for w in want] for _ in range(8)]
+    torch.cuda.synchronize()
+    for row in outs:
+        with torch.cuda.stream(streams[0]):
+            b.attend(row[0], 0)
+        with torch.cuda.stream(streams[1]):
+            own, b.ws = b.ws, ws
+            b.attend(row[1], 1)
+            b.ws = own
+        with torch.cuda.stream(streams[2]):
+            c.make_plan()
+            c.attend(row[2], 0)
+    torch.cuda.synchronize()
+    for row in outs:
+        assert all(torch.equal(x, w) for x, w in zip(row, want))
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+def test_graphs_that_share_a_workspace(dev, heads, dim):
+    """Two captured steps with one plan buffer and one workspace, replayed in turn with
+    eager calls between."""
+    import torch
+    a = Batch(dev, heads, dim, [1, 40], [3000, 64])
+    b = Batch(dev, heads, dim, [20, 21], [10, 900], seed=2)
+    b.plan, b.ws = a.plan, a.ws  # the same sizes
+    want = [a.run(), b.run()]
+    outs = [torch.empty_like(w) for w in want]
+    graphs = []
+    for x, out in zip((a, b), outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            x.make_plan()
+            x.attend(out)
+        graphs.append(graph)
+    for turn in range(4):
+        for o in outs:
+            o.fill_(7.0)
+        for graph in graphs if turn % 2 else graphs[::-1]:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+        assert torch.equal((a, b)[turn % 2].run(), want[turn % 2])

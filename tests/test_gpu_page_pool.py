@@ -438,3 +438,35 @@ def test_other_stream(dev):
     p.release([9] * 5, [EVERYTHING] * 5)
     p.release([5] * 5, [EVERYTHING] * 5)
     d.check()
+
+
+@pytest.mark.parametrize("heads,dim,pages", [(8, 256, 21000), (1, 512, 84000)])
+def test_a_cache_of_more_than_four_gigabytes(dev, heads, dim, pages):
+    """Fork and compact at the far end of a cache past 2^32 bytes."""
+    import torch
+    page, layers = 64, 2
+    cfg = gk.make_config(layers, pages, page, 4, 2, heads, dim, 0)
+    k, v = (torch.empty((layers, pages, page, heads * dim), dtype=torch.int16, device=dev) for _ in range(2))
+    assert k[0].numel() * 2 > 2**32
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    refs = torch.ones(pages, dtype=torch.int32, device=dev)
+    refs[pages - 2:] = 0
+    table = i32([[pages - 3, pages - 5, -1, -1], [-1] * 4])
+    gen = torch.Generator(device="cpu").manual_seed(1)
+    rows = [torch.randint(-2**15, 2**15, (layers, 2, page, heads * dim), generator=gen).to(torch.int16).to(dev) for _ in range(2)]
+    for x, r in zip((k, v), rows):
+        x[:, pages - 3], x[:, pages - 5] = r[:, 0], r[:, 1]
+    lens, status = i32([100, 0]), i32([77])
+    gk.check(gk.kv_cache_fork_bf16(k, v, cfg, table, refs, lens, i32([0]), i32([1]), 1, status))
+    assert int(status) == 0 and lens.tolist() == [100, 100]
+    assert table[1].tolist() == [pages - 3, pages - 2, -1, -1]
+    assert refs[pages - 5:].tolist() == [1, 1, 2, 1, 0]
+    for x, r in zip((k, v), rows):
+        assert torch.equal(x[:, pages - 2, :36], r[:, 1, :36])
+    kept = [66, 70, 71, 99]
+    st = i32([77])
+    gk.check(gk.kv_cache_compact_bf16(k, v, cfg, table, refs, i32([1]), i32([65]), i32([0, 4]), i32(kept), 1, 4, st))
+    assert int(st) == 0
+    for x, r in zip((k, v), rows):
+        assert torch.equal(x[:, pages - 2, 1:5], r[:, 1, [p - 64 for p in kept]])
+        assert torch.equal(x[:, pages - 5], r[:, 1]) and torch.equal(x[:, pages - 3], r[:, 0])
