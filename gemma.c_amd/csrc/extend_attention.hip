@@ -56,11 +56,10 @@ __device__ __forceinline__ T block_prefix(T x, T &total, T *waves, F f) {
 constexpr int kPlanShares = 256;
 constexpr int kShareTiles = 2;  // least cost worth a workgroup
 // Besides its tiles a row block costs the way to its first keys, its queries and its
-// rows' end, in tiles' times: at 8 x 256 7.8 us, of 1.3 us a tile, where it holds several
-// waves' rows, 4.5 where one's; at 1 x 512 12 and 7, of 2.1. Batches of 1 x 512 are
-// shared out best (by a few percent) with somewhat less.
+// rows' end. Where it holds several waves' rows that is 7.8 us at 8 x 256, of 1.3 us a
+// tile, and 12 at 1 x 512, of 2.1; where one's, 4.5 and 7.
 __device__ __forceinline__ int32_t block_cost(const ExtendGeometry &g, int32_t rows) {
-  return rows <= g.wave_rows ? 3 : (g.rows == kExtend256.rows ? 6 : 4);
+  return rows > g.wave_rows ? 6 : 3;
 }
 
 // One workgroup. The row blocks laid end to end are cut into shares of equal cost,
@@ -120,9 +119,9 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     }
     r.sequence = lo;
     // Causal work grows along a sequence: its blocks are laid out first, last, second,
-    // last but one, .. so that every pair costs the same. Where two shares serve a
-    // pair, every other cut falls between blocks, and the shares of one parity walk
-    // the same keys at about the same time, which L2 notices.
+    // last but one, .. so that every pair costs the same, and where two shares serve a
+    // pair every other cut falls between blocks (2048 rows after 6144 at 1 x 512: 462 us,
+    // 518 with the blocks last to first).
     const int32_t at = j - s_blocks[lo], blocks = s_blocks[lo + 1] - s_blocks[lo];
     r.row0 = (at % 2 == 0 ? at / 2 : blocks - 1 - at / 2) * p.g.rows;
     r.rows = min(s_begin[lo + 1] - s_begin[lo] - r.row0, p.g.rows);
@@ -214,7 +213,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
   if (t == 0) {
     *reinterpret_cast<ExtendHeader *>(p.plan) = {
         kExtendMagic, p.batch, p.total_rows, p.heads, p.window, p.sinks, p.page_size, n_segments,
-        (int32_t)counts & 0xFFFF, s_parts};
+        (int32_t)counts & 0xFFFF, s_parts, (int32_t)max(step, 1.0)};
   }
 }
 

@@ -64,6 +64,7 @@ struct ExtendHeader {
   int32_t segments;
   int32_t merges;
   int32_t most_parts;  // of a split row block
+  int32_t period;      // tiles of a share, about
 };
 // In a (row, query head) that has to be worked out again, the first element of one of
 // its quarters: a signalling NaN, which no arithmetic gives.

@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
       plan_read<ExtendShare>(p.plan + p.shares + (int64_t)share * sizeof(ExtendShare));
   const ExtendHeader header = plan_read<ExtendHeader>(p.plan);
   if (!extend_plan_fits(p, header)) return;
-  const int32_t window = header.window, sinks = header.sinks;
+  const int32_t window = header.window, sinks = header.sinks, period = header.period;
 
   const bool ring = p.c.window_size > 0;
   const int32_t max_pages = p.c.max_pages_per_seq;
@@ -223,6 +223,7 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     return lane;
   };
 
+  int32_t elapsed = 0;  // of the share, in tiles
   for (int32_t segment = mine.first; segment < mine.end; ++segment) {
     // ---- the segment ---------------------------------------------------------
     ExtendSegment seg = mine.segment;
@@ -234,8 +235,18 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     const int32_t first = prior + row0, last = first + rows - 1;  // positions
     const ExtendTiles tiles = extend_tiles(first, last, window, sinks, kTile);
     const int32_t tile_skip = tiles.window_tile - tiles.sink_tiles;
+    // Shares begin at any tile of a row block, and last equally long. A share visits its
+    // tiles from the one whose number is `elapsed` modulo the period on, and round to the
+    // ones before: so all shares that need a tile come to it at about the same time,
+    // and the later ones find it in their XCD's L2 (ten mixed sequences at 1 x 512 read 280
+    // MB past L2 instead of 750, 187 -> 182 us).
+    const int32_t ahead = elapsed - (tile_lo + tile_skip);
+    const int32_t turn = ahead - (ahead >= 0 ? ahead : ahead - period + 1) / period * period;
+    const int32_t start = turn < n_tiles ? tile_lo + turn : tile_lo;
+    const int32_t before_wrap = tile_lo + n_tiles - start;
+    elapsed += n_tiles + 6;  // with the block's own cost
     auto tile_key = [&](int it) __attribute__((always_inline)) -> int32_t {
-      const int32_t i = tile_lo + it;
+      const int32_t i = it + (it < before_wrap ? start : tile_lo - before_wrap);
       return (i < tiles.sink_tiles ? i : i + tile_skip) * kTile;
     };
 
