@@ -62,7 +62,8 @@ __device__ __forceinline__ int32_t block_cost(const ExtendGeometry &g, int32_t r
   return rows > g.wave_rows ? 6 : 3;
 }
 
-// One workgroup. The row blocks laid end to end are cut into shares of equal cost,
+// One workgroup, once a step for all layers: 13 to 17 us of dependent loads and prefix
+// sums. The row blocks laid end to end are cut into shares of equal cost,
 // wherever the cuts fall: cuts that kept a tile or four away from a block's ends, to
 // save partial sums, left shares of twice the mean where blocks are short (geometric
 // mean of 32 batches of 1 to 30 sequences 38 -> 34 us without).
@@ -221,7 +222,9 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
 // Item: 1 KiB of partial sums (256 fp32, four to a lane) and the parts of a split row
 // block that have them. A block of few parts is one wave's, kMergeBatch parts' loads
 // at a time; of many, the four waves' of a workgroup, each a quarter of the parts.
-// Parts are folded in a fixed order either way.
+// Parts are folded in a fixed order either way. Bound by the partial sums' bytes, 84 MB
+// in 22 us for ten mixed sequences at 1 x 512 (3.8 TB/s), and by its launch and three
+// dependent loads where there are few (4 us).
 constexpr int kMergeThreads = 256;
 constexpr int kMergeWaves = kMergeThreads / kWave;
 constexpr int kMergeGrid = 2048;
@@ -248,7 +251,7 @@ struct MergeState {
 
 // A (row, query head) from the keys that it sees alone, by one wave, kAgainKeys at a
 // time: for columns that an infinity or NaN of V got into, which may be of a key that
-// they do not see. For those only: a wave reads about 10 GB/s.
+// they do not see. For those only: all of 2048 rows after 6144 keys take 0.1 s.
 constexpr int kAgainKeys = 4;
 template <int kDim>
 __device__ __forceinline__ void extend_again(int32_t segment, int32_t row, int32_t qh) {

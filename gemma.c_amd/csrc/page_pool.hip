@@ -53,8 +53,8 @@ __device__ __forceinline__ SlotRange slot_range(const PoolParams &p, int32_t lo,
 }
 
 // ---- release --------------------------------------------------------------
-// One thread per table entry; what is read and written is a few kilobytes and
-// the launch is its time.
+// One thread per table entry; what is read and written is a few kilobytes (64
+// sequences of 512 pages: 128 KiB) and the launch is its time, 2 us.
 __global__ __launch_bounds__(256) void release_pages_kernel(
     PoolParams p, const int32_t *__restrict__ first_position,
     const int32_t *__restrict__ end_position, int64_t entries) {
@@ -155,7 +155,9 @@ __device__ __forceinline__ int32_t find_free(const PoolParams &p, int32_t from, 
 // ---- reserve ----------------------------------------------------------------
 // One workgroup: the order of the pages handed out is the order of the entries.
 // The entries of all ranges form one list (offsets by a prefix sum over the
-// sequences), read twice: to count what is missing, then to fill it.
+// sequences), read twice: to count what is missing, then to fill it. The chain of
+// lengths, table, counts and table again is its time, 3.0 us for 5 sequences and 3.7
+// for 64 of 512 pages.
 struct ReserveLds {
   int32_t offset[kPoolBatch + 1];  // of a sequence's entries in the list
   int32_t first[kPoolBatch];       // its first table slot
@@ -424,7 +426,9 @@ constexpr int kCopyPacks = kCopyThreads * kCopyUnroll;  // 16-byte packs per wor
 // branch's table says where to, what the parent's length leaves in a begun page
 // how much. All loads of a piece are in flight before its first store. In a
 // full-length cache the first layer's workgroups of a branch also share its
-// parent's whole pages.
+// parent's whole pages. A ring of 1024 tokens in 40 layers of 8 x 256 (713 MB read and
+// written): 139 us, 5.1 TB/s, the rate of a large copy; a branch's begun pages are
+// few bytes and the launch is their time (18 of 1 x 512: 6.4 us).
 __global__ __launch_bounds__(kCopyThreads) void fork_copy_kernel(ForkParams f, uint16_t *cache_k,
                                                                  uint16_t *cache_v, int32_t pieces,
                                                                  int32_t slots) {
@@ -498,7 +502,10 @@ constexpr int kStatusList = 1, kStatusUnmapped = 2, kStatusShared = 3;
 // a batch at a time: every load of a batch has arrived before its first store,
 // and a later batch's sources lie behind everything that was stored before
 // (kept[j] > kept[i] >= first + i for j > i), so nothing is overwritten unread and
-// the next batch's loads go out ahead of the stores.
+// the next batch's loads go out ahead of the stores. Four requests that keep 3001
+// rows each in 8 layers of 1 x 512 (393 MB): 92 us, 4.3 TB/s of 4.9 for a large copy,
+// the rest being the wait of a batch for its last load; 7 of 32 drafts of 8 sequences
+// in 10 layers of 8 x 256: 11 us, the chain of list, table, row and store.
 __global__ __launch_bounds__(kCompactThreads) void compact_kernel(CompactParams p) {
   __shared__ int32_t s_src[kCompactList], s_dst[kCompactList];
   __shared__ int32_t s_error;

@@ -213,8 +213,9 @@ hipError_t gemma4_flash_attention_prefill_chunk_paged_bf16_ws(
 // no initialisation; sizes for the largest batch_size and total_rows of a program
 // serve its smaller calls. Calls that share a workspace must not overlap; a plan
 // may be read by several. Offsets that do not ascend or pass total_rows are
-// clamped to it, a negative prior length counts as 0: such a plan attends to the
-// wrong keys but reads and writes within the tensors. Rows that no sequence
+// clamped to it, a negative prior length counts as 0 and one past a full-length
+// table's end as that: such a plan attends to the wrong keys but reads and writes
+// within the tensors. Rows that no sequence
 // holds (total_rows past the last offset) are left as they were. batch_size is at
 // most 4096 and config.batch_size, total_rows 2^24, num_pages * page_size below
 // 2^31 (sizes outside: 0 bytes). A key that a row does not see has no part in it,
