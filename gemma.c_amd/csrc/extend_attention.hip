@@ -11,9 +11,6 @@
 namespace gemma4 {
 namespace {
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWaves = kPlanThreads / kWave;
-
 struct PlanParams {
   char *plan;
   int32_t shares, segments, merges;
@@ -32,7 +29,7 @@ struct Max {
 };
 // Inclusive prefix of one value per thread over the workgroup; the last
 // thread's in `total`.
-template <class T, class F>
+template <int kWaves, class T, class F>
 __device__ __forceinline__ T block_prefix(T x, T &total, T *waves, F f) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -44,7 +41,7 @@ __device__ __forceinline__ T block_prefix(T x, T &total, T *waves, F f) {
   __syncthreads();
   T head = waves[0], all = waves[0];
 #pragma unroll
-  for (int w = 1; w < kPlanWaves; ++w) {
+  for (int w = 1; w < kWaves; ++w) {
     if (w < wave) head = f(head, waves[w]);
     all = f(all, waves[w]);
   }
@@ -62,17 +59,20 @@ __device__ __forceinline__ int32_t block_cost(const ExtendGeometry &g, int32_t r
   return rows > g.wave_rows ? 6 : 3;
 }
 
-// One workgroup, once a step for all layers: 13 to 17 us of dependent loads and prefix
-// sums. The row blocks laid end to end are cut into shares of equal cost,
+// One workgroup, once a step for all layers: 10 to 14 us of dependent loads, barriers
+// and prefix sums. The row blocks laid end to end are cut into shares of equal cost,
 // wherever the cuts fall: cuts that kept a tile or four away from a block's ends, to
 // save partial sums, left shares of twice the mean where blocks are short (geometric
 // mean of 32 batches of 1 to 30 sequences 38 -> 34 us without).
-__global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p) {
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void extend_plan_kernel(PlanParams p) {
+  constexpr int kWaves = kThreads / kWave;
   __shared__ int32_t s_begin[kExtendBatch + 1];   // first row of a sequence
   __shared__ int32_t s_blocks[kExtendBatch + 1];  // row blocks before it
+  __shared__ int32_t s_prior[kExtendBatch];       // keys in the cache
   __shared__ int32_t s_share[kPlanShares + 1];    // first segment of a share
-  __shared__ int64_t s_waves[kPlanWaves];
-  __shared__ int32_t s_waves32[kPlanWaves];
+  __shared__ int64_t s_waves[kWaves];
+  __shared__ int32_t s_waves32[kWaves];
   __shared__ int32_t s_parts;
   const int t = threadIdx.x;
   auto *shares_at = reinterpret_cast<ExtendShare *>(p.plan + p.shares);
@@ -83,22 +83,23 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
   // say, no row belongs to two sequences and the sections above hold the plan.
   if (t == 0) s_parts = 0;
   int32_t reach = 0;
-  for (int32_t b0 = 0; b0 <= p.batch; b0 += kPlanThreads) {
+  for (int32_t b0 = 0; b0 <= p.batch; b0 += kThreads) {
     const int32_t b = b0 + t;
     int32_t last;
     const int32_t own = b <= p.batch ? min(max(p.row_offsets[b], 0), p.total_rows) : 0;
-    const int32_t top = max(block_prefix(own, last, s_waves32, Max()), reach);
+    if (b < p.batch) s_prior[b] = min(max(p.prior_lengths[b], 0), p.max_prior);
+    const int32_t top = max(block_prefix<kWaves>(own, last, s_waves32, Max()), reach);
     if (b <= p.batch) s_begin[b] = top;
     reach = max(reach, last);
   }
   __syncthreads();
   int32_t n_blocks = 0;
-  for (int32_t b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+  for (int32_t b0 = 0; b0 < p.batch; b0 += kThreads) {
     const int32_t b = b0 + t;
     int32_t all;
     const int32_t own =
         b < p.batch ? (s_begin[b + 1] - s_begin[b] + p.g.rows - 1) / p.g.rows : 0;
-    const int32_t sum = block_prefix(own, all, s_waves32, Sum());
+    const int32_t sum = block_prefix<kWaves>(own, all, s_waves32, Sum());
     if (b < p.batch) s_blocks[b] = n_blocks + sum - own;
     n_blocks += all;
   }
@@ -126,38 +127,39 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     const int32_t at = j - s_blocks[lo], blocks = s_blocks[lo + 1] - s_blocks[lo];
     r.row0 = (at % 2 == 0 ? at / 2 : blocks - 1 - at / 2) * p.g.rows;
     r.rows = min(s_begin[lo + 1] - s_begin[lo] - r.row0, p.g.rows);
-    r.prior = min(max(p.prior_lengths[lo], 0), p.max_prior);
+    r.prior = s_prior[lo];
     const int32_t first = r.prior + r.row0;
     r.tiles = extend_tiles(first, first + r.rows - 1, p.window, p.sinks, p.g.tile).count;
     r.cost = (int64_t)r.tiles + block_cost(p.g, r.rows);
     return r;
   };
+  const Block own_block = block_of(t);
   int64_t cost = 0;
-  for (int32_t j0 = 0; j0 < n_blocks; j0 += kPlanThreads) {
+  for (int32_t j0 = 0; j0 < n_blocks; j0 += kThreads) {
     int64_t all;
-    block_prefix(block_of(j0 + t).cost, all, s_waves, Sum());
+    block_prefix<kWaves>(j0 == 0 ? own_block.cost : block_of(j0 + t).cost, all, s_waves, Sum());
     cost += all;
   }
   const int32_t shares =
       (int32_t)min((int64_t)p.g.shares, max(cost / kShareTiles, (int64_t)1));
   // Cut k of 1 .. shares - 1 lies at this cost. Every thread evaluates the same
   // expression, so the blocks agree on it.
-  const double step = (double)cost / (double)shares;
+  const double step = (double)cost / (double)shares, per_step = 1.0 / step;
   auto cut_at = [&](int32_t k) { return (int64_t)((double)k * step); };
 
   int64_t before = 0;                        // cost of the blocks of earlier rounds
   int64_t counts = 0;                        // their segments, partial and merged rows
-  for (int32_t j0 = 0; j0 < n_blocks; j0 += kPlanThreads) {
-    const Block r = block_of(j0 + t);
+  for (int32_t j0 = 0; j0 < n_blocks; j0 += kThreads) {
+    const Block r = j0 == 0 ? own_block : block_of(j0 + t);
     int64_t all;
-    const int64_t end = before + block_prefix(r.cost, all, s_waves, Sum());
+    const int64_t end = before + block_prefix<kWaves>(r.cost, all, s_waves, Sum());
     const int64_t begin = end - r.cost;
     before += all;
     const int32_t ahead = block_cost(p.g, r.rows);
     // f(cut k, the tile it lies at: 0 is no cut of the block)
     auto for_cuts = [&](auto &&f) {
       if (r.rows == 0) return;
-      int32_t k = max((int32_t)((double)begin / step), 1);
+      int32_t k = max((int32_t)((double)begin * per_step), 1);  // about: put right here
       while (k > 1 && cut_at(k - 1) >= begin) --k;
       while (k < shares && cut_at(k) < begin) ++k;
       for (; k < shares && cut_at(k) < end; ++k) {
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
     const int64_t own = (int64_t)parts << 32 |
                         (parts > 1 ? (int64_t)(parts * stride) << 16 | stride : (int64_t)0);
     int64_t sums;
-    const int64_t at = counts + block_prefix(own, sums, s_waves, Sum()) - own;
+    const int64_t at = counts + block_prefix<kWaves>(own, sums, s_waves, Sum()) - own;
     counts += sums;
     const int32_t segment = (int32_t)(at >> 32);
     const int32_t partial = (int32_t)(at >> 16) & 0xFFFF, merge = (int32_t)at & 0xFFFF;
@@ -203,10 +205,10 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(PlanParams p)
   }
   const int32_t n_segments = (int32_t)(counts >> 32);
   if (t == 0) s_share[0] = 0;
-  for (int32_t k = max(shares, 1) + t; k <= p.g.shares; k += kPlanThreads) s_share[k] = n_segments;
+  for (int32_t k = max(shares, 1) + t; k <= p.g.shares; k += kThreads) s_share[k] = n_segments;
   __threadfence_block();
   __syncthreads();
-  for (int32_t k = t; k < p.g.shares; k += kPlanThreads) {
+  for (int32_t k = t; k < p.g.shares; k += kThreads) {
     ExtendShare s = {s_share[k], s_share[k + 1], {}, {}};
     if (s.first < s.end) s.segment = segments[s.first];
     shares_at[k] = s;
@@ -559,7 +561,13 @@ extern "C" hipError_t gemma4_flash_attention_extend_plan(
   // to stay below 2^31 with the new rows.
   p.max_prior = (int32_t)std::min<int64_t>(config.window_size > 0 ? 0x7fffffff : capacity,
                                            0x7fffffff - total_rows - 256);
-  hipLaunchKernelGGL(extend_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
+  // A thread per row block, where that is so: barriers of four waves instead of 16 (one
+  // token's plan 14.1 -> 10.4 us, 24 tokens' 17.5 -> 13.9).
+  if (l.max_segments - g.shares <= 256) {
+    hipLaunchKernelGGL(extend_plan_kernel<256>, dim3(1), dim3(256), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL(extend_plan_kernel<1024>, dim3(1), dim3(1024), 0, stream, p);
+  }
   return hipGetLastError();
 }
 
