@@ -1,31 +1,45 @@
 // The rows of a ragged extension batch on bf16 MFMA, gfx950: one share of the
 // plan's segments per workgroup.
 //
-// Formulation: S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_32x32x16_bf16 on
-// blocks of 32 keys. A wave owns 32 columns: (row, query head) pairs of the KV
-// head, 16 rows x 2 heads at 8 x 256, 2 rows x 16 heads at 1 x 512, so that either
-// geometry keeps a full MFMA and a workgroup of four waves reads every key once
-// for 128 columns. In the accumulator lane l holds column l % 32 and 16 of a
-// block's keys (or dims): a column's maximum needs one exchange (lane ^ 32), the
-// rescale is a per-lane factor, and P^T is the second product's operand as it
-// stands, its key order {4h .. 4h+3, 8+4h .. 8+4h+3} per 16 keys being the order in
-// which V^T is read (ds_read_b64_tr_b16).
+// Formulation: S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_32x32x16_bf16 on tiles
+// of 32 keys. A workgroup of four waves has 128 columns, (row, query head) pairs of
+// the KV head: 16 rows x 2 heads per wave at 8 x 256, 2 rows x 16 heads at 1 x 512.
+// A wave scores its own 32 columns over all dims, with its Q^T in registers. In the
+// accumulator lane l holds column l % 32 and 16 of the keys: a column's maximum
+// needs one exchange (lane ^ 32), and the weights leave in the second product's
+// operand order, {4h .. 4h+3, 8+4h .. 8+4h+3} per 16 keys, in which V^T is read
+// (ds_read_b64_tr_b16). The second product is split by dims instead: the waves trade
+// their weights through LDS (4 KiB a tile each) and each adds up a quarter of the
+// dims for all 128 columns, so that V is read from LDS once per workgroup and not
+// once per wave. Where a block has one wave's rows at most, the first wave scores and
+// all four add up.
 //
-// Keys stream in tiles of 32 through LDS stages (four of 16 KiB each of K and V at
-// 8 x 256, two of 32 KiB at 1 x 512), copied by the waves themselves
-// (global_load_lds) from addresses their lanes resolved an iteration earlier: a
-// page-table entry per key, any page size, the packed new rows behind the cached
-// ones. Keys that no row of the block sees, that no page maps, or past the
-// segment's tiles are copied from a row of zeros, so nothing in such a place is
-// ever multiplied. Rows land swizzled by 16-byte chunks (K row k, chunk c at c ^ (k
-// & 15); V at c ^ ((k & 3) << 2)), which keeps the operand reads free of bank
-// conflicts.
+// Keys stream in tiles through LDS stages (four of 16 KiB each of K and V at 8 x 256,
+// two of 32 KiB at 1 x 512), copied by the waves themselves (global_load_lds) from row
+// addresses that their lanes resolve for eight tiles at once: a page-table entry per
+// key, any page size, the packed new rows behind the cached ones. Keys that no row of
+// the block sees, that no page maps, or past the segment's tiles are copied from a
+// row of zeros, so nothing in such a place is ever multiplied. Rows land swizzled by
+// 16-byte chunks (K row k, chunk c at c ^ (k & 15); V at c ^ ((k & 3) << 2)): no bank
+// conflict in the operand reads (counted: 0).
 //
 // With one wave per SIMD nothing else fills the matrix cores while a wave does its
 // softmax, so iteration t interleaves the softmax of tile t with the second
 // product of tile t - 1. Registers: at 1 x 512 the accumulators are all 256 AGPRs
 // (the second product is asm, the first one's results stay in VGPRs by a build flag
 // for this file), Q^T half of the VGPRs.
+//
+// Measured, 2048 rows after 6144 keys: at 1 x 512 459 us with the merge, 1.05 PFLOP/s
+// (a large library product reaches 1.30), at 8 x 256 284 us, 0.85. A tile takes 3740
+// clocks at 1 x 512 and 2550 at 8 x 256, of which the matrix cores work 2048 and 1024;
+// the rest is what the one wave per SIMD issues besides (some 430 and 290 instructions,
+// the copies among them 340 clocks and 90) and the LDS latency behind its barrier. The
+// clock itself falls to 1.95 GHz of
+// 2.4 under this load, and forms with fewer or better spread instructions (scalar row
+// addresses, half of the copies under each product with a barrier between) changed
+// clocks and clock rate against each other and not the time. Batches of single tokens
+// stream at 4.1 to 5.1 TB/s with start-up and merge (24 sequences at 1 x 512, 302 MB:
+// 73 us).
 #include "extend_common.hpp"
 #include "extend_rows.hpp"
 #include "lds_copy.hpp"
