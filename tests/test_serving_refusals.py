@@ -1,6 +1,9 @@
 """What the ragged extension attention and the page pool refuse before any
 launch: bad sizes, null and misaligned pointers, windows that a cache cannot
 hold. Runs without a GPU: no call here reaches the device."""
+import subprocess
+from pathlib import Path
+
 import pytest
 
 import gemma_kv as gk
@@ -136,3 +139,16 @@ def test_compact_refuses(what):
 
 def test_nothing_to_do_is_a_success():
     assert fork(fork_count=0) == OK and compact(sequence_count=0) == OK
+
+
+def test_c_caller(tmp_path):
+    """The same interface from plain C, compiled with gcc against the headers."""
+    repo = Path(__file__).resolve().parent.parent
+    lib = repo / "gemma.c_amd" / "gemma_kv"
+    exe = tmp_path / "serving_caller"
+    cmd = ["gcc", "-std=c11", "-Wall", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", f"-I{repo / 'include'}",
+           str(repo / "tests" / "cpp" / "serving_caller.c"), f"-L{lib}", "-lgemma4_kv", f"-Wl,-rpath,{lib}",
+           "-o", str(exe)]
+    proc = subprocess.run(cmd, capture_output=True, text=True, timeout=300)
+    assert proc.returncode == 0, proc.stderr
+    assert "serving caller ok" in subprocess.run([str(exe)], capture_output=True, text=True, timeout=60).stdout
