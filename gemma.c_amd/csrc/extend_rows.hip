@@ -30,7 +30,7 @@
 // for this file), Q^T half of the VGPRs.
 //
 // Measured, 2048 rows after 6144 keys: at 1 x 512 459 us with the merge, 1.05 PFLOP/s
-// (a large library product reaches 1.30), at 8 x 256 284 us, 0.85. A tile takes 3740
+// (a large library product reaches 1.30), at 8 x 256 285 us, 0.84. A tile takes 3740
 // clocks at 1 x 512 and 2550 at 8 x 256, of which the matrix cores work 2048 and 1024;
 // the rest is what the one wave per SIMD issues besides (some 430 and 290 instructions,
 // the copies among them 340 clocks and 90) and the LDS latency behind its barrier. The
