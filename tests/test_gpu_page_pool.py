@@ -470,3 +470,59 @@ def test_a_cache_of_more_than_four_gigabytes(dev, heads, dim, pages):
     for x, r in zip((k, v), rows):
         assert torch.equal(x[:, pages - 2, 1:5], r[:, 1, [p - 64 for p in kept]])
         assert torch.equal(x[:, pages - 5], r[:, 1]) and torch.equal(x[:, pages - 3], r[:, 0])
+
+
+@pytest.mark.parametrize("window", [0, 37])
+@pytest.mark.parametrize("seed", range(10))
+def test_random_walk(dev, window, seed):
+    """Any of the operators in any order, refused calls among them, over many sequences
+    and a pool that runs short; table, counts, lengths and rows after every one."""
+    rng = np.random.default_rng(seed)
+    page = int(rng.choice([1, 3, 8, 16]))
+    max_pages = (window + 2 * page - 2) // page if window else int(rng.integers(1, 70))
+    batch = int(rng.integers(2, 60))
+    pages = int(rng.integers(max_pages, batch * max_pages + 2))
+    heads, dim = [(1, 8), (2, 24), (8, 256)][int(rng.integers(3))]
+    p, d = make(dev, layers=2, pages=pages, page=page, max_pages=max_pages, batch=batch, heads=heads, dim=dim,
+                window=window, seed=seed)
+    cap = max_pages * page
+    seen = set()
+    for turn in range(30):
+        kind = ["reserve", "release", "fork", "compact"][int(rng.integers(4))]
+        if kind == "reserve":
+            some = rng.random(batch) < 0.2
+            end = np.where(some, rng.integers(0, cap + (3 if rng.random() < 0.1 else 1), batch), p.lens)
+            first = np.minimum(p.lens, end) if window else np.zeros(batch, int)
+            got = d.reserve(first, end)
+            assert got == p.reserve(first, end), (turn, kind)
+            if got == 0:
+                p.lens[:] = np.maximum(p.lens, end)
+                d.lens.copy_(d.i32(p.lens))
+        elif kind == "release":
+            gone = rng.random(batch) < 0.3
+            first = np.where(gone, 0, p.lens)
+            d.release(first, [EVERYTHING] * batch)
+            p.release(first, [EVERYTHING] * batch)
+            p.lens[gone] = 0
+            d.lens.copy_(d.i32(p.lens))
+            got = 0
+        elif kind == "fork":
+            empty = [b for b in range(batch) if (p.table[b] < 0).all()]
+            n = int(rng.integers(1, 6))
+            held = [b for b in range(batch) if b not in empty] or [0]
+            children = [int(c) for c in rng.permutation(empty if empty and rng.random() < 0.9 else batch)[:n]]
+            parents = [int(x) for x in rng.choice(held, len(children))]
+            got = d.fork(parents, children)
+            assert got == p.fork(parents, children), (turn, kind)
+        else:
+            who = [int(b) for b in rng.permutation(batch)[:int(rng.integers(1, 5))]]
+            first = [int(rng.integers(0, max(int(p.lens[b]), 1))) for b in who]
+            kept = [sorted(int(x) for x in rng.choice(np.arange(f, max(int(p.lens[b]), f + 1)),
+                                                      int(rng.integers(0, max(int(p.lens[b]) - f, 1))), replace=False))
+                    for b, f in zip(who, first)]
+            got = d.compact(who, first, kept)
+            assert got == p.compact(who, first, kept), (turn, kind)
+            got = max(got)
+        seen.add((kind, got))
+        d.check((turn, kind))
+    assert len({kind for kind, _ in seen}) == 4, seen
