@@ -367,7 +367,7 @@ __global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendPa
   uint16_t mark = first_item < units ? marks_of(seg, first_item) : 0;
 
   // Where an item's values are: this lane's in the first part's sums and stats, and in
-  // the output (row -1: a column without a row).
+  // the output (out -1: a column without a row).
   struct Place {
     int64_t sum, stat, out;
     int32_t odd;   // the first part's words (all lanes' the same)
