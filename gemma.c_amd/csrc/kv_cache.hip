@@ -49,6 +49,9 @@ __device__ __forceinline__ int64_t append_row(const Gemma4KvCacheConfig &c,
 // One thread = one 16-byte pack of K and of V. Source rows are selected by
 // `row = row_base(t)`: for plain writes t itself; for the prefill tail policy
 // batch-major rows starting at `first_live` within each batch of `seq_len`.
+// ring_rows > 0: a ring's slots, fewer than the launch's rows. Threads come in no
+// order, so a row whose slot a later row of its sequence takes must not be stored:
+// where a sequence's rows follow each other that is the row `ring_rows` on.
 __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(
     uint16_t *__restrict__ cache_k, uint16_t *__restrict__ cache_v,
     Gemma4KvCacheConfig c, const int32_t *__restrict__ page_table,
@@ -56,7 +59,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(
     const int32_t *__restrict__ token_position, int32_t layer,
     const uint16_t *__restrict__ k, const uint16_t *__restrict__ v,
     int64_t total_packs, int32_t packs_per_token, int32_t rows_per_batch,
-    int32_t seq_len, int32_t first_live) {
+    int32_t seq_len, int32_t first_live, int32_t ring_rows) {
   const int64_t p = (int64_t)blockIdx.x * kAppendThreads + threadIdx.x;
   if (p >= total_packs) return;
   const int32_t t = (int32_t)(p / packs_per_token);
@@ -64,9 +67,13 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(
   // Map the launch row to its source row (identity unless the tail policy).
   const int32_t b = t / rows_per_batch;
   const int32_t src_row = b * seq_len + first_live + (t - b * rows_per_batch);
-  const int64_t dst_row = append_row(c, page_table, layer, token_batch[src_row],
-                                     token_position[src_row]);
+  const int32_t batch = token_batch[src_row], position = token_position[src_row];
+  const int64_t dst_row = append_row(c, page_table, layer, batch, position);
   if (dst_row < 0) return;
+  if (ring_rows > 0 && src_row + (int64_t)ring_rows < rows_per_batch) {
+    const int32_t newer = src_row + ring_rows;
+    if (token_batch[newer] == batch && token_position[newer] - (int64_t)position == ring_rows) return;
+  }
   const int64_t row_elems = (int64_t)c.num_heads * c.head_dim;
   const int64_t src = (int64_t)src_row * row_elems + (int64_t)within * kPackElems;
   const int64_t dst = dst_row * row_elems + (int64_t)within * kPackElems;
@@ -88,7 +95,7 @@ hipError_t launch_append(uint16_t *cache_k, uint16_t *cache_v,
                          const int32_t *token_batch, const int32_t *token_position,
                          int32_t rows, int32_t layer, const uint16_t *k,
                          const uint16_t *v, int32_t rows_per_batch,
-                         int32_t seq_len, int32_t first_live,
+                         int32_t seq_len, int32_t first_live, int32_t ring_rows,
                          hipStream_t stream) {
   const int32_t packs_per_token = c.num_heads * (c.head_dim / kPackElems);
   const int64_t total = (int64_t)rows * packs_per_token;
@@ -97,7 +104,7 @@ hipError_t launch_append(uint16_t *cache_k, uint16_t *cache_v,
   hipLaunchKernelGGL(kv_append_kernel, dim3((uint32_t)blocks), dim3(kAppendThreads),
                      0, stream, cache_k, cache_v, c, page_table, token_batch,
                      token_position, layer, k, v, total, packs_per_token,
-                     rows_per_batch, seq_len, first_live);
+                     rows_per_batch, seq_len, first_live, ring_rows);
   return hipGetLastError();
 }
 
@@ -210,13 +217,15 @@ hipError_t gemma4_kv_cache_write_bf16(
       d_k == nullptr || d_v == nullptr) {
     return hipErrorInvalidValue;
   }
+  const int64_t slots = (int64_t)config.max_pages_per_seq * config.page_size;
+  const bool laps = config.window_size > 0 && slots < token_count;
   return launch_append(reinterpret_cast<uint16_t *>(d_cache_k),
                        reinterpret_cast<uint16_t *>(d_cache_v), config,
                        d_page_table, d_token_batch, d_token_position,
                        token_count, layer, reinterpret_cast<const uint16_t *>(d_k),
                        reinterpret_cast<const uint16_t *>(d_v),
                        /*rows_per_batch=*/token_count, /*seq_len=*/0,
-                       /*first_live=*/0, stream);
+                       /*first_live=*/0, /*ring_rows=*/laps ? (int32_t)slots : 0, stream);
 }
 
 hipError_t gemma4_kv_cache_write_prefill_bf16(
@@ -245,7 +254,7 @@ hipError_t gemma4_kv_cache_write_prefill_bf16(
                        (int32_t)rows, layer,
                        reinterpret_cast<const uint16_t *>(d_k),
                        reinterpret_cast<const uint16_t *>(d_v), rows_per_batch,
-                       seq_len, first_live, stream);
+                       seq_len, first_live, /*ring_rows=*/0, stream);
 }
 
 }  // extern "C"

@@ -198,8 +198,9 @@ hipError_t gemma4_flash_attention_prefill_chunk_paged_bf16_ws(
 // window_size or j < sink_tokens (window_size 0: all of them): those at P and
 // after from the rows' own prepared k and v, earlier ones from the cache through
 // the page table; keys on unmapped pages are skipped. The cache is only read: the
-// caller writes the rows afterwards (gemma4_kv_cache_write_bf16), as for a prefill
-// chunk. Geometries 8 KV heads x 256 and 1 KV head x 512, 16 query heads.
+// caller writes the rows afterwards (gemma4_kv_cache_write_bf16, which takes packed k
+// and v; a sequence may bring more rows than its ring has slots). Geometries 8 KV heads
+// x 256 and 1 KV head x 512, 16 query heads.
 // window_size: 1 .. config.window_size over a sliding cache (whose ring must hold
 // that many slots; sink_tokens is 0 there, the ring has overwritten them); any
 // over a full-length one, where the pages between the sinks and the window may

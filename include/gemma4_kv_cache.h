@@ -105,6 +105,10 @@ int32_t gemma4_kv_cache_ensure_range_ptr(int32_t *page_table,
 // into the paged cache. Rows whose batch/position/page is out of range are
 // skipped on the device. token_count == 0 is a no-op success; bad geometry or
 // null pointers return hipErrorInvalidValue before any launch.
+// A sequence may bring more rows than its ring has slots (max_pages_per_seq *
+// page_size) where they follow each other in the call, at consecutive positions:
+// the newest of a slot stays. Other rows for one place (the same position twice, a
+// lap out of order) must not come in one call.
 hipError_t gemma4_kv_cache_write_bf16(
     gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cache_v, Gemma4KvCacheConfig config,
     const int32_t *d_page_table, const int32_t *d_token_batch,

@@ -556,3 +556,39 @@ def test_graphs_that_share_a_workspace(dev, heads, dim):
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
         assert torch.equal((a, b)[turn % 2].run(), want[turn % 2])
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+@pytest.mark.parametrize("page,window", [(16, 64), (1, 40), (64, 100)])
+def test_prompts_longer_than_the_ring(dev, heads, dim, page, window):
+    """Attend, append and attend again where prompts bring several laps of a ring at once,
+    beside short ones: the rows of the second step see the last of the first."""
+    import torch
+    first = [300, 1, 2 * window + 200, 0, 7]
+    b = Batch(dev, heads, dim, first, [0, 333, 50, 0, window], page=page, window=window, ring=True)
+    b.check(b.run())
+    # The second step's batch, its cache and table the first's: every slot mapped.
+    slots, i32 = b.max_pages, lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    pages = b.batch * slots
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).int().view(b.batch, slots)
+    c = Batch(dev, heads, dim, [3, 1, 30, 2, 9], [n + p for n, p in zip(first, b.prior)], page=page, window=window,
+              ring=True, seed=1)
+    ck, cv = (torch.full((1, pages, page, heads, dim), NAN, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    for i in range(b.batch):
+        for j in range(slots):
+            if int(b.table[i, j]) >= 0:
+                ck[:, table[i, j]], cv[:, table[i, j]] = b.ck[:, int(b.table[i, j])], b.cv[:, int(b.table[i, j])]
+    c.table = table.to(dev)
+    c.config = gk.make_config(1, pages, page, slots, b.batch, heads, dim, window)
+    who = i32([s for s, n in enumerate(first) for _ in range(n)])
+    where = [p + j for p, n in zip(b.prior, first) for j in range(n)]
+    gk.check(gk.kv_cache_write_bf16(ck, cv, c.config, c.table, who, i32(where), b.total, 0, b.k, b.v))
+    c.ck, c.cv = ck, cv
+    # What has to be there, row after row.
+    at = 0
+    for s, (n, p) in enumerate(zip(first, b.prior)):
+        for j in range(max(0, n - slots * page), n):
+            page_of, offset = int(table[s, (p + j) // page % slots]), (p + j) % page
+            assert torch.equal(ck[0, page_of, offset], b.k[at + j]) and torch.equal(cv[0, page_of, offset], b.v[at + j])
+        at += n
+    c.check(c.run())

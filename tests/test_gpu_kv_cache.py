@@ -116,3 +116,30 @@ def test_append_error_convention(dev):
     assert gk.kv_cache_write_bf16(buf, None, cfg, idx, idx, idx, 1, 0, buf, buf) == gk.HIP_ERROR_INVALID_VALUE
     bad = gk.make_config(1, 2, 4, 2, 1, 2, 12, 0)  # head_dim not a multiple of 8
     assert gk.kv_cache_write_bf16(buf, buf, bad, idx, idx, idx, 1, 0, buf, buf) == gk.HIP_ERROR_INVALID_VALUE
+
+
+@pytest.mark.parametrize("page,slots", [(1, 40), (16, 80), (64, 128)])
+def test_append_of_more_rows_than_the_ring_has_slots(dev, page, slots):
+    """Ragged rows that follow each other, several laps of the ring among them: of the
+    rows for one slot the newest stays, K and V, as when they are written in turn."""
+    rng = np.random.default_rng(slots)
+    heads, dim, layers = 8, 256, 2
+    lengths = [3 * slots + 7, 1, 0, slots, slots + 1, 5 * slots]
+    first = [11, 5000, 3, 0, 4 * slots - 1, 777]
+    cfg = cache_config(layers, len(lengths), page, slots // page, heads, dim, slots - page)
+    pt = rng.permutation(cfg[1]).astype(np.int32)
+    pt[4 * (slots // page)] = -1  # an unmapped page takes no row of any lap
+    token_batch = np.repeat(np.arange(len(lengths), dtype=np.int32), lengths)
+    token_pos = np.concatenate([f + np.arange(n) for f, n in zip(first, lengths)]).astype(np.int32)
+    # Rows that no sequence holds, behind the others.
+    token_batch, token_pos = np.append(token_batch, [-1, 0]).astype(np.int32), np.append(token_pos, [9, -1]).astype(np.int32)
+    tokens = len(token_pos)
+    k, v = (randn_bf16(rng, (tokens, heads, dim)) for _ in range(2))
+    exp_k, exp_v = (randn_bf16(rng, _cache_elems(cfg)) for _ in range(2))
+    ck, cv = to_dev(exp_k, dev), to_dev(exp_v, dev)
+    for t in range(tokens):
+        oracle.kv_cache_write(exp_k, exp_v, cfg, pt, token_batch[t:t + 1], token_pos[t:t + 1], 1, k[t:t + 1], v[t:t + 1])
+    gk.check(gk.kv_cache_write_bf16(ck, cv, gk.make_config(*cfg), to_dev(pt, dev), to_dev(token_batch, dev),
+                                    to_dev(token_pos, dev), tokens, 1, to_dev(k, dev), to_dev(v, dev)))
+    assert np.array_equal(from_dev_bf16(ck), exp_k)
+    assert np.array_equal(from_dev_bf16(cv), exp_v)
