@@ -495,7 +495,8 @@ struct CompactParams {
 constexpr int kCompactThreads = 1024;
 constexpr int kCompactList = 4096;   // rows whose places LDS holds at a time
 constexpr int kCompactUnroll = 4;
-constexpr int kStatusList = 1, kStatusUnmapped = 2, kStatusShared = 3;
+// A request that breaks several rules gets the lowest of their codes.
+constexpr int kStatusList = 1, kStatusUnmapped = 2, kStatusShared = 3, kStatusNone = 4;
 
 // Workgroup (request, slice of a row, layer x {K, V}). Kept token j moves from
 // position kept[j] to first + j <= kept[j], in place. Rows are taken in order,
@@ -519,11 +520,13 @@ __global__ __launch_bounds__(kCompactThreads) void compact_kernel(CompactParams 
   if (t == 0)
     s_error = b >= 0 && b < p.c.batch_size && first >= 0 && begin >= 0 && end >= begin &&
                       end <= p.total && first <= 0x7fffffff - n
-                  ? 0 : kStatusList;
+                  ? kStatusNone : kStatusList;
   __syncthreads();
   int32_t error = s_error;
+  const bool readable = error == kStatusNone;
+  __syncthreads();  // every wave has read it before any adds what it finds
   // One request per sequence.
-  if (error == 0) {
+  if (readable) {
     for (int32_t j = t; j < p.count; j += kCompactThreads)
       if (j != i && p.sequences[j] == b) error = kStatusList;
   }
@@ -537,20 +540,20 @@ __global__ __launch_bounds__(kCompactThreads) void compact_kernel(CompactParams 
     if (page < 0 || page >= p.c.num_pages) return -1;
     return (int64_t)page * p.c.page_size + (position - (int32_t)logical * p.c.page_size);
   };
-  if (s_error == 0) {
+  if (readable) {
     for (int32_t j = t; j < n; j += kCompactThreads) {
       const int32_t from = kept[j], to = first + j;
       if (from < to || (j > 0 && kept[j - 1] >= from) ||
           (p.c.window_size > 0 ? from - first >= capacity : from >= capacity)) {
-        error = max(error, kStatusList);
+        error = kStatusList;
         continue;
       }
       int32_t src_page, dst_page;
       const int64_t src = row_of(from, src_page), dst = row_of(to, dst_page);
       if (src < 0 || dst < 0) {
-        error = max(error, kStatusUnmapped);
+        error = min(error, kStatusUnmapped);
       } else if (from != to && p.refs != nullptr && p.refs[dst_page] > 1) {
-        error = max(error, kStatusShared);
+        error = min(error, kStatusShared);
       }
       if (j < kCompactList) {
         s_src[j] = (int32_t)src;
@@ -558,11 +561,11 @@ __global__ __launch_bounds__(kCompactThreads) void compact_kernel(CompactParams 
       }
     }
   }
-  if (error != 0) atomicMax(&s_error, error);
+  if (error != kStatusNone) atomicMin(&s_error, error);
   __syncthreads();
   error = s_error;
-  if (t == 0 && slice == 0 && blockIdx.y == 0) p.status[i] = error;
-  if (error != 0) return;
+  if (t == 0 && slice == 0 && blockIdx.y == 0) p.status[i] = error == kStatusNone ? kStatusOk : error;
+  if (error != kStatusNone) return;
 
   const int32_t row_packs = p.c.num_heads * p.c.head_dim / kPackElems;
   const int32_t c0 = (int32_t)((int64_t)row_packs * slice / p.slices);

@@ -194,8 +194,8 @@ hipError_t gemma4_kv_cache_fork_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cach
 // that would write to a page with more than one reference is refused.
 // d_status[i]: 0, or with the sequence's rows unchanged 1 (a list, sequence or
 // position against these rules, two requests for one sequence), 2 (a page is
-// unmapped) or 3 (a destination page is shared). total_kept is the length of
-// d_kept_positions. The table, the counts and the lengths stay as they are.
+// unmapped) or 3 (a destination page is shared), the lowest where several hold.
+// total_kept is the length of d_kept_positions. The table, the counts and the lengths stay as they are.
 // sequence_count == 0 is a no-op success; sequence_count <= batch_size.
 hipError_t gemma4_kv_cache_compact_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cache_v,
                                         Gemma4KvCacheConfig config, const int32_t *d_page_table,

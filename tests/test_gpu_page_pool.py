@@ -526,3 +526,26 @@ def test_random_walk(dev, window, seed):
         seen.add((kind, got))
         d.check((turn, kind))
     assert len({kind for kind, _ in seen}) == 4, seen
+
+
+def test_compact_requests_that_break_several_rules(dev):
+    """The lowest code, on every run, wherever in a long list the rules are broken."""
+    n, page = 4500, 4
+    mp = n // page
+    p, _ = make(dev, layers=1, pages=6 * mp, max_pages=mp, batch=6, dim=8, page=page)
+    assert p.reserve([0] * 6, [n] * 6) == 0
+    for b in range(6):
+        p.refs[p.table[b, 30]] = 2            # positions 120 .. 123
+    for b in (0, 1, 2, 4):
+        p.refs[p.table[b, 700]] = 0
+        p.table[b, 700] = -1                  # positions 2800 .. 2803
+    kept = [list(range(1, n)) for _ in range(6)]
+    kept[1][4000] = 4000                      # not behind the one before
+    kept[3][0] = -1
+    kept[4] = [2800, 2801] + list(range(4000, 4400))
+    d = OnDevice(p, dev)
+    seqs, first = [0, 1, 2, 3, 4, 5], [0, 0, 0, 0, 100, 0]
+    for turn in range(20):
+        assert d.compact(seqs, first, kept) == p.compact(seqs, first, kept) == [2, 1, 2, 1, 2, 3]
+    assert d.compact([2, 5, 2], [0, 0, 0], [kept[2], kept[5], [5]]) == [1, 3, 1]
+    d.check()
