@@ -22,7 +22,7 @@ constexpr int kPoolRound = kPoolThreads * kPoolUnroll;    // items per round
 constexpr int kPoolBatch = 4096;                          // sequences at most
 constexpr int kPoolList = 16384;                          // free pages held in LDS at a time
 
-constexpr int kStatusOk = 0, kStatusPages = 1, kStatusArguments = 2;
+constexpr int kStatusOk = 0, kStatusPages = 1, kStatusArguments = 2, kStatusWritten = 3;
 
 struct PoolParams {
   int32_t *page_table;
@@ -155,15 +155,18 @@ __device__ __forceinline__ int32_t find_free(const PoolParams &p, int32_t from, 
 // ---- reserve ----------------------------------------------------------------
 // One workgroup: the order of the pages handed out is the order of the entries.
 // The entries of all ranges form one list (offsets by a prefix sum over the
-// sequences), read twice: to count what is missing, then to fill it. The chain of
-// lengths, table, counts and table again is its time, 3.0 us for 5 sequences and 3.7
-// for 64 of 512 pages.
+// sequences), read twice: to count what is missing and shared, then to fill it. The
+// chain of lengths, table, counts and table again is its time: 6.2 us for 5 sequences
+// of which 2 change, 8.0 for 64 of 512 pages of which 10 do; 0.4 us of it for the
+// counts of the mapped pages.
 struct ReserveLds {
   int32_t offset[kPoolBatch + 1];  // of a sequence's entries in the list
   int32_t first[kPoolBatch];       // its first table slot
+  bool written[kPoolBatch];        // its range begins behind position 0
   int32_t list[kPoolList];
   RankScratch scratch;
   int32_t bad;
+  int32_t shared;
 };
 __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
     PoolParams p, const int32_t *__restrict__ first_position,
@@ -171,7 +174,7 @@ __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
   __shared__ ReserveLds lds;
   const int t = threadIdx.x, lane = t & 63;
   const int32_t batch = p.c.batch_size, pages = p.c.max_pages_per_seq;
-  if (t == 0) lds.bad = 0;
+  if (t == 0) lds.bad = lds.shared = 0;
   __syncthreads();
   for (int32_t b = t; b < batch; b += kPoolThreads) {
     const int32_t first = first_position[b], end = end_position[b];
@@ -187,6 +190,7 @@ __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
     if (!r.ok) lds.bad = 1;
     lds.first[b] = r.first;
     lds.offset[b] = r.count;
+    lds.written[b] = first > 0;
   }
   __syncthreads();
   if (lds.bad) {
@@ -214,7 +218,7 @@ __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
   const int32_t items = lds.offset[batch];
   // Table index of an item: its sequence is the last one that begins at or
   // before it.
-  auto entry_of = [&](int32_t item) -> int64_t {
+  auto entry_of = [&](int32_t item, bool &written) -> int64_t {
     int32_t lo = 0, hi = batch;
     while (hi - lo > 1) {
       const int32_t mid = (lo + hi) >> 1;
@@ -222,21 +226,30 @@ __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
     }
     int32_t slot = lds.first[lo] + (item - lds.offset[lo]);
     if (slot >= pages) slot -= pages;
+    written = lds.written[lo];
     return (int64_t)lo * pages + slot;
   };
-  // f(table index or -1, rank of a missing entry or -1) for every item; returns
-  // how many are missing.
-  auto for_missing = [&](auto &&f) -> int32_t {
+  // f(table index, rank) for every missing entry; returns how many there are. `held`
+  // (page) is whether a page that a range's rows will be written to is another's too.
+  auto for_missing = [&](auto &&f, auto &&held) -> int32_t {
     int32_t missing = 0;
+    bool shared = false;
     for (uint32_t base = 0; base < (uint32_t)items; base += kPoolRound) {
       int64_t at[kPoolUnroll];
-      bool flag[kPoolUnroll];
+      int32_t page[kPoolUnroll];
+      bool flag[kPoolUnroll], written[kPoolUnroll];
       int32_t rank[kPoolUnroll];
 #pragma unroll
       for (int u = 0; u < kPoolUnroll; ++u) {
         const uint32_t item = base + u * kPoolThreads + t;
-        at[u] = item < (uint32_t)items ? entry_of((int32_t)item) : -1;
-        flag[u] = at[u] >= 0 && p.page_table[at[u]] < 0;
+        written[u] = false;
+        at[u] = item < (uint32_t)items ? entry_of((int32_t)item, written[u]) : -1;
+        page[u] = at[u] >= 0 ? p.page_table[at[u]] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < kPoolUnroll; ++u) {
+        flag[u] = page[u] < 0;
+        if (written[u] && page[u] >= 0 && page[u] < p.c.num_pages) shared |= held(page[u]);
       }
       const int32_t found = round_ranks(flag, rank, lds.scratch);
 #pragma unroll
@@ -244,12 +257,14 @@ __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
         if (flag[u]) f(at[u], missing + rank[u]);
       missing += found;
     }
+    if (shared) lds.shared = 1;
     return missing;
   };
-  const int32_t wanted = for_missing([](int64_t, int32_t) {});
+  const int32_t wanted =
+      for_missing([](int64_t, int32_t) {}, [&](int32_t page) { return p.refs[page] > 1; });
   const int32_t seen = find_free(p, 0, wanted, load_refs(p, 0), lds.list, lds.scratch);
-  if (seen < wanted) {
-    if (t == 0) *status = kStatusPages;
+  if (lds.shared || seen < wanted) {  // find_free ends with a barrier
+    if (t == 0) *status = lds.shared ? kStatusWritten : kStatusPages;
     return;
   }
   if (t == 0) *status = kStatusOk;
@@ -262,7 +277,7 @@ __global__ __launch_bounds__(kPoolThreads) void reserve_pages_kernel(
       const int32_t page = lds.list[rank];
       p.page_table[at] = page;
       p.refs[page] = 1;
-    });
+    }, [](int32_t) { return false; });
     __threadfence_block();
     __syncthreads();
   }

@@ -156,9 +156,15 @@ hipError_t gemma4_kv_cache_release_pages(int32_t *d_page_table, int32_t *d_page_
 
 // Takes pages: for every sequence b < batch_size, every unmapped page that holds
 // a position of [d_first_position[b], d_end_position[b]) gets a free page with
-// one reference. *d_status: 0, or with nothing changed 1 (not enough free pages)
-// or 2 (a negative first position of a range, or one past a full-length table's
-// end).
+// one reference. A range that begins behind position 0 is where a sequence goes on:
+// its rows will be written, so no page of it may be shared; one from 0 on may hold
+// shared pages. *d_status: 0, or with nothing changed 1 (not enough free pages), 2 (a
+// negative first position of a range, or one past a full-length table's end; comes
+// before the others) or 3 (a page that will be written is mapped more than once; comes
+// before 1). That is a branch, or its parent, that was shortened into the pages they
+// share: release what lies behind its new length, then, if it ends within a page, fork
+// it to an empty sequence, which gets that page as its own, release it whole, and go
+// on with the new one.
 hipError_t gemma4_kv_cache_reserve_pages(int32_t *d_page_table, int32_t *d_page_refs,
                                          Gemma4KvCacheConfig config,
                                          const int32_t *d_first_position,
@@ -191,7 +197,8 @@ hipError_t gemma4_kv_cache_fork_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cach
 // verifies n drafts needs n slots more than its window.) A request's positions ascend strictly, none lies before its new
 // place, and for a sliding cache all lie within the ring's slots of the first
 // position. d_page_refs may be null where no page is shared; otherwise a request
-// that would write to a page with more than one reference is refused.
+// that would write to a page with more than one reference is refused (a way on: see
+// gemma4_kv_cache_reserve_pages).
 // d_status[i]: 0, or with the sequence's rows unchanged 1 (a list, sequence or
 // position against these rules, two requests for one sequence), 2 (a page is
 // unmapped) or 3 (a destination page is shared), the lowest where several hold.

@@ -549,3 +549,113 @@ def test_compact_requests_that_break_several_rules(dev):
         assert d.compact(seqs, first, kept) == p.compact(seqs, first, kept) == [2, 1, 2, 1, 2, 3]
     assert d.compact([2, 5, 2], [0, 0, 0], [kept[2], kept[5], [5]]) == [1, 3, 1]
     d.check()
+
+
+def test_reserve_refuses_shared_pages_that_will_be_written(dev):
+    """A branch, or its parent, that was shortened into their shared pages."""
+    p, _ = make(dev, batch=6, max_pages=6, pages=14, page=4)
+    p.lens[0] = 18
+    assert p.reserve([0] * 6, [18] + [0] * 5) == 0
+    d = OnDevice(p, dev)
+    assert d.fork([0, 0], [1, 2]) == p.fork([0, 0], [1, 2]) == 0
+    d.release([EVERYTHING, 10] + [EVERYTHING] * 4, [EVERYTHING] * 6)
+    p.release([EVERYTHING, 10] + [EVERYTHING] * 4, [EVERYTHING] * 6)
+    p.lens[1] = 10
+    d.lens.copy_(d.i32(p.lens))
+    d.check()
+    nothing, one = [0] * 6, lambda b, x: [x if i == b else 0 for i in range(6)]  # noqa: E731
+    for b, at in ((1, 10), (1, 11), (1, 8), (0, 15), (2, 1)):
+        assert d.reserve(one(b, at), one(b, at + 1)) == 3, (b, at)
+        d.check((b, at))
+    # Before too few pages, behind bad ranges; from 0 on nothing is taken to be written.
+    assert d.reserve([0, 10, 0, 0, 0, 0], [0, 11, 0, 24, 24, 24]) == 3
+    assert d.reserve([0, 10, 0, -1, 0, 0], [0, 11, 0, 4, 0, 0]) == 2
+    assert d.reserve(nothing, [18, 10, 18, 0, 0, 0]) == 0
+    assert d.reserve([18, 0, 18, 0, 0, 0], [20, 0, 19, 0, 0, 0]) == 0  # pages of their own
+    d.check()
+    # The way on: a branch of the shortened branch has the begun page as its own.
+    assert d.fork([1], [3]) == p.fork([1], [3]) == 0
+    d.release([EVERYTHING, 0] + [EVERYTHING] * 4, [EVERYTHING] * 6)
+    p.release([EVERYTHING, 0] + [EVERYTHING] * 4, [EVERYTHING] * 6)
+    assert d.reserve(one(3, 10), one(3, 14)) == p.reserve(one(3, 10), one(3, 14)) == 0
+    d.check()
+    # Shared no more, the pages may be written again.
+    d.release([EVERYTHING, 0, 0, 0, 0, 0], [EVERYTHING] * 6)
+    p.release([EVERYTHING, 0, 0, 0, 0, 0], [EVERYTHING] * 6)
+    assert d.reserve(one(0, 15), one(0, 16)) == 0
+    d.check()
+
+
+@pytest.mark.parametrize("page", [1, 4, 16])
+@pytest.mark.parametrize("seed", range(4))
+def test_appends_never_reach_another_sequence(dev, page, seed):
+    """Branches that grow, shrink to anywhere and branch again: after every step each
+    sequence's rows in the cache are its own tokens."""
+    import torch
+    rng = np.random.default_rng(seed)
+    batch, max_pages = 7, 40 // page + 1
+    pages, dim, cap = 5 * max_pages, 8, max_pages * page
+    cfg = gk.make_config(1, pages, page, max_pages, batch, 1, dim, 0)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    table, refs = torch.full((batch, max_pages), -1, dtype=torch.int32, device=dev), i32([0] * pages)
+    k, v = (torch.zeros((pages, page, dim), dtype=torch.int16, device=dev) for _ in range(2))
+    lengths, status = i32([0] * batch), i32([77])
+    tokens, count, codes = [[] for _ in range(batch)], 0, set()
+
+    def release(first):
+        gk.check(gk.kv_cache_release_pages(table, refs, cfg, i32(first), i32([EVERYTHING] * batch)))
+
+    def fork(parent, child):
+        lengths.copy_(i32([len(x) for x in tokens]))
+        gk.check(gk.kv_cache_fork_bf16(k, v, cfg, table, refs, lengths, i32([parent]), i32([child]), 1, status))
+        if int(status) == 0:
+            tokens[child] = list(tokens[parent])
+        return int(status)
+
+    for turn in range(300):
+        b = int(rng.integers(batch))
+        kind = ["append", "append", "fork", "shorten", "drop"][int(rng.integers(5))]
+        if kind == "append":
+            n = int(rng.integers(1, 2 * page + 3))
+            if len(tokens[b]) + n > cap:
+                continue
+            first = [len(x) for x in tokens]
+            end = [f + n if i == b else f for i, f in enumerate(first)]
+            for attempt in range(2):
+                gk.check(gk.kv_cache_reserve_pages(table, refs, cfg, i32(first), i32(end), status))
+                codes.add(int(status))
+                empty = [c for c in range(batch) if not tokens[c]]
+                if int(status) != 3 or not empty or attempt:
+                    break
+                if fork(b, empty[0]) != 0:
+                    break
+                release([0 if i == b else EVERYTHING for i in range(batch)])
+                tokens[b], b = [], empty[0]
+                first = [len(x) for x in tokens]
+                end = [f + n if i == b else f for i, f in enumerate(first)]
+            if int(status) == 0:
+                new = list(range(count + 1, count + 1 + n))
+                count += n
+                rows = i32(new).to(torch.int16)[:, None].expand(n, dim).contiguous()
+                at = [len(tokens[b]) + j for j in range(n)]
+                gk.check(gk.kv_cache_write_bf16(k, v, cfg, table, i32([b] * n), i32(at), n, 0, rows, -rows))
+                tokens[b] += new
+        elif kind == "fork":
+            empty = [c for c in range(batch) if not tokens[c] and c != b]
+            if empty and tokens[b]:
+                release([0 if i == empty[0] else EVERYTHING for i in range(batch)])
+                fork(b, empty[0])
+        else:
+            tokens[b] = tokens[b][:int(rng.integers(0, len(tokens[b]) + 1))] if kind == "shorten" else []
+            release([len(x) for x in tokens])
+        held = table.cpu().numpy()
+        for c in range(batch):
+            if tokens[c]:
+                at = np.arange(len(tokens[c]))
+                rows = torch.from_numpy(held[c, at // page].astype(np.int64)).to(dev)
+                offset = torch.from_numpy(at % page).to(dev)
+                want = i32(tokens[c]).to(torch.int16)[:, None].expand(-1, dim)
+                assert torch.equal(k[rows, offset], want) and torch.equal(v[rows, offset], -want), (turn, kind, c)
+        mapped = np.bincount(held[held >= 0], minlength=pages)
+        assert np.array_equal(refs.cpu().numpy(), mapped), (turn, kind)
+    assert 0 in codes and (3 in codes) == (page > 1)  # whole pages are never gone on in
