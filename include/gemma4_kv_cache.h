@@ -142,13 +142,18 @@ hipError_t gemma4_kv_cache_write_prefill_bf16(
 // must not overlap.
 //
 // Positions of a sliding cache name ring slots: logical page p sits in slot
-// p % max_pages_per_seq, as in gemma4_kv_cache_write_bf16.
+// p % max_pages_per_seq, as in gemma4_kv_cache_write_bf16, and a range of positions
+// means these slots, whichever lap of the ring they hold: one that is as long as the
+// ring means all of it.
 
 // Returns pages: for every sequence b < batch_size, the pages that lie wholly in
 // positions [d_first_position[b], d_end_position[b]) are unmapped and lose one
-// reference each (0 .. INT32_MAX: all of the sequence's; length .. INT32_MAX:
-// what a shortened sequence no longer needs; sinks .. length - window: what no
-// row of a windowed sequence will see again). An empty range changes nothing.
+// reference each. 0 .. INT32_MAX: all of the sequence's. Over a full-length cache
+// also length .. INT32_MAX: what a shortened sequence no longer needs, and sinks ..
+// length - window: what no row of a windowed sequence will see again. Over a ring
+// those two would reach live slots: a shortened sequence there gives back new length
+// .. old length, or nothing; what the window has passed is overwritten in its place.
+// An empty range changes nothing.
 hipError_t gemma4_kv_cache_release_pages(int32_t *d_page_table, int32_t *d_page_refs,
                                          Gemma4KvCacheConfig config,
                                          const int32_t *d_first_position,

@@ -592,3 +592,30 @@ def test_prompts_longer_than_the_ring(dev, heads, dim, page, window):
             assert torch.equal(ck[0, page_of, offset], b.k[at + j]) and torch.equal(cv[0, page_of, offset], b.v[at + j])
         at += n
     c.check(c.run())
+
+
+@pytest.mark.parametrize("page", [1, 4, 16])
+def test_a_shortened_ring_gives_back_what_was_dropped(dev, page):
+    """Drafts that were rejected: what lies between the new length and the old goes back
+    to the pool, and no key that the next rows see goes with it."""
+    import torch
+    window, drafts = 40, 23
+    slots = -(-(window + drafts) // page) + 1
+    old, rows = [700, drafts + 5, 3 * slots * page, 50], [3, 9, 1, 20]
+    b = Batch(dev, 8, 256, rows, old, page=page, window=window, ring=True, max_pages=slots, spare=40)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    cut = [drafts, drafts, page, 0]
+    b.prior = [n - c for n, c in zip(old, cut)]
+    b.lengths.copy_(i32(b.prior))
+    want = b.expected()
+    before = b.table.clone()
+    refs = i32(np.bincount(b.table[b.table >= 0].cpu().numpy(), minlength=b.pages))
+    gk.check(gk.kv_cache_release_pages(b.table, refs, b.config, b.lengths, i32(old)))
+    for s, (new, was) in enumerate(zip(b.prior, old)):
+        gone = {j % slots for j in range(-(-new // page), was // page)}
+        assert set(torch.nonzero(before[s] != b.table[s])[:, 0].tolist()) == gone
+    status = i32([77])
+    gk.check(gk.kv_cache_reserve_pages(b.table, refs, b.config, b.lengths, i32([n + p for n, p in zip(rows, b.prior)]), status))
+    assert int(status) == 0
+    b.expected = lambda layer=0: want
+    b.check(b.run())
