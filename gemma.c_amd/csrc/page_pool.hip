@@ -704,7 +704,9 @@ hipError_t gemma4_kv_cache_fork_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cach
   const int32_t slots = config.window_size > 0 ? config.max_pages_per_seq : 1;
   const int64_t pieces = (page_packs + kCopyPacks - 1) / kCopyPacks;
   const int64_t blocks = pieces * slots * fork_count;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  // A launch holds fewer than 2^32 threads in a grid dimension. One that is refused
+  // behind the tables' would leave children that map pages without their rows.
+  if (blocks * kCopyThreads > 0xffffffffll) return hipErrorInvalidValue;
   hipLaunchKernelGGL(fork_tables_kernel, dim3(1), dim3(kPoolThreads), 0, stream, f, slots,
                      make_fast_div(slots));
   hipLaunchKernelGGL(fork_copy_kernel, dim3((uint32_t)blocks, 2 * config.num_layers),

@@ -186,7 +186,8 @@ hipError_t gemma4_kv_cache_reserve_pages(int32_t *d_page_table, int32_t *d_page_
 // in the call; fork_count <= batch_size. *d_status: 0, or with nothing changed 1
 // (not enough free pages) or 2 (a sequence out of range or named against these
 // rules, a length out of range). fork_count == 0 is a no-op success. Caches are
-// 16-byte aligned.
+// 16-byte aligned. Copies are launched in pieces of 32 KiB of a page: fork_count *
+// (a ring's max_pages_per_seq, or 1) * pieces is below 2^24.
 hipError_t gemma4_kv_cache_fork_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_cache_v,
                                      Gemma4KvCacheConfig config, int32_t *d_page_table,
                                      int32_t *d_page_refs, int32_t *d_seq_lengths,

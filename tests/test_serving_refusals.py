@@ -152,3 +152,11 @@ def test_c_caller(tmp_path):
     proc = subprocess.run(cmd, capture_output=True, text=True, timeout=300)
     assert proc.returncode == 0, proc.stderr
     assert "serving caller ok" in subprocess.run([str(exe)], capture_output=True, text=True, timeout=60).stdout
+
+
+@pytest.mark.parametrize("config", [
+    cfg(batch=4096, page=1024, max_pages=64, pages=4096, window=60000),  # a ring: every page may be copied
+    cfg(batch=4096, page=1 << 19, max_pages=2, pages=64)])               # a begun page of 2^19 rows each
+def test_fork_refuses_more_copies_than_a_launch_holds(config):
+    """Before the tables' launch, which could not be taken back."""
+    assert fork(config=config, fork_count=4096) == BAD
