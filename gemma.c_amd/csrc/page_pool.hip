@@ -510,6 +510,7 @@ struct CompactParams {
 constexpr int kCompactThreads = 1024;
 constexpr int kCompactList = 4096;   // rows whose places LDS holds at a time
 constexpr int kCompactUnroll = 4;
+constexpr int kCompactGroups = 256;  // workgroups that run at once, one per CU
 // A request that breaks several rules gets the lowest of their codes.
 constexpr int kStatusList = 1, kStatusUnmapped = 2, kStatusShared = 3, kStatusNone = 4;
 
@@ -521,7 +522,7 @@ constexpr int kStatusList = 1, kStatusUnmapped = 2, kStatusShared = 3, kStatusNo
 // the next batch's loads go out ahead of the stores. Four requests that keep 3001
 // rows each in 8 layers of 1 x 512 (393 MB): 92 us, 4.3 TB/s of 4.9 for a large copy,
 // the rest being the wait of a batch for its last load; 7 of 32 drafts of 8 sequences
-// in 10 layers of 8 x 256: 11 us, the chain of list, table, row and store.
+// in 10 layers of 8 x 256: 5.9 us, the chain of list, table, row and store.
 __global__ __launch_bounds__(kCompactThreads) void compact_kernel(CompactParams p) {
   __shared__ int32_t s_src[kCompactList], s_dst[kCompactList];
   __shared__ int32_t s_error;
@@ -732,11 +733,15 @@ hipError_t gemma4_kv_cache_compact_bf16(gemma4_bf16 *d_cache_k, gemma4_bf16 *d_c
     return hipErrorInvalidValue;
   }
   const int32_t row_packs = config.num_heads * (config.head_dim / kPackElems);
-  // Slices of 256 bytes or more, at most a workgroup's width, until there are two
-  // workgroups per CU.
+  // Slices of 256 bytes or more, at most a workgroup's width, as long as every
+  // workgroup has a CU to itself: 1024 threads of 76 registers leave no room for a
+  // second one, and a further round is the whole chain again. 8 sequences of 10 layers
+  // of 8 x 256, 7 rows each: 5.9 us in 160 workgroups, 8.3 in 320, 11.1 in 640; 3001
+  // rows each: 792 us, 905 and 801; 4 of 5 layers, 3001 rows each: 201 us in 160, 229
+  // in 320, 220 in 640.
   const int64_t wide = (int64_t)sequence_count * 2 * config.num_layers;
   int32_t slices = (row_packs + kCompactThreads - 1) / kCompactThreads;
-  while (row_packs / (2 * slices) >= 16 && wide * slices < 512) slices *= 2;
+  while (row_packs / (2 * slices) >= 16 && wide * slices * 2 <= kCompactGroups) slices *= 2;
   const CompactParams p = {reinterpret_cast<uint16_t *>(d_cache_k),
                            reinterpret_cast<uint16_t *>(d_cache_v),
                            config,
