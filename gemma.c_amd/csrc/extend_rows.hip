@@ -107,7 +107,8 @@ __device__ __forceinline__ void mfma_pv(f32x16_t &acc, u32x4v_t v, u32x4v_t p) {
 __device__ __forceinline__ void mfma_zero(f32x16_t &acc, u32x4v_t zero) {
   asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "=a"(acc) : "v"(zero));
 }
-// Every product above has written its accumulators (16 passes and the write).
+// Every product above has written its accumulators: a product is 8 passes (32 clocks,
+// as the 2048 of a tile's 64 show) and the write; the waits would cover 16.
 template <int kCount>
 __device__ __forceinline__ void mfma_pv_done(f32x16_t (&acc)[kCount]) {
 #pragma unroll
@@ -263,7 +264,9 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
     const int32_t turn = ahead - (ahead >= 0 ? ahead : ahead - period + 1) / period * period;
     const int32_t start = turn < n_tiles ? tile_lo + turn : tile_lo;
     const int32_t before_wrap = tile_lo + n_tiles - start;
-    elapsed += n_tiles + 6;  // with the block's own cost
+    // With a wide block's own cost. A block of one wave's rows is 3 in the plan: in
+    // batches of many such blocks the shares drift apart, which costs reads past L2 only.
+    elapsed += n_tiles + 6;
     auto tile_key = [&](int it) __attribute__((always_inline)) -> int32_t {
       const int32_t i = it + (it < before_wrap ? start : tile_lo - before_wrap);
       return (i < tiles.sink_tiles ? i : i + tile_skip) * kTile;
@@ -541,7 +544,11 @@ __global__ __launch_bounds__(kThreads, 1) void extend_rows_kernel(ExtendParams p
         } else if constexpr (u >= 7 && u < 23) {
           constexpr int i = u - 7;
           const float w = __builtin_amdgcn_exp2f(fmaf(score[i], p.q_scale, -m_use));
-          // P is the product's operand: bf16, half a step (2^-8) of each weight.
+          // P is the product's operand in one bf16, half a step (2^-8) of each weight, as
+          // in the chunk kernels: 0.0016 of the outputs' norm beside the 0.0017 of their own
+          // rounding, 0.0023 together. A second bf16 for the rest would be another 1024
+          // clocks of products in a tile of 3740 at 1 x 512. The sums l are of the weights
+          // in 32 bits.
           if constexpr (i % 2 == 0) {
             even = w;
           } else {

@@ -54,7 +54,7 @@ __device__ __forceinline__ SlotRange slot_range(const PoolParams &p, int32_t lo,
 
 // ---- release --------------------------------------------------------------
 // One thread per table entry; what is read and written is a few kilobytes (64
-// sequences of 512 pages: 128 KiB) and the launch is its time, 2 us.
+// sequences of 512 pages: 128 KiB) and the launch is its time, 1.6 to 2.7 us.
 __global__ __launch_bounds__(256) void release_pages_kernel(
     PoolParams p, const int32_t *__restrict__ first_position,
     const int32_t *__restrict__ end_position, int64_t entries) {
