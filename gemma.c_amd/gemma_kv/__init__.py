@@ -61,6 +61,7 @@ _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 _CFG = Gemma4KvCacheConfig
 
 # name -> (restype, argtypes); every symbol include/*.h declares with C linkage.
@@ -71,6 +72,18 @@ SIGNATURES = {
     "gemma4_kv_cache_ensure_range_ptr": (_I32, [_P, _P, _I64, ctypes.POINTER(_CFG), _I32, _I32, _I32]),
     "gemma4_kv_cache_write_bf16": (_I32, [_P, _P, _CFG, _P, _P, _P, _I32, _I32, _P, _P, _P]),
     "gemma4_kv_cache_write_prefill_bf16": (_I32, [_P, _P, _CFG, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P]),
+    "gemma4_kv_cache_write_fp8": (_I32, [_P, _P, _CFG, _P, _P, _P, _I32, _I32, _P, _P, _I64, _P, _P, _P]),
+    "gemma4_kv_cache_read_fp8": (_I32, [_P, _P, _P, _P, _CFG, _P, _P, _P, _I32, _I32, _I64, _P, _P, _P]),
+    "gemma4_flash_attention_decode_paged_fp8": (
+        _I32, [_P] * 11 + [_CFG, _I32, _F32, _I32, _I32, _I32, _P]),
+    "gemma4_flash_attention_append_decode_paged_fp8": (
+        _I32, [_P] * 14 + [_CFG, _I32, _F32, _I32, _I32, _I32, _P]),
+    "gemma4_decode_split_plan_fp8": (
+        _I32, [_CFG, _I32, _I32, _I32, ctypes.POINTER(_I32), ctypes.POINTER(_I32)]),
+    "gemma4_rope_frequencies": (
+        _I32, [_P, ctypes.POINTER(_F32), _I32, _I32, _F64, _I32, _F64, _F64, _F64, _F64]),
+    "gemma4_rope_rows_bf16": (
+        _I32, [_P] * 10 + [_F32, _I32, _I32, _I32, _I32, _I32, _I64, _I64, _P]),
     "gemma4_flash_attention_decode_paged_bf16": (
         _I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _CFG, _I32, _F32, _I32, _I32, _I32, _P]),
     "gemma4_flash_attention_append_decode_paged_bf16": (
@@ -241,6 +254,33 @@ def decode_split_plan(config, batch_count: int, max_live_keys: int,
                                          target_workgroups, ctypes.byref(s),
                                          ctypes.byref(n)), "gemma4_decode_split_plan")
     return s.value, n.value
+
+
+def decode_split_plan_fp8(config, batch_count: int, max_live_keys: int,
+                          target_workgroups: int = 0):
+    s = _I32()
+    n = _I32()
+    check(lib().gemma4_decode_split_plan_fp8(config, batch_count, max_live_keys,
+                                             target_workgroups, ctypes.byref(s),
+                                             ctypes.byref(n)), "gemma4_decode_split_plan_fp8")
+    return s.value, n.value
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BY_PARTS = range(4)
+
+
+def rope_frequencies(rotary_dim: int, theta: float, scaling: int = ROPE_PLAIN,
+                     factor: float = 1.0, original_context: float = 0.0,
+                     fast_turns: float = 32.0, slow_turns: float = 1.0, exponent_dim: int = 0):
+    """(turns, amplitude): numpy float64 [rotary_dim / 2] and a float; exponent_dim 0 is
+    rotary_dim. The turns go to the device once."""
+    import numpy as np
+    turns = np.zeros(max(rotary_dim, 0) // 2, dtype=np.float64)
+    amplitude = _F32()
+    check(lib().gemma4_rope_frequencies(
+        turns.ctypes.data, ctypes.byref(amplitude), rotary_dim, exponent_dim or rotary_dim, theta,
+        scaling, factor, original_context, fast_turns, slow_turns), "gemma4_rope_frequencies")
+    return turns, amplitude.value
 
 
 # ---- device entry points (return hipError_t codes, like the reference) ----
@@ -598,3 +638,56 @@ def flash_attention_extend_paged_bf16(out, q, k, v, cache_k, cache_v, page_table
         ptr(out), ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(page_table), ptr(plan),
         plan_bytes, config, layer, batch_size, total_rows, q_stride, kv_stride, softmax_scale,
         ptr(workspace), workspace_bytes, stream_handle(stream))
+
+
+# ---- preparation of ragged rows ----------------------------------------------
+
+def rope_rows_bf16(q_out, k_out, v_out, q, k, v, q_norm_weight, k_norm_weight, token_position,
+                   turns, amplitude, rotary_dim, interleaved, num_heads, head_dim, rows,
+                   stream=None, q_stride=0, kv_stride=0) -> int:
+    return lib().gemma4_rope_rows_bf16(
+        ptr(q_out), ptr(k_out), ptr(v_out), ptr(q), ptr(k), ptr(v), ptr(q_norm_weight),
+        ptr(k_norm_weight), ptr(token_position), ptr(turns), amplitude, rotary_dim,
+        int(interleaved), num_heads, head_dim, rows, q_stride, kv_stride, stream_handle(stream))
+
+
+# ---- a cache in 8 bits -------------------------------------------------------
+
+def kv_cache_write_fp8(cache_k, cache_v, config, page_table, token_batch, token_position,
+                       token_count, layer, k, v, k_scales=None, v_scales=None, stream=None,
+                       kv_stride=0) -> int:
+    return lib().gemma4_kv_cache_write_fp8(
+        ptr(cache_k), ptr(cache_v), config, ptr(page_table), ptr(token_batch),
+        ptr(token_position), token_count, layer, ptr(k), ptr(v), kv_stride, ptr(k_scales),
+        ptr(v_scales), stream_handle(stream))
+
+
+def kv_cache_read_fp8(k, v, cache_k, cache_v, config, page_table, token_batch, token_position,
+                      token_count, layer, k_scales=None, v_scales=None, stream=None,
+                      kv_stride=0) -> int:
+    return lib().gemma4_kv_cache_read_fp8(
+        ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), config, ptr(page_table), ptr(token_batch),
+        ptr(token_position), token_count, layer, kv_stride, ptr(k_scales), ptr(v_scales),
+        stream_handle(stream))
+
+
+def flash_attention_decode_paged_fp8(out, partial_m, partial_l, partial_acc, q, cache_k, cache_v,
+                                     k_scales, v_scales, page_table, seq_lengths, config, layer,
+                                     softmax_scale, split_size, num_splits, batch_count,
+                                     stream=None) -> int:
+    return lib().gemma4_flash_attention_decode_paged_fp8(
+        ptr(out), ptr(partial_m), ptr(partial_l), ptr(partial_acc), ptr(q), ptr(cache_k),
+        ptr(cache_v), ptr(k_scales), ptr(v_scales), ptr(page_table), ptr(seq_lengths), config,
+        layer, softmax_scale, split_size, num_splits, batch_count, stream_handle(stream))
+
+
+def flash_attention_append_decode_paged_fp8(out, partial_m, partial_l, partial_acc, q, cache_k,
+                                            cache_v, k_scales, v_scales, page_table, seq_lengths,
+                                            token_position, k, v, config, layer, softmax_scale,
+                                            split_size, num_splits, batch_count,
+                                            stream=None) -> int:
+    return lib().gemma4_flash_attention_append_decode_paged_fp8(
+        ptr(out), ptr(partial_m), ptr(partial_l), ptr(partial_acc), ptr(q), ptr(cache_k),
+        ptr(cache_v), ptr(k_scales), ptr(v_scales), ptr(page_table), ptr(seq_lengths),
+        ptr(token_position), ptr(k), ptr(v), config, layer, softmax_scale, split_size, num_splits,
+        batch_count, stream_handle(stream))

@@ -38,6 +38,7 @@ HIP_FLAGS = [
 # holds its accumulators in AGPRs by inline asm; the form keeps its scores in VGPRs.
 EXTRA_FLAGS = {
     "decode_d512": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "decode_fp8": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "extend_rows": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "prefill_attention": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "prefill_norm_rope": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],

@@ -187,6 +187,55 @@ hipError_t gemma4_flash_attention_prefill_chunk_paged_bf16_ws(
     int32_t layer, int32_t batch_size, int32_t chunk_len, float softmax_scale,
     void *d_workspace, size_t workspace_bytes, hipStream_t stream);
 
+// ---- preparation of ragged rows ---------------------------------------------------
+// Frequencies of rotary positions, on the host: turns[i], i < rotary_dim / 2, is the
+// pair's rotation per position in whole turns, theta^(-2 i / exponent_dim) / (2 pi) and
+// scaled for contexts `factor` (>= 1) times as long as those of the training:
+//   LINEAR    divided by factor;
+//   BASE      theta times factor^(exponent_dim / (exponent_dim - 2)): the fastest pair
+//             stays, the slowest is divided by factor;
+//   BY_PARTS  a pair that turns fast_turns times or more over original_context positions
+//             stays, one that turns slow_turns times or fewer is divided by factor, between
+//             them in proportion; *amplitude is 0.1 ln(factor) + 1.
+// *amplitude, 1 otherwise, multiplies cos and sin. Arguments that a kind does not name
+// are not looked at. rotary_dim is even, at most 512 and exponent_dim (head_dim where a
+// model rotates a part of its heads as the reference does, src/gemma4_runtime.cu:27-44;
+// otherwise rotary_dim).
+typedef enum Gemma4RopeScaling {
+  GEMMA4_ROPE_PLAIN = 0,
+  GEMMA4_ROPE_LINEAR = 1,
+  GEMMA4_ROPE_BASE = 2,
+  GEMMA4_ROPE_BY_PARTS = 3
+} Gemma4RopeScaling;
+hipError_t gemma4_rope_frequencies(double *turns, float *amplitude, int32_t rotary_dim,
+                                   int32_t exponent_dim, double theta,
+                                   Gemma4RopeScaling scaling, double factor,
+                                   double original_context, double fast_turns,
+                                   double slow_turns);
+
+// The rows of a step of any lengths (packed as for the extension below, row r at
+// d_token_position[r]; a row at a negative position is left alone) from a projection's
+// rows: q and k get the learned RMSNorm of d_q_norm_weight / d_k_norm_weight [head_dim]
+// (null: none) and the rotation of their first rotary_dim dims, a multiple of 16, in
+// pairs (i, i + rotary_dim / 2) or, interleaved != 0, (2 i, 2 i + 1), by
+// position * d_turns[i] turns (d_turns [rotary_dim / 2] on the device, of any finite
+// values) and times `amplitude`; v gets scale-free RMSNorm, eps 1e-6. d_v null with d_v_out: v
+// from the raw k, as in the reference's global layers; both null: no v. q [rows][16][head_dim], rows
+// q_stride elements apart, k and v [rows][num_heads][head_dim], rows kv_stride apart
+// (multiples of 8 up to 2^30; 0: packed). The outputs are packed and overlap no input.
+// All are 16-byte aligned, d_turns 8. Geometries 8 KV heads x 256 and 1 x 512, at most
+// 2^22 rows; rows == 0 is a no-op success. No tables: angles are worked out in 64 bits
+// for any position. (The entry points that take cos and sin tables are served by tables
+// made of the same frequencies.)
+hipError_t gemma4_rope_rows_bf16(gemma4_bf16 *d_q_out, gemma4_bf16 *d_k_out, gemma4_bf16 *d_v_out,
+                                 const gemma4_bf16 *d_q, const gemma4_bf16 *d_k,
+                                 const gemma4_bf16 *d_v, const gemma4_bf16 *d_q_norm_weight,
+                                 const gemma4_bf16 *d_k_norm_weight,
+                                 const int32_t *d_token_position, const double *d_turns,
+                                 float amplitude, int32_t rotary_dim, int32_t interleaved,
+                                 int32_t num_heads, int32_t head_dim, int32_t rows,
+                                 int64_t q_stride, int64_t kv_stride, hipStream_t stream);
+
 // ---- attention of a ragged batch of new tokens over the cache ---------------
 // One step of a server: every sequence b < batch_size brings its own number of
 // new tokens, one (a decode step), a few (drafts to verify) or many (a prompt's
@@ -293,6 +342,40 @@ hipError_t gemma4_decode_split_plan(Gemma4KvCacheConfig config,
                                     int32_t batch_count, int32_t max_live_keys,
                                     int32_t target_workgroups,
                                     int32_t *split_size, int32_t *num_splits);
+
+// ---- decode over a quantised cache ----------------------------------------------
+// gemma4_flash_attention_decode_paged_bf16 over e4m3 codes (gemma4_kv_cache_write_fp8):
+// key and value rows are code * scale with d_k_scales / d_v_scales [num_layers][num_heads]
+// (null: 1). The same lengths, windows, rings, partial buffers and geometries; the split
+// plan is gemma4_decode_split_plan_fp8's (any other that covers the keys works too).
+// Caches, q, k, v, out and partial_acc are 16-byte aligned. A NaN code in a live key
+// gives NaN; what is in keys that are not live, or on unmapped pages, has no part. A
+// prompt's chunk over such a cache: gemma4_kv_cache_read_fp8 its keys, then attend.
+// No counterpart in the reference.
+hipError_t gemma4_flash_attention_decode_paged_fp8(
+    gemma4_bf16 *d_out, float *d_partial_m, float *d_partial_l, float *d_partial_acc,
+    const gemma4_bf16 *d_q, const uint8_t *d_cache_k, const uint8_t *d_cache_v,
+    const float *d_k_scales, const float *d_v_scales, const int32_t *d_page_table,
+    const int32_t *d_seq_lengths, Gemma4KvCacheConfig config, int32_t layer, float softmax_scale,
+    int32_t split_size, int32_t num_splits, int32_t batch_count, hipStream_t stream);
+
+// The same with the token's prepared bf16 rows d_k / d_v [batch_count][num_heads][head_dim]
+// quantised and appended at d_token_position[b] first, in the one launch: the same codes
+// and the same output as gemma4_kv_cache_write_fp8 followed by the call above.
+// d_token_position[b] as for gemma4_flash_attention_append_decode_paged_bf16; sequences
+// whose token goes to one page entry shared by others are not for it.
+hipError_t gemma4_flash_attention_append_decode_paged_fp8(
+    gemma4_bf16 *d_out, float *d_partial_m, float *d_partial_l, float *d_partial_acc,
+    const gemma4_bf16 *d_q, uint8_t *d_cache_k, uint8_t *d_cache_v, const float *d_k_scales,
+    const float *d_v_scales, const int32_t *d_page_table, const int32_t *d_seq_lengths,
+    const int32_t *d_token_position, const gemma4_bf16 *d_k, const gemma4_bf16 *d_v,
+    Gemma4KvCacheConfig config, int32_t layer, float softmax_scale, int32_t split_size,
+    int32_t num_splits, int32_t batch_count, hipStream_t stream);
+
+// gemma4_decode_split_plan for the two calls above.
+hipError_t gemma4_decode_split_plan_fp8(Gemma4KvCacheConfig config, int32_t batch_count,
+                                        int32_t max_live_keys, int32_t target_workgroups,
+                                        int32_t *split_size, int32_t *num_splits);
 
 // Decode-token preparation + cache append (replaces
 // phase_decode_q_paged_kv_norm_rope, src/gemma4_flash_attention_decode.cu:285-375):
