@@ -1,7 +1,7 @@
 // Attention of a ragged batch of new tokens over the paged cache, gfx950: the
 // plan that shares the work out, the merge of split row blocks and the entry
 // points. No counterpart in the reference.
-#include "extend_common.hpp"
+#include "extend_plan.hpp"
 #include "extend_rows.hpp"
 
 #include <math.h>
@@ -20,44 +20,6 @@ struct PlanParams {
   int32_t batch, total_rows, window, sinks, heads, page_size;
   int32_t max_prior;
 };
-
-struct Sum {
-  template <class T> __device__ T operator()(T a, T b) const { return a + b; }
-};
-struct Max {
-  template <class T> __device__ T operator()(T a, T b) const { return a > b ? a : b; }
-};
-// Inclusive prefix of one value per thread over the workgroup; the last
-// thread's in `total`.
-template <int kWaves, class T, class F>
-__device__ __forceinline__ T block_prefix(T x, T &total, T *waves, F f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const T other = __shfl_up(x, d);
-    if (lane >= d) x = f(other, x);
-  }
-  if (lane == kWave - 1) waves[wave] = x;
-  __syncthreads();
-  T head = waves[0], all = waves[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    if (w < wave) head = f(head, waves[w]);
-    all = f(all, waves[w]);
-  }
-  total = all;
-  __syncthreads();
-  return wave > 0 ? f(head, x) : x;
-}
-
-constexpr int kPlanShares = 256;
-constexpr int kShareTiles = 2;  // least cost worth a workgroup
-// Besides its tiles a row block costs the way to its first keys, its queries and its
-// rows' end. Where it holds several waves' rows that is 7.8 us at 8 x 256, of 1.3 us a
-// tile, and 12 at 1 x 512, of 2.1; where one's, 4.5 and 7.
-__device__ __forceinline__ int32_t block_cost(const ExtendGeometry &g, int32_t rows) {
-  return rows > g.wave_rows ? 6 : 3;
-}
 
 // One workgroup, once a step for all layers: 10 to 14 us of dependent loads, barriers
 // and prefix sums. The row blocks laid end to end are cut into shares of equal cost,
@@ -334,7 +296,10 @@ __device__ __forceinline__ void extend_again(int32_t segment, int32_t row, int32
   *reinterpret_cast<Words *>(p.out + ((int64_t)row * kQueryHeads + qh) * kDim + kPer * lane) = words;
 }
 
-template <int kDim>
+// kShared: a block of a prefix that sequences share has the prefix's parts; each of its
+// rows has others, behind the prefix, in the partial sums of its own sequence's blocks,
+// which are folded in when the prefix's are.
+template <int kDim, bool kShared>
 __global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendParams p) {
   __shared__ float4 s_acc[kMergeWaves][kWave];
   __shared__ float2 s_stats[kMergeWaves][kWave];
@@ -406,6 +371,39 @@ __global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendPa
     at.head = head;
     return at;
   };
+  // The parts of this lane's column behind the prefix: one or a few, read 16 bytes a
+  // lane from where the rows' kernel left them (see place).
+  auto fold_own = [&](const Place &at, int32_t dim, MergeState &s, int32_t &segment) {
+    if (at.out < 0) return;
+    const ExtendMerge own = *reinterpret_cast<const ExtendMerge *>(
+        p.plan + p.rows + (int64_t)at.row * sizeof(ExtendMerge));
+    segment = own.segment;
+    const int32_t row = own.index, kv = at.head / kGroup;
+    int64_t sum, stat, odd;
+    uint32_t bit;
+    if (own.rows <= kG.wave_rows) {
+      stat = (int64_t)(own.partial + row) * kQueryHeads + at.head;
+      sum = stat * kDim + dim;
+      odd = ((int64_t)own.partial * kHeads + kv) * 4;
+      bit = 1u << (kGroup == 2 ? at.head % 2 * 16 + row : row * 16 + at.head);
+    } else {
+      const int32_t group = row / kG.wave_rows;
+      const int32_t n = kGroup == 2 ? at.head % 2 * 16 + row % 16 : row % 2 * 16 + at.head;
+      stat = (int64_t)own.partial * kQueryHeads + kv * own.stride * kGroup + group * 32 + n;
+      sum = ((int64_t)own.partial * kRowItems + kv * (own.stride * kGroup * kDim / 256) +
+             group * (kDim / 8) + dim / 8) * 256 + 4 * (n + dim / 4 % 2 * 32);
+      odd = ((int64_t)(own.partial + group * kG.wave_rows) * kHeads + kv) * 4;
+      bit = 1u << n;
+    }
+    const int64_t part_stats = (int64_t)own.stride * kQueryHeads;
+    for (int32_t part = 0; part < own.parts; ++part) {
+      const float2 stats = *reinterpret_cast<const float2 *>(p.stats + 2 * (stat + part * part_stats));
+      const float4 a = *reinterpret_cast<const float4 *>(p.partial + sum + part * part_stats * kDim);
+      const uint4 words = *reinterpret_cast<const uint4 *>(p.odd + odd + (int64_t)part * own.stride * kHeads * 4);
+      s.fold(stats.x, stats.y, a);
+      if ((words.x | words.y | words.z | words.w) & bit) s.odd |= at.bit;
+    }
+  };
   // Parts first, first + step, .. of an item.
   auto gather = [&](const ExtendMerge &m, const Place &at, int32_t first, int32_t step) {
     MergeState s;
@@ -438,7 +436,11 @@ __global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendPa
       for (int d = 1; d < kWave; d <<= 1) s.odd |= __shfl_xor(s.odd, d);
     return s;
   };
-  auto store = [&](const Place &at, const ExtendMerge &m, const MergeState &s) {
+  auto store = [&](const Place &at, const ExtendMerge &m, MergeState s) {
+    int32_t segment = m.segment;
+    if constexpr (kShared) {
+      if (m.prefix != 0) fold_own(at, (int32_t)(at.out % kDim), s, segment);
+    }
     const float inv = s.l > 0.0f ? 1.0f / s.l : 0.0f;
     if (at.out >= 0 && (s.odd & at.bit) == 0)
       *reinterpret_cast<uint2 *>(p.out + at.out) = make_uint2(
@@ -446,7 +448,8 @@ __global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendPa
     uint64_t again = __ballot((s.odd & at.bit) != 0 && at.out >= 0 && at.again);
     for (; __builtin_expect(again != 0, 0); again &= again - 1) {
       const int from = __builtin_ctzll(again);
-      extend_again<kDim>(m.segment, __shfl(at.row, from), __shfl(at.head, from));
+      extend_again<kDim>(kShared ? __shfl(segment, from) : m.segment, __shfl(at.row, from),
+                         __shfl(at.head, from));
     }
   };
   // Blocks of few parts.
@@ -495,7 +498,11 @@ __global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendPa
 }
 
 // ---- host -------------------------------------------------------------------------
-bool valid_extend(const Gemma4KvCacheConfig &c, int32_t batch, int32_t total_rows) {
+bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace
+
+bool extend_sizes_ok(const Gemma4KvCacheConfig &c, int32_t batch, int32_t total_rows) {
   const bool geometry =
       (c.num_heads == 8 && c.head_dim == 256) || (c.num_heads == 1 && c.head_dim == 512);
   return geometry && batch > 0 && batch <= kExtendBatch && batch <= c.batch_size &&
@@ -503,9 +510,74 @@ bool valid_extend(const Gemma4KvCacheConfig &c, int32_t batch, int32_t total_row
          c.page_size > 0 && c.max_pages_per_seq > 0 && c.window_size >= 0 &&
          (int64_t)c.num_pages * c.page_size <= 0x7fffffff;
 }
-bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-}  // namespace
+hipError_t extend_attend(const ExtendCall &call, const ExtendPlanLayout &l, uint32_t magic,
+                         int64_t shared_rows, hipStream_t stream) {
+  const Gemma4KvCacheConfig &config = call.config;
+  if (call.out == nullptr || call.q == nullptr || call.k == nullptr || call.v == nullptr ||
+      call.cache_k == nullptr || call.cache_v == nullptr || call.page_table == nullptr ||
+      call.plan == nullptr || call.workspace == nullptr || call.layer < 0 ||
+      call.layer >= config.num_layers || !(call.softmax_scale > 0.0f) ||
+      !isfinite(call.softmax_scale * kLog2e)) {
+    return hipErrorInvalidValue;
+  }
+  const int64_t q_width = (int64_t)kQueryHeads * config.head_dim;
+  const int64_t kv_width = (int64_t)config.num_heads * config.head_dim;
+  const int64_t q_stride = call.q_stride == 0 ? q_width : call.q_stride;
+  const int64_t kv_stride = call.kv_stride == 0 ? kv_width : call.kv_stride;
+  const int64_t most = (int64_t)1 << 30;
+  if (q_stride < q_width || kv_stride < kv_width || q_stride % kPackElems != 0 ||
+      kv_stride % kPackElems != 0 || q_stride > most || kv_stride > most ||
+      !aligned(call.out, 16) || !aligned(call.q, 16) || !aligned(call.k, 16) ||
+      !aligned(call.v, 16) || !aligned(call.cache_k, 16) || !aligned(call.cache_v, 16) ||
+      !aligned(call.plan, 256) || !aligned(call.workspace, 256) ||
+      call.workspace_bytes < extend_workspace_bytes(l, config)) {
+    return hipErrorInvalidValue;
+  }
+  ExtendParams p{};
+  p.out = reinterpret_cast<uint16_t *>(call.out);
+  p.q = reinterpret_cast<const uint16_t *>(call.q);
+  p.k = reinterpret_cast<const uint16_t *>(call.k);
+  p.v = reinterpret_cast<const uint16_t *>(call.v);
+  p.cache_k = reinterpret_cast<const uint16_t *>(call.cache_k);
+  p.cache_v = reinterpret_cast<const uint16_t *>(call.cache_v);
+  p.page_table = call.page_table;
+  p.plan = static_cast<const char *>(call.plan);
+  p.shares = (int32_t)l.shares;
+  p.segments = (int32_t)l.segments;
+  p.merges = (int32_t)l.merges;
+  p.max_merges = (int32_t)l.max_merges;
+  p.max_segments = (int32_t)l.max_segments;
+  p.c = config;
+  p.page_div = make_fast_div(config.page_size);
+  p.slot_div = make_fast_div(config.max_pages_per_seq);
+  p.layer = call.layer;
+  p.batch = call.batch;
+  p.total_rows = call.total_rows;
+  p.magic = magic;
+  p.q_stride = q_stride;
+  p.kv_stride = kv_stride;
+  p.q_scale = call.softmax_scale * kLog2e;
+  char *workspace = static_cast<char *>(call.workspace);
+  p.partial = reinterpret_cast<float *>(workspace);
+  p.stats = reinterpret_cast<float *>(workspace + extend_stats_offset(l, config.head_dim));
+  p.odd = reinterpret_cast<uint32_t *>(workspace + extend_odd_offset(l, config.head_dim));
+  p.rows = shared_rows;
+  const uint32_t merge_grid = (uint32_t)std::min<int64_t>(
+      kMergeGrid, std::max<int64_t>(l.max_merges, 1) * kQueryHeads * (config.head_dim / 256));
+  launch_extend_rows(p, stream);
+  auto merge = [&](auto *kernel) {
+    hipLaunchKernelGGL(kernel, dim3(merge_grid), dim3(kMergeThreads), 0, stream, p);
+  };
+  const bool shared = magic == kExtendSharedMagic;
+  if (config.num_heads == 1) {
+    shared ? merge(extend_merge_kernel<512, true>) : merge(extend_merge_kernel<512, false>);
+  } else {
+    shared ? merge(extend_merge_kernel<256, true>) : merge(extend_merge_kernel<256, false>);
+  }
+  return hipGetLastError();
+}
+
 }  // namespace gemma4
 
 using namespace gemma4;
@@ -513,24 +585,23 @@ using namespace gemma4;
 extern "C" size_t gemma4_flash_attention_extend_plan_bytes(Gemma4KvCacheConfig config,
                                                            int32_t batch_size,
                                                            int32_t total_rows) {
-  if (!valid_extend(config, batch_size, total_rows)) return 0;
+  if (!extend_sizes_ok(config, batch_size, total_rows)) return 0;
   return (size_t)extend_layout(extend_geometry(config), batch_size, total_rows).bytes;
 }
 
 extern "C" size_t gemma4_flash_attention_extend_workspace_bytes(Gemma4KvCacheConfig config,
                                                                 int32_t batch_size,
                                                                 int32_t total_rows) {
-  if (!valid_extend(config, batch_size, total_rows)) return 0;
-  const ExtendPlanLayout l = extend_layout(extend_geometry(config), batch_size, total_rows);
-  return (size_t)(extend_odd_offset(l, config.head_dim) +
-                  extend_round(l.max_partials * config.num_heads * 16));
+  if (!extend_sizes_ok(config, batch_size, total_rows)) return 0;
+  return extend_workspace_bytes(extend_layout(extend_geometry(config), batch_size, total_rows),
+                                config);
 }
 
 extern "C" hipError_t gemma4_flash_attention_extend_plan(
     void *d_plan, size_t plan_bytes, const int32_t *d_row_offsets, const int32_t *d_prior_lengths,
     Gemma4KvCacheConfig config, int32_t batch_size, int32_t total_rows, int32_t window_size,
     int32_t sink_tokens, hipStream_t stream) {
-  if (!valid_extend(config, batch_size, total_rows) || d_plan == nullptr || !aligned(d_plan, 256) ||
+  if (!extend_sizes_ok(config, batch_size, total_rows) || d_plan == nullptr || !aligned(d_plan, 256) ||
       d_row_offsets == nullptr || d_prior_lengths == nullptr || window_size < 0 ||
       sink_tokens < 0) {
     return hipErrorInvalidValue;
@@ -578,66 +649,11 @@ extern "C" hipError_t gemma4_flash_attention_extend_paged_bf16(
     int32_t batch_size, int32_t total_rows, int64_t q_stride, int64_t kv_stride,
     float softmax_scale, void *d_workspace, size_t workspace_bytes, hipStream_t stream) {
   if (total_rows == 0) return hipSuccess;
-  if (!valid_extend(config, batch_size, total_rows) || d_out == nullptr || d_q == nullptr ||
-      d_k == nullptr || d_v == nullptr || d_cache_k == nullptr || d_cache_v == nullptr ||
-      d_page_table == nullptr || d_plan == nullptr || d_workspace == nullptr || layer < 0 ||
-      layer >= config.num_layers || !(softmax_scale > 0.0f) || !isfinite(softmax_scale * kLog2e)) {
-    return hipErrorInvalidValue;
-  }
-  const int64_t q_width = (int64_t)kQueryHeads * config.head_dim;
-  const int64_t kv_width = (int64_t)config.num_heads * config.head_dim;
-  if (q_stride == 0) q_stride = q_width;
-  if (kv_stride == 0) kv_stride = kv_width;
-  const int64_t most = (int64_t)1 << 30;
-  if (q_stride < q_width || kv_stride < kv_width || q_stride % kPackElems != 0 ||
-      kv_stride % kPackElems != 0 || q_stride > most || kv_stride > most || !aligned(d_out, 16) ||
-      !aligned(d_q, 16) || !aligned(d_k, 16) || !aligned(d_v, 16) || !aligned(d_cache_k, 16) ||
-      !aligned(d_cache_v, 16) || !aligned(d_plan, 256) || !aligned(d_workspace, 256)) {
-    return hipErrorInvalidValue;
-  }
-  const ExtendGeometry &g = extend_geometry(config);
-  const ExtendPlanLayout l = extend_layout(g, batch_size, total_rows);
-  if (plan_bytes < (size_t)l.bytes ||
-      workspace_bytes <
-          gemma4_flash_attention_extend_workspace_bytes(config, batch_size, total_rows)) {
-    return hipErrorInvalidValue;
-  }
-  ExtendParams p{};
-  p.out = reinterpret_cast<uint16_t *>(d_out);
-  p.q = reinterpret_cast<const uint16_t *>(d_q);
-  p.k = reinterpret_cast<const uint16_t *>(d_k);
-  p.v = reinterpret_cast<const uint16_t *>(d_v);
-  p.cache_k = reinterpret_cast<const uint16_t *>(d_cache_k);
-  p.cache_v = reinterpret_cast<const uint16_t *>(d_cache_v);
-  p.page_table = d_page_table;
-  p.plan = static_cast<const char *>(d_plan);
-  p.shares = (int32_t)l.shares;
-  p.segments = (int32_t)l.segments;
-  p.merges = (int32_t)l.merges;
-  p.max_merges = (int32_t)l.max_merges;
-  p.max_segments = (int32_t)l.max_segments;
-  p.c = config;
-  p.page_div = make_fast_div(config.page_size);
-  p.slot_div = make_fast_div(config.max_pages_per_seq);
-  p.layer = layer;
-  p.batch = batch_size;
-  p.total_rows = total_rows;
-  p.q_stride = q_stride;
-  p.kv_stride = kv_stride;
-  p.q_scale = softmax_scale * kLog2e;
-  p.partial = static_cast<float *>(d_workspace);
-  char *workspace = static_cast<char *>(d_workspace);
-  p.stats = reinterpret_cast<float *>(workspace + extend_stats_offset(l, config.head_dim));
-  p.odd = reinterpret_cast<uint32_t *>(workspace + extend_odd_offset(l, config.head_dim));
-  const uint32_t merge_grid = (uint32_t)std::min<int64_t>(
-      kMergeGrid, std::max<int64_t>(l.max_merges, 1) * kQueryHeads * (config.head_dim / 256));
-  launch_extend_rows(p, stream);
-  if (config.num_heads == 1) {
-    hipLaunchKernelGGL(extend_merge_kernel<512>, dim3(merge_grid), dim3(kMergeThreads), 0, stream,
-                       p);
-  } else {
-    hipLaunchKernelGGL(extend_merge_kernel<256>, dim3(merge_grid), dim3(kMergeThreads), 0, stream,
-                       p);
-  }
-  return hipGetLastError();
+  if (!extend_sizes_ok(config, batch_size, total_rows)) return hipErrorInvalidValue;
+  const ExtendPlanLayout l = extend_layout(extend_geometry(config), batch_size, total_rows);
+  if (plan_bytes < (size_t)l.bytes) return hipErrorInvalidValue;
+  return extend_attend({d_out, d_q, d_k, d_v, d_cache_k, d_cache_v, d_page_table, d_plan, config,
+                        layer, batch_size, total_rows, q_stride, kv_stride, softmax_scale,
+                        d_workspace, workspace_bytes},
+                       l, kExtendMagic, 0, stream);
 }

@@ -54,7 +54,7 @@ struct ExtendMerge {
   int32_t stride;     // partial rows from one segment's to the next's
   int32_t index;      // this one among them
   int32_t segment;    // the block's first
-  int32_t pad;
+  int32_t prefix;     // nonzero: the block's rows have parts behind a shared prefix, too
 };
 static_assert(sizeof(ExtendMerge) == 32, "two 16-byte loads");
 
@@ -70,6 +70,7 @@ struct ExtendHeader {
 // its quarters: a signalling NaN, which no arithmetic gives.
 constexpr uint16_t kExtendOdd = 0x7FA5;
 constexpr uint32_t kExtendMagic = 0x67345850;
+constexpr uint32_t kExtendSharedMagic = 0x67345351;  // of groups that share prefixes
 
 // Sections of the plan, by byte offset; all sizes follow from what the host knows.
 struct ExtendPlanLayout {
@@ -90,6 +91,36 @@ inline ExtendPlanLayout extend_layout(const ExtendGeometry &g, int32_t batch, in
   l.merges = extend_round(l.segments + l.max_segments * (int64_t)sizeof(ExtendSegment));
   l.bytes = extend_round(l.merges + l.max_merges * (int64_t)sizeof(ExtendMerge));
   return l;
+}
+// The plan of a batch in groups: besides these, for every row of a sequence whose
+// prefix is attended with its group its own block (ExtendMerge, index: the row
+// within it; parts 0 elsewhere), and the leading pages a sequence has in common with
+// the one before it. All of such a row's parts are partial sums, at least one of the
+// prefix and one behind it.
+struct ExtendSharedLayout {
+  ExtendPlanLayout plan;
+  int64_t rows, common;
+};
+inline ExtendSharedLayout extend_shared_layout(const ExtendGeometry &g, int32_t batch,
+                                               int32_t total_rows) {
+  ExtendSharedLayout s{extend_layout(g, batch, total_rows), 0, 0};
+  ExtendPlanLayout &l = s.plan;
+  const int64_t groups = (int64_t)(batch < total_rows ? batch : total_rows) / 2;
+  const int64_t blocks = total_rows / g.rows + groups;  // of prefixes
+  // Partial rows of one part of each of n blocks: the rows, rounded up to a wave's in
+  // blocks of more than a wave's.
+  auto partial_rows = [&](int64_t n) {
+    const int64_t wide = total_rows / (g.wave_rows + 1);
+    return total_rows + (g.wave_rows - 1) * (wide < n ? wide : n);
+  };
+  l.max_segments += blocks;
+  l.max_merges += partial_rows(blocks);
+  l.max_partials += partial_rows(blocks) + partial_rows(blocks + batch);
+  l.merges = extend_round(l.segments + l.max_segments * (int64_t)sizeof(ExtendSegment));
+  s.rows = extend_round(l.merges + l.max_merges * (int64_t)sizeof(ExtendMerge));
+  s.common = extend_round(s.rows + total_rows * (int64_t)sizeof(ExtendMerge));
+  l.bytes = extend_round(s.common + batch * (int64_t)sizeof(int32_t));
+  return s;
 }
 inline const ExtendGeometry &extend_geometry(const Gemma4KvCacheConfig &c) {
   return c.num_heads == 1 ? kExtend512 : kExtend256;
@@ -135,11 +166,13 @@ struct ExtendParams {
   Gemma4KvCacheConfig c;
   FastDiv page_div, slot_div;
   int32_t layer, batch, total_rows;
+  uint32_t magic;                    // of the plan
   int64_t q_stride, kv_stride;
   float q_scale;          // softmax_scale * log2(e)
   float *partial;
   float *stats;
   uint32_t *odd;
+  int64_t rows;                      // byte offset in a shared plan
 };
 
 // The plan is the same for every workgroup and read through the scalar cache.
@@ -158,7 +191,7 @@ __device__ __forceinline__ T plan_read(const char *at) {
 
 // Whether the plan was made for this call's sizes.
 __device__ __forceinline__ bool extend_plan_fits(const ExtendParams &p, const ExtendHeader &h) {
-  return h.magic == kExtendMagic && h.batch == p.batch && h.total_rows == p.total_rows &&
+  return h.magic == p.magic && h.batch == p.batch && h.total_rows == p.total_rows &&
          h.heads == p.c.num_heads && h.page_size == p.c.page_size;
 }
 

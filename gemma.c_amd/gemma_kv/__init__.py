@@ -104,6 +104,13 @@ SIGNATURES = {
     "gemma4_flash_attention_extend_paged_bf16": (
         _I32, [_P] * 8 + [ctypes.c_size_t, _CFG, _I32, _I32, _I32, _I64, _I64, _F32, _P,
                           ctypes.c_size_t, _P]),
+    "gemma4_flash_attention_extend_shared_plan_bytes": (ctypes.c_size_t, [_CFG, _I32, _I32]),
+    "gemma4_flash_attention_extend_shared_workspace_bytes": (ctypes.c_size_t, [_CFG, _I32, _I32]),
+    "gemma4_flash_attention_extend_shared_plan": (
+        _I32, [_P, ctypes.c_size_t, _P, _P, _P, _P, _I32, _CFG, _I32, _I32, _P]),
+    "gemma4_flash_attention_extend_shared_paged_bf16": (
+        _I32, [_P] * 8 + [ctypes.c_size_t, _CFG, _I32, _I32, _I32, _I64, _I64, _F32, _P,
+                          ctypes.c_size_t, _P]),
     "gemma4_kv_cache_release_pages": (_I32, [_P, _P, _CFG, _P, _P, _P]),
     "gemma4_kv_cache_reserve_pages": (_I32, [_P, _P, _CFG, _P, _P, _P, _P]),
     "gemma4_kv_cache_fork_bf16": (_I32, [_P, _P, _CFG, _P, _P, _P, _P, _P, _I32, _P, _P]),
@@ -635,6 +642,35 @@ def flash_attention_extend_paged_bf16(out, q, k, v, cache_k, cache_v, page_table
                                       softmax_scale, workspace, workspace_bytes, stream=None,
                                       q_stride=0, kv_stride=0) -> int:
     return lib().gemma4_flash_attention_extend_paged_bf16(
+        ptr(out), ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(page_table), ptr(plan),
+        plan_bytes, config, layer, batch_size, total_rows, q_stride, kv_stride, softmax_scale,
+        ptr(workspace), workspace_bytes, stream_handle(stream))
+
+
+# ---- groups of sequences that share a prefix ---------------------------------
+
+def flash_attention_extend_shared_plan_bytes(config, batch_size, total_rows) -> int:
+    return lib().gemma4_flash_attention_extend_shared_plan_bytes(config, batch_size, total_rows)
+
+
+def flash_attention_extend_shared_workspace_bytes(config, batch_size, total_rows) -> int:
+    return lib().gemma4_flash_attention_extend_shared_workspace_bytes(config, batch_size,
+                                                                      total_rows)
+
+
+def flash_attention_extend_shared_plan(plan, plan_bytes, row_offsets, prior_lengths, page_table,
+                                       group_offsets, group_count, config, batch_size, total_rows,
+                                       stream=None) -> int:
+    return lib().gemma4_flash_attention_extend_shared_plan(
+        ptr(plan), plan_bytes, ptr(row_offsets), ptr(prior_lengths), ptr(page_table),
+        ptr(group_offsets), group_count, config, batch_size, total_rows, stream_handle(stream))
+
+
+def flash_attention_extend_shared_paged_bf16(out, q, k, v, cache_k, cache_v, page_table, plan,
+                                             plan_bytes, config, layer, batch_size, total_rows,
+                                             softmax_scale, workspace, workspace_bytes,
+                                             stream=None, q_stride=0, kv_stride=0) -> int:
+    return lib().gemma4_flash_attention_extend_shared_paged_bf16(
         ptr(out), ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(page_table), ptr(plan),
         plan_bytes, config, layer, batch_size, total_rows, q_stride, kv_stride, softmax_scale,
         ptr(workspace), workspace_bytes, stream_handle(stream))

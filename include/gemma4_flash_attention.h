@@ -295,6 +295,38 @@ hipError_t gemma4_flash_attention_extend_paged_bf16(
     int32_t batch_size, int32_t total_rows, int64_t q_stride, int64_t kv_stride,
     float softmax_scale, void *d_workspace, size_t workspace_bytes, hipStream_t stream);
 
+// ---- groups of sequences that share a prefix --------------------------------------
+// The extension above for sequences whose page tables begin with the same pages: the
+// branches of a prompt, the conversations behind a system prompt (what
+// gemma4_kv_cache_fork_bf16 makes). The keys that a group has in common are read and
+// scored once for all its rows. Sequences d_group_offsets[i] .. d_group_offsets[i + 1]
+// are group i (d_group_offsets [group_count + 1], ascending, at most batch_size; those
+// past the last are in none); how far its tables agree the plan finds out itself, and it shares the
+// whole tiles of 32 keys that all of the group have in the cache, where that saves work:
+// groups that share nothing cost as much as without. A group's sequences that bring no
+// rows limit what it shares as the others do. group_count is at most 2048. Full-length
+// caches, no window; rows, offsets, lengths, geometries, limits and results as above (the
+// sums' order differs, so results may by their last bit).
+// No counterpart in the reference.
+//
+// A plan of one kind is refused by the other kind's attention, which then writes nothing.
+// The plan holds for the page table it was made of, too.
+size_t gemma4_flash_attention_extend_shared_plan_bytes(Gemma4KvCacheConfig config,
+                                                       int32_t batch_size, int32_t total_rows);
+size_t gemma4_flash_attention_extend_shared_workspace_bytes(Gemma4KvCacheConfig config,
+                                                            int32_t batch_size,
+                                                            int32_t total_rows);
+hipError_t gemma4_flash_attention_extend_shared_plan(
+    void *d_plan, size_t plan_bytes, const int32_t *d_row_offsets, const int32_t *d_prior_lengths,
+    const int32_t *d_page_table, const int32_t *d_group_offsets, int32_t group_count,
+    Gemma4KvCacheConfig config, int32_t batch_size, int32_t total_rows, hipStream_t stream);
+hipError_t gemma4_flash_attention_extend_shared_paged_bf16(
+    gemma4_bf16 *d_out, const gemma4_bf16 *d_q, const gemma4_bf16 *d_k, const gemma4_bf16 *d_v,
+    const gemma4_bf16 *d_cache_k, const gemma4_bf16 *d_cache_v, const int32_t *d_page_table,
+    const void *d_plan, size_t plan_bytes, Gemma4KvCacheConfig config, int32_t layer,
+    int32_t batch_size, int32_t total_rows, int64_t q_stride, int64_t kv_stride,
+    float softmax_scale, void *d_workspace, size_t workspace_bytes, hipStream_t stream);
+
 // Prefill self-attention with Q/K/V preparation (seqlen_q == seqlen_k, no
 // prior context), same names, argument order and validation as the
 // reference launchers (src/gemma4_flash_attention.cuh:9-45,

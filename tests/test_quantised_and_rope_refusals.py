@@ -181,3 +181,63 @@ def test_plan_refuses(change):
         gk.decode_split_plan_fp8(cfg(), 0, 100)
     with pytest.raises(gk.HipError):
         gk.decode_split_plan_fp8(cfg(), 1, -1)
+
+
+# ---- groups that share a prefix --------------------------------------------------------
+
+def shared_plan(config=None, batch=4, rows=10, groups=1, plan_ptr=P, offsets=P, prior=P, table=P, at=P, nbytes=None):
+    config = config or cfg()
+    n = gk.flash_attention_extend_shared_plan_bytes(config, batch, rows) if nbytes is None else nbytes
+    return gk.flash_attention_extend_shared_plan(plan_ptr, n, offsets, prior, table, at, groups, config, batch, rows, 0)
+
+
+@pytest.mark.parametrize("what", [
+    dict(config=cfg(heads=8, dim=512)), dict(config=cfg(heads=4)), dict(batch=0), dict(batch=5), dict(rows=-1),
+    dict(rows=(1 << 24) + 1), dict(config=cfg(batch=5000), batch=4097), dict(config=cfg(page=0)),
+    dict(config=cfg(window=64)), dict(groups=-1), dict(groups=2049), dict(plan_ptr=0), dict(plan_ptr=P + 128),
+    dict(offsets=0), dict(prior=0), dict(table=0), dict(at=0), dict(nbytes=255)])
+def test_shared_plan_refuses(what):
+    assert shared_plan(**what) == BAD
+
+
+def test_shared_plan_needs_its_bytes():
+    n = gk.flash_attention_extend_shared_plan_bytes(cfg(), 4, 10)
+    assert shared_plan(nbytes=n - 1) == BAD
+    assert gk.flash_attention_extend_shared_plan_bytes(cfg(window=64), 4, 10) == 0
+    assert gk.flash_attention_extend_shared_workspace_bytes(cfg(window=64), 4, 10) == 0
+    assert gk.flash_attention_extend_shared_plan_bytes(cfg(), 0, 10) == 0
+    assert n > gk.flash_attention_extend_plan_bytes(cfg(), 4, 10)
+    for heads, dim in ((8, 256), (1, 512)):
+        c = cfg(heads=heads, dim=dim, batch=4096)
+        last = 0
+        for rows in (0, 1, 2, 63, 64, 65, 1000, 1 << 16, 1 << 24):
+            size = gk.flash_attention_extend_shared_workspace_bytes(c, 64, rows)
+            assert size >= last and gk.flash_attention_extend_shared_plan_bytes(c, 64, rows) > 0
+            last = size
+
+
+def shared_attend(**change):
+    config = change.pop("config", None) or cfg()
+    rows, batch = change.pop("rows", 10), change.pop("batch", 4)
+    a = dict(out=P, q=P, k=P, v=P, cache_k=P, cache_v=P, page_table=P, plan=P,
+             plan_bytes=gk.flash_attention_extend_shared_plan_bytes(config, batch, rows), config=config, layer=0,
+             batch_size=batch, total_rows=rows, softmax_scale=0.0625, workspace=P,
+             workspace_bytes=gk.flash_attention_extend_shared_workspace_bytes(config, batch, rows), stream=0,
+             q_stride=0, kv_stride=0)
+    a.update(change)
+    return gk.flash_attention_extend_shared_paged_bf16(**a)
+
+
+@pytest.mark.parametrize("what", [
+    *[{n: 0} for n in ("out", "q", "k", "v", "cache_k", "cache_v", "page_table", "plan", "workspace")],
+    *[{n: P + 8} for n in ("out", "q", "k", "v", "cache_k", "cache_v")],
+    dict(plan=P + 16), dict(workspace=P + 16), dict(layer=-1), dict(layer=2), dict(batch_size=0), dict(batch_size=5),
+    dict(total_rows=-1), dict(softmax_scale=0.0), dict(softmax_scale=float("nan")), dict(q_stride=4088),
+    dict(q_stride=4100), dict(kv_stride=2040), dict(kv_stride=(1 << 30) + 8), dict(plan_bytes=1), dict(workspace_bytes=1),
+    dict(config=cfg(window=64))])
+def test_shared_attention_refuses(what):
+    assert shared_attend(**what) == BAD
+
+
+def test_shared_attention_without_rows():
+    assert shared_attend(rows=0, q=0) == OK
