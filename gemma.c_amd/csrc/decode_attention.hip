@@ -650,7 +650,7 @@ constexpr int kCombineThreads = 256;
 template <int kDim>
 constexpr int combine_dims() { return kDim == 512 ? 32 : 64; }
 
-template <int kDim, bool kBalanced, int kCombineDims = combine_dims<kDim>()>
+template <int kDim, bool kBalanced, int kCombineDims = combine_dims<kDim>(), class Cut = D512Cut>
 __global__ __launch_bounds__(kCombineThreads) void decode_combine_kernel(CombineParams p) {
   constexpr int kCombineLanes = kCombineThreads / (kCombineDims / 4);  // split lanes
   constexpr int kGroups = kCombineDims / 4;      // 4-dim groups: threads per split lane
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(kCombineThreads) void decode_combine_kernel(Combine
   int32_t cut_splits = 0;
   if constexpr (kBalanced) {
     const int32_t keys = lane_live_keys(p);
-    const int32_t splits = balanced_cut(p, keys).splits;
+    const int32_t splits = Cut::cut(p, keys).splits;
     cut_splits = __builtin_amdgcn_readlane(keys > 0 ? splits : 0, b);
   }
   const int32_t slots = kBalanced ? cut_splits : num_splits;
@@ -942,6 +942,18 @@ hipError_t noalloc_scratch(float **out) {
 }
 
 }  // namespace
+
+hipError_t launch_combine_fp8(const CombineParams &p, int32_t head_dim, int32_t batch_count,
+                              hipStream_t stream) {
+  auto launch = [&](auto *kernel, int dims) {
+    hipLaunchKernelGGL(kernel, dim3(batch_count * kQueryHeads, head_dim / dims),
+                       dim3(kCombineThreads), 0, stream, p);
+    return hipGetLastError();
+  };
+  // Every workgroup derives the cut, so there are few: 128 dims of 512, all of 256.
+  return head_dim == 512 ? launch(decode_combine_kernel<512, true, 128, Fp8Cut<512>>, 128)
+                         : launch(decode_combine_kernel<256, true, 256, Fp8Cut<256>>, 256);
+}
 
 hipError_t decode_append_gated(uint16_t *out, float *pm, float *pl, float *pacc,
                                const uint16_t *q, uint16_t *cache_k, uint16_t *cache_v,

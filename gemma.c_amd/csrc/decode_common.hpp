@@ -6,6 +6,8 @@
 #include "gemma4_device.hpp"
 #include "gemma4_kv_cache.h"
 
+#include <type_traits>
+
 namespace gemma4 {
 
 // Arguments of the split-K decode kernels (decode_attention.hip).
@@ -275,6 +277,87 @@ __device__ __forceinline__ BalancedCut balanced_cut(const Params &p, int32_t key
   cut.splits = lane < p.batch ? max(1, (int32_t)((held + size - 1) / size)) : 0;
   return cut;
 }
+// The policy of the 1 x 512 bf16 decode, and the one over a quantised cache.
+struct D512Cut {
+  template <class Params>
+  static __device__ __forceinline__ BalancedCut cut(const Params &p, int32_t keys) {
+    return balanced_cut(p, keys);
+  }
+};
+// Over a quantised cache (decode_fp8.hip): p.balanced is the number of KV heads, and a
+// split is whole steps of four waves' tiles. At 1 x 512 a workgroup has a CU to itself, so
+// the splits are as long as leave one for each: a second round of few would take as long
+// as the first (64 sequences, 429 000 keys: 125 us with 272 workgroups). At 8 x 256, eight
+// heads and two workgroups on a CU, as long as leave 2048 in all, and kFp8Long keys
+// where that still fills the chip. In tiles of 32 keys, so that sums fit 32 bits.
+constexpr int kFp8Tile = 32, kFp8Step = 128, kFp8Long = 512, kFp8Cus = 256;
+// Inclusive sum over lanes 0 .. lane.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  auto add = [&](auto ctrl, auto mask) __attribute__((always_inline)) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(mask)::value,
+                                               0xF, false);
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});  // row_shr:1
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast:15
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // row_bcast:31
+  return x;
+}
+template <int kDim>
+struct Fp8Cut {
+  // `keys` of this lane's sequence; upto: splits of sequences 0 .. lane.
+  template <class Params>
+  static __device__ __forceinline__ BalancedCut cut(const Params &p, int32_t keys, uint32_t &upto) {
+    const int lane = __lane_id();
+    constexpr uint32_t kStep = kFp8Step / kFp8Tile;
+    const int64_t capacity = (int64_t)p.split_size * p.num_splits;
+    const uint32_t held = (uint32_t)min((int64_t)keys, capacity);
+    const uint32_t tiles = (held + kFp8Tile - 1) / kFp8Tile;
+    const uint32_t total = __builtin_amdgcn_readlane(wave_scan(min(tiles, 1u << 25)), kWave - 1);
+    uint32_t longest = tiles;  // its float orders as the number does
+    auto top = [&](auto mask) __attribute__((always_inline)) {
+      longest = max(longest, __float_as_uint(lane_xor<decltype(mask)::value>(__uint_as_float(longest))));
+    };
+    top(std::integral_constant<int, 1>{});
+    top(std::integral_constant<int, 2>{});
+    top(std::integral_constant<int, 4>{});
+    top(std::integral_constant<int, 8>{});
+    top(std::integral_constant<int, 16>{});
+    top(std::integral_constant<int, 32>{});
+    auto whole = [](uint32_t n) { return max((n + kStep - 1) & ~(kStep - 1), kStep); };
+    const uint32_t slots = (uint32_t)p.num_splits;
+    uint32_t size = whole((longest + slots - 1) / slots);
+    uint32_t mine = 0;
+    auto count = [&]() __attribute__((always_inline)) {
+      mine = lane < p.batch ? max(1u, (tiles + size - 1) / size) : 0;
+      upto = wave_scan(mine);
+      return (uint32_t)__builtin_amdgcn_readlane(upto, kWave - 1);
+    };
+    if constexpr (kDim == 512) {
+      const uint32_t batch = (uint32_t)p.batch;  // at most 64
+      size = max(size, whole(total / (kFp8Cus - batch / 2)));
+      for (int i = 0; count() > kFp8Cus; ++i)
+        size = i < 6 ? size + whole(size / 16) : max(size + kStep, whole(total / (kFp8Cus - batch) + 1));
+    } else {
+      constexpr uint32_t kTotal = 8 * kFp8Cus / 8;  // per head
+      const uint32_t even = total / (kFp8Cus / 8);
+      size = max(size, whole(max(min(even, (uint32_t)kFp8Long / kFp8Tile), (total + kTotal - 1) / kTotal)));
+      count();
+    }
+    BalancedCut r;
+    r.size = wave_uniform((int32_t)(min(size, 1u << 25) * kFp8Tile));
+    r.splits = (int32_t)mine;
+    return r;
+  }
+  template <class Params>
+  static __device__ __forceinline__ BalancedCut cut(const Params &p, int32_t keys) {
+    uint32_t upto;
+    return cut(p, keys, upto);
+  }
+};
 // Live keys of sequence `lane` of the batch (0 past it).
 template <class Params>
 __device__ __forceinline__ int32_t lane_live_keys(const Params &p) {
@@ -287,6 +370,10 @@ __device__ __forceinline__ int32_t lane_live_keys(const Params &p) {
 // Split phase of the 1 x 512 geometry (decode_d512.hip) on a grid of
 // (p.num_splits, batch_count); checked arguments.
 hipError_t launch_split_d512(const DecodeParams &p, int32_t batch_count, hipStream_t stream);
+
+// Combine of splits cut by Fp8Cut (decode_attention.hip).
+hipError_t launch_combine_fp8(const CombineParams &p, int32_t head_dim, int32_t batch_count,
+                              hipStream_t stream);
 
 // The fused append + split-K decode with the separate combine
 // (decode_attention.hip) for the persistent step's 1 x 512 global layers:
