@@ -1,6 +1,7 @@
 // Attention of a ragged batch of new tokens over the paged cache, gfx950: the
 // plan that shares the work out, the merge of split row blocks and the entry
 // points. No counterpart in the reference.
+#include "extend_few.hpp"
 #include "extend_plan.hpp"
 #include "extend_rows.hpp"
 
@@ -192,6 +193,7 @@ __global__ __launch_bounds__(kThreads) void extend_plan_kernel(PlanParams p) {
 constexpr int kMergeThreads = 256;
 constexpr int kMergeWaves = kMergeThreads / kWave;
 constexpr int kMergeGrid = 2048;
+constexpr int kMergeOwn = 4;  // parts behind a prefix whose loads are in flight together
 constexpr int kMergeBatch = 4;
 constexpr int kMergeFew = 16;  // parts a single wave folds
 
@@ -299,12 +301,14 @@ __device__ __forceinline__ void extend_again(int32_t segment, int32_t row, int32
 // kShared: a block of a prefix that sequences share has the prefix's parts; each of its
 // rows has others, behind the prefix, in the partial sums of its own sequence's blocks,
 // which are folded in when the prefix's are.
-template <int kDim, bool kShared>
-__global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendParams p) {
+// kFew: all blocks are of a few rows (extend_few.hip).
+template <int kDim, bool kShared, bool kFew = false>
+__global__ __launch_bounds__(kMergeThreads, kShared ? 4 : 5) void extend_merge_kernel(ExtendParams p) {
   __shared__ float4 s_acc[kMergeWaves][kWave];
   __shared__ float2 s_stats[kMergeWaves][kWave];
   __shared__ uint32_t s_odd[kMergeWaves];
-  constexpr ExtendGeometry kG = kDim == 256 ? kExtend256 : kExtend512;
+  constexpr ExtendGeometry kG = kFew ? (kDim == 256 ? kFew256 : kFew512)
+                                     : (kDim == 256 ? kExtend256 : kExtend512);
   constexpr int kHeads = kDim == 256 ? 8 : 1, kGroup = kQueryHeads / kHeads;
   constexpr int kRowItems = kQueryHeads * kDim / 256;  // items of a partial row
   constexpr int kWaveDims = kDim / 4;                  // dims of a wave in the rows' kernel
@@ -396,12 +400,24 @@ __global__ __launch_bounds__(kMergeThreads, 5) void extend_merge_kernel(ExtendPa
       bit = 1u << n;
     }
     const int64_t part_stats = (int64_t)own.stride * kQueryHeads;
-    for (int32_t part = 0; part < own.parts; ++part) {
-      const float2 stats = *reinterpret_cast<const float2 *>(p.stats + 2 * (stat + part * part_stats));
-      const float4 a = *reinterpret_cast<const float4 *>(p.partial + sum + part * part_stats * kDim);
-      const uint4 words = *reinterpret_cast<const uint4 *>(p.odd + odd + (int64_t)part * own.stride * kHeads * 4);
-      s.fold(stats.x, stats.y, a);
-      if ((words.x | words.y | words.z | words.w) & bit) s.odd |= at.bit;
+    for (int32_t part0 = 0; part0 < own.parts; part0 += kMergeOwn) {
+      float2 stats[kMergeOwn];
+      float4 a[kMergeOwn];
+      uint4 words[kMergeOwn];
+#pragma unroll
+      for (int i = 0; i < kMergeOwn; ++i) {
+        if (part0 + i >= own.parts) break;
+        const int64_t part = part0 + i;
+        stats[i] = *reinterpret_cast<const float2 *>(p.stats + 2 * (stat + part * part_stats));
+        a[i] = *reinterpret_cast<const float4 *>(p.partial + sum + part * part_stats * kDim);
+        words[i] = *reinterpret_cast<const uint4 *>(p.odd + odd + part * own.stride * kHeads * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < kMergeOwn; ++i) {
+        if (part0 + i >= own.parts) break;
+        s.fold(stats[i].x, stats[i].y, a[i]);
+        if ((words[i].x | words[i].y | words[i].z | words[i].w) & bit) s.odd |= at.bit;
+      }
     }
   };
   // Parts first, first + step, .. of an item.
@@ -565,15 +581,20 @@ hipError_t extend_attend(const ExtendCall &call, const ExtendPlanLayout &l, uint
   p.rows = shared_rows;
   const uint32_t merge_grid = (uint32_t)std::min<int64_t>(
       kMergeGrid, std::max<int64_t>(l.max_merges, 1) * kQueryHeads * (config.head_dim / 256));
-  launch_extend_rows(p, stream);
+  const bool few = magic == kExtendFewMagic;
+  few ? launch_extend_few(p, stream) : launch_extend_rows(p, stream);
   auto merge = [&](auto *kernel) {
     hipLaunchKernelGGL(kernel, dim3(merge_grid), dim3(kMergeThreads), 0, stream, p);
   };
-  const bool shared = magic == kExtendSharedMagic;
-  if (config.num_heads == 1) {
-    shared ? merge(extend_merge_kernel<512, true>) : merge(extend_merge_kernel<512, false>);
+  if (few) {
+    config.num_heads == 1 ? merge(extend_merge_kernel<512, true, true>)
+                          : merge(extend_merge_kernel<256, true, true>);
+  } else if (magic == kExtendSharedMagic) {
+    config.num_heads == 1 ? merge(extend_merge_kernel<512, true>)
+                          : merge(extend_merge_kernel<256, true>);
   } else {
-    shared ? merge(extend_merge_kernel<256, true>) : merge(extend_merge_kernel<256, false>);
+    config.num_heads == 1 ? merge(extend_merge_kernel<512, false>)
+                          : merge(extend_merge_kernel<256, false>);
   }
   return hipGetLastError();
 }

@@ -71,6 +71,7 @@ struct ExtendHeader {
 constexpr uint16_t kExtendOdd = 0x7FA5;
 constexpr uint32_t kExtendMagic = 0x67345850;
 constexpr uint32_t kExtendSharedMagic = 0x67345351;  // of groups that share prefixes
+constexpr uint32_t kExtendFewMagic = 0x67344652;     // the same, in blocks of a few rows
 
 // Sections of the plan, by byte offset; all sizes follow from what the host knows.
 struct ExtendPlanLayout {

@@ -5,19 +5,33 @@
 // Softmax over a union of key sets joins from their maxima, sums and weighted values:
 // m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m) / l. So a row of a
 // group is attended in two kinds of row blocks: its group's rows together over the
-// prefix, and its sequence's rows over what lies behind it. To the rows' kernel both are
+// prefix, and its sequence's rows over what lies behind it. To the rows' kernels both are
 // ordinary segments: the group's packed rows follow each other, and a block of them
 // that is said to begin behind the prefix (prior = its keys) sees all of it, by any
 // member's page table. What differs is the plan, which lays prefixes' blocks and
 // sequences' blocks end to end and cuts the line into equal shares, and the merge,
 // which folds a row's parts of both kinds (extend_merge_kernel<.., true>).
 // The prefix is cut down to whole tiles; the rest of it is read with each sequence.
+//
+// Of two kernels for the rows the host takes one by their number: extend_few.hip's
+// blocks of a few rows, or extend_rows.hip's larger ones, which read a long prefix less
+// often (few_rows).
+#include "extend_few.hpp"
 #include "extend_plan.hpp"
 
 #include <algorithm>
 
 namespace gemma4 {
 namespace {
+
+// What tells whether a group's prefix is attended together, in tiles' time: of a row
+// (its sums go to memory and back twice, by way of the merge) and at all (the merge's way
+// from the prefix's parts to the rows' own, while the chip would still take a tile each
+// of more blocks at once).
+struct SharedCosts {
+  int32_t row, least;
+  int32_t share;  // least cost worth a workgroup
+};
 
 struct SharedPlanParams {
   char *plan;
@@ -30,6 +44,8 @@ struct SharedPlanParams {
   ExtendGeometry g;
   int32_t batch, groups, total_rows, heads, page_size, max_pages;
   int32_t max_prior;
+  uint32_t magic;
+  SharedCosts costs;
 };
 
 __device__ __forceinline__ int32_t prior_of(const SharedPlanParams &p, int32_t b) {
@@ -81,8 +97,10 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
     int32_t blocks[kExtendBatch * 3 / 2 + 1];  // row blocks before a group's prefix, or a sequence's own
     int32_t share[kPlanShares + 1];      // first segment of a share
     int64_t waves[kPlanWaves];
+    int64_t order[kPlanShares];
     int32_t waves32[kPlanWaves];
     int32_t parts;
+    unsigned long long saved;
   };
   __shared__ Lds lds;
   const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave;
@@ -93,7 +111,10 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
   const auto *common = reinterpret_cast<const int32_t *>(p.plan + p.common);
 
   // Offsets within the batch and, by a running maximum, ascending, whatever they say.
-  if (t == 0) lds.parts = 0;
+  if (t == 0) {
+    lds.parts = 0;
+    lds.saved = 0;
+  }
   auto ascending = [&](const int32_t *from, int32_t count, int32_t most, int32_t *to) {
     int32_t reach = 0;
     for (int32_t i0 = 0; i0 < count; i0 += kPlanThreads) {
@@ -117,8 +138,8 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
   // A wave a group: the whole tiles that all its sequences share, if attending them once
   // saves more than it costs. It saves the prefix's tiles in the blocks that the
   // group's rows need less when they are laid out together; it costs those blocks
-  // themselves, and the way of every row's sums to memory and back, which is a
-  // quarter of a tile's bytes at 8 x 256 (per KV head) and two tiles' at 1 x 512.
+  // themselves and SharedCosts. None is shared where all that is saved is less than
+  // SharedCosts::least.
   for (int32_t i = wave; i < p.groups; i += kPlanWaves) {
     const int32_t from = lds.group[i], to = lds.group[i + 1];
     int32_t keys = 0x7fffffff, pages = 0x7fffffff, apart = 0;
@@ -139,11 +160,16 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
     const int32_t rows = to > from ? lds.begin[to] - lds.begin[from] : 0;
     const int64_t together = blocks_of(rows);
     const int64_t saved = (int64_t)tiles * (apart - together);
-    const int64_t spent = together * block_cost(p.g, min(rows, p.g.rows)) +
-                          (p.heads == 1 ? 2 * (int64_t)rows : rows / 4);
-    if (tiles > 0 && saved > spent)
+    const int64_t spent =
+        together * block_cost(p.g, min(rows, p.g.rows)) + (int64_t)p.costs.row * rows;
+    if (tiles > 0 && saved > spent) {
       for (int32_t b = from + lane; b < to; b += kWave) lds.tiles0[b] = tiles;
+      if (lane == 0) atomicAdd(&lds.saved, (unsigned long long)(saved - spent));
+    }
   }
+  __syncthreads();
+  if (lds.saved < (unsigned long long)p.costs.least)
+    for (int32_t b = t; b < p.batch; b += kPlanThreads) lds.tiles0[b] = 0;
   __syncthreads();
 
   // Units: the groups' prefixes, then the sequences. lds.blocks: row blocks before each.
@@ -207,7 +233,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
     cost += all;
   }
   const int32_t shares =
-      (int32_t)min((int64_t)p.g.shares, max(cost / kShareTiles, (int64_t)1));
+      (int32_t)min((int64_t)p.g.shares, max(cost / p.costs.share, (int64_t)1));
   const double step = (double)cost / (double)shares, per_step = 1.0 / step;
   auto cut_at = [&](int32_t k) { return (int64_t)((double)k * step); };
 
@@ -280,20 +306,74 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
   for (int32_t k = max(shares, 1) + t; k <= p.g.shares; k += kPlanThreads) lds.share[k] = n_segments;
   __threadfence_block();
   __syncthreads();
-  for (int32_t k = t; k < p.g.shares; k += kPlanThreads) {
-    ExtendShare s = {lds.share[k], lds.share[k + 1], {}, {}};
+  // At 1 x 512 an XCD runs a range of the shares (see extend_rows_kernel): those of a
+  // group's blocks in the order of their tiles, so that it reads an eighth of a prefix
+  // once for all its rows (32 sequences, 8000 shared keys, blocks of 2 rows: 49.5 us to
+  // 42.4, of 8 rows 46.6 to 44.8).
+  static_assert(kPlanShares <= kPlanThreads, "a thread a share");
+  const int32_t k = t;
+  ExtendShare s = {0, 0, {}, {}};
+  if (k < p.g.shares) {
+    s.first = lds.share[k];
+    s.end = lds.share[k + 1];
     if (s.first < s.end) s.segment = segments[s.first];
-    shares_at[k] = s;
+    const ExtendSegment &g = s.segment;
+    const bool prefix = s.first < s.end && g.tile_lo < lds.tiles0[g.sequence];
+    lds.order[k] = prefix ? (int64_t)g.sequence << 32 | g.tile_lo : (int64_t)1 << 62;
+  }
+  __syncthreads();
+  if (k < p.g.shares) {
+    int32_t rank = p.heads == 1 ? 0 : k;
+    if (p.heads == 1) {
+      const int64_t own = lds.order[k];
+      for (int32_t i = 0; i < p.g.shares; ++i)
+        rank += lds.order[i] < own || (lds.order[i] == own && i < k);
+    }
+    shares_at[rank] = s;
   }
   if (t == 0) {
     *reinterpret_cast<ExtendHeader *>(p.plan) = {
-        kExtendSharedMagic, p.batch, p.total_rows, p.heads, 0, 0, p.page_size, n_segments,
+        p.magic, p.batch, p.total_rows, p.heads, 0, 0, p.page_size, n_segments,
         (int32_t)counts, lds.parts, (int32_t)max(step, 1.0)};
   }
 }
 
 bool shared_sizes_ok(const Gemma4KvCacheConfig &c, int32_t batch, int32_t total_rows) {
   return extend_sizes_ok(c, batch, total_rows) && c.window_size == 0;
+}
+// Rows of a call up to which they go to extend_few.hip's kernel. Both kernels on one group
+// of 32 (us, few against large blocks): rows 32 and 64 after 4096 shared keys 30 and 38
+// against 40 and 47 at 1 x 512, 30 and 35 against 31 and 33 at 8 x 256; after 500, 16 and 22
+// against 28 and 30, 18 and 19 against 19 and 22. At 128 rows after 4096 keys it is 63
+// against 54, and 49 against 38: each of many blocks reads the prefix.
+constexpr int32_t kFewRows512 = 96, kFewRows256 = 64;
+bool few_rows(const Gemma4KvCacheConfig &c, int32_t total_rows) {
+  return total_rows <= (c.num_heads == 1 ? kFewRows512 : kFewRows256);
+}
+const ExtendGeometry &shared_geometry(const Gemma4KvCacheConfig &c, int32_t total_rows) {
+  if (few_rows(c, total_rows)) return c.num_heads == 1 ? kFew512 : kFew256;
+  return extend_geometry(c);
+}
+uint32_t shared_magic(const Gemma4KvCacheConfig &c, int32_t total_rows) {
+  return few_rows(c, total_rows) ? kExtendFewMagic : kExtendSharedMagic;
+}
+// From where sharing took less time than not: groups of 2 to 64 sequences of a row each
+// and of 5 and 300 keys behind a prefix of 64 to 16384. At 1 x 512 a few rows' line is at
+// 4 sequences x 10000 keys, 8 x 5000, 16 x 4500 and 32 x 4000 (prefix blocks of two rows
+// save half the reads, of which 256 workgroups make little); at 8 x 256, at 2 x 600, 10 x
+// 500 and 32 x 350. In large blocks it is at 100 x 900 and at 100 x 64.
+SharedCosts shared_costs(const Gemma4KvCacheConfig &c, int32_t total_rows) {
+  if (few_rows(c, total_rows)) return c.num_heads == 1 ? SharedCosts{10, 256, 1} : SharedCosts{6, 0, 1};
+  return c.num_heads == 1 ? SharedCosts{15, 0, kShareTiles} : SharedCosts{1, 0, kShareTiles};
+}
+// A larger call's buffers hold a smaller one's, also where that goes to the other kernel.
+template <class Bytes>
+size_t largest(const Gemma4KvCacheConfig &c, int32_t batch, int32_t total_rows, Bytes bytes) {
+  if (!shared_sizes_ok(c, batch, total_rows)) return 0;
+  const int32_t few = std::min(total_rows, c.num_heads == 1 ? kFewRows512 : kFewRows256);
+  return std::max(
+      bytes(extend_shared_layout(shared_geometry(c, total_rows), batch, total_rows).plan),
+      bytes(extend_shared_layout(shared_geometry(c, few), batch, few).plan));
 }
 bool aligned256(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 255) == 0; }
 
@@ -306,16 +386,15 @@ extern "C" {
 
 size_t gemma4_flash_attention_extend_shared_plan_bytes(Gemma4KvCacheConfig config,
                                                        int32_t batch_size, int32_t total_rows) {
-  if (!shared_sizes_ok(config, batch_size, total_rows)) return 0;
-  return (size_t)extend_shared_layout(extend_geometry(config), batch_size, total_rows).plan.bytes;
+  return largest(config, batch_size, total_rows,
+                 [](const ExtendPlanLayout &l) { return (size_t)l.bytes; });
 }
 
 size_t gemma4_flash_attention_extend_shared_workspace_bytes(Gemma4KvCacheConfig config,
                                                             int32_t batch_size,
                                                             int32_t total_rows) {
-  if (!shared_sizes_ok(config, batch_size, total_rows)) return 0;
-  return extend_workspace_bytes(
-      extend_shared_layout(extend_geometry(config), batch_size, total_rows).plan, config);
+  return largest(config, batch_size, total_rows,
+                 [&](const ExtendPlanLayout &l) { return extend_workspace_bytes(l, config); });
 }
 
 hipError_t gemma4_flash_attention_extend_shared_plan(
@@ -328,7 +407,7 @@ hipError_t gemma4_flash_attention_extend_shared_plan(
       group_count > kExtendBatch / 2) {
     return hipErrorInvalidValue;
   }
-  const ExtendGeometry &g = extend_geometry(config);
+  const ExtendGeometry &g = shared_geometry(config, total_rows);
   const ExtendSharedLayout s = extend_shared_layout(g, batch_size, total_rows);
   if (plan_bytes < (size_t)s.plan.bytes) return hipErrorInvalidValue;
   SharedPlanParams p{};
@@ -343,6 +422,8 @@ hipError_t gemma4_flash_attention_extend_shared_plan(
   p.page_table = d_page_table;
   p.group_offsets = d_group_offsets;
   p.g = g;
+  p.magic = shared_magic(config, total_rows);
+  p.costs = shared_costs(config, total_rows);
   p.batch = batch_size;
   p.groups = group_count;
   p.total_rows = total_rows;
@@ -365,12 +446,12 @@ hipError_t gemma4_flash_attention_extend_shared_paged_bf16(
   if (total_rows == 0) return hipSuccess;
   if (!shared_sizes_ok(config, batch_size, total_rows)) return hipErrorInvalidValue;
   const ExtendSharedLayout s =
-      extend_shared_layout(extend_geometry(config), batch_size, total_rows);
+      extend_shared_layout(shared_geometry(config, total_rows), batch_size, total_rows);
   if (plan_bytes < (size_t)s.plan.bytes) return hipErrorInvalidValue;
   return extend_attend({d_out, d_q, d_k, d_v, d_cache_k, d_cache_v, d_page_table, d_plan, config,
                         layer, batch_size, total_rows, q_stride, kv_stride, softmax_scale,
                         d_workspace, workspace_bytes},
-                       s.plan, kExtendSharedMagic, s.rows, stream);
+                       s.plan, shared_magic(config, total_rows), s.rows, stream);
 }
 
 }  // extern "C"

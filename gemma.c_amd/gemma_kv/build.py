@@ -39,6 +39,7 @@ HIP_FLAGS = [
 EXTRA_FLAGS = {
     "decode_d512": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "decode_fp8": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "extend_few": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "extend_rows": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "prefill_attention": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "prefill_norm_rope": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],

@@ -302,7 +302,7 @@ hipError_t gemma4_flash_attention_extend_paged_bf16(
 // scored once for all its rows. Sequences d_group_offsets[i] .. d_group_offsets[i + 1]
 // are group i (d_group_offsets [group_count + 1], ascending, at most batch_size; those
 // past the last are in none); how far its tables agree the plan finds out itself, and it shares the
-// whole tiles of 32 keys that all of the group have in the cache, where that saves work:
+// whole tiles (of 32 or 64 keys) that all of the group have in the cache, where that saves time:
 // groups that share nothing cost as much as without. A group's sequences that bring no
 // rows limit what it shares as the others do. group_count is at most 2048. Full-length
 // caches, no window; rows, offsets, lengths, geometries, limits and results as above (the

@@ -92,16 +92,25 @@ class Groups:
         return out
 
     def blocks(self):
-        """Row blocks of prefixes in the plan: segments whose last tile ends at their prior keys."""
+        """The plan's segments: row0, rows, base, prior, sequence, first tile, last tile, partial."""
         import torch
         words = self.plan.cpu().view(torch.int32)
-        size = 64 if self.heads == 8 else 8
+        few = self.total <= (64 if self.heads == 8 else 96)
+        size = (16 if few else 64) if self.heads == 8 else (2 if few else 8)
         shares = 32 if self.heads == 8 else 256
         first = 256 + shares * 48
         first = (first + 255) // 256 * 256 // 4
         segments = words[first:first + 8 * int(words[7])].view(-1, 8).tolist()
         assert all(s[1] <= size for s in segments)
         return segments
+
+    def shared_tiles(self, group):
+        """Tiles of a group's prefix that its rows attend together: its sequences' own blocks begin there."""
+        members = range(self.group_offsets[group], self.group_offsets[group + 1])
+        own = {b: [s[5] for s in self.blocks() if s[4] == b and s[3] == self.prior[b]] for b in members if self.rows[b]}
+        tiles = {min(x) for x in own.values() if x}
+        assert len(tiles) == 1
+        return tiles.pop()
 
     def check(self, out, layer=1):
         import torch
@@ -152,20 +161,77 @@ def test_groups(dev, heads, dim, page, groups, alone):
     g.check(g.run())
 
 
-@pytest.mark.parametrize("heads,dim", GEOMETRIES)
-def test_the_prefix_is_in_one_block_of_all_rows(dev, heads, dim):
-    g = Groups(dev, heads, dim, [(1024, [(1, 40)] * 6)], 16)
+# Of both kernels, by the call's rows: geometry, sequences, prefix keys, rows of a block, keys of a tile.
+SHARING = [(8, 256, 6, 1024, 16, 64), (1, 512, 24, 7168, 2, 64), (8, 256, 70, 640, 64, 32), (1, 512, 104, 2048, 8, 32)]
+
+
+@pytest.mark.parametrize("heads,dim,count,prefix,block,tile", SHARING)
+def test_the_prefix_is_in_blocks_of_all_rows(dev, heads, dim, count, prefix, block, tile):
+    import torch
+    g = Groups(dev, heads, dim, [(prefix, [(1, 40)] * count)], 16)
     g.check(g.run())
-    shared = [s for s in g.blocks() if s[1] == 6]
-    assert sorted((s[5], s[6]) for s in shared)[0][0] == 0 and sum(s[6] - s[5] for s in shared) == 32
-    own = [s for s in g.blocks() if s[1] == 1]
-    assert {s[4] for s in own} == set(range(6)) and min(s[5] for s in own) == 32
-    # Tables that part behind 16 keys share no whole tile: six sequences of their own.
+    segments, tiles = g.blocks(), prefix // tile
+    shared = [s for s in segments if s[3] == prefix]
+    assert sum(s[1] * (s[6] - s[5]) for s in shared) == count * tiles
+    assert max(s[1] for s in shared) == min(block, count) and max(s[6] for s in shared) == tiles
+    own = [s for s in segments if s[3] == prefix + 40]
+    assert {s[4] for s in own} == set(range(count)) and min(s[5] for s in own) == tiles
+    assert len(own) + len(shared) == len(segments) and all(s[1] == 1 for s in own)
+    # Tables that part behind 16 keys share no whole tile: sequences of their own.
     g.table[4, 1:] = g.table[3, 1:].flip(0)
     g.make_plan()
-    import torch
     torch.cuda.synchronize()
-    assert all(s[1] == 1 and s[4] in range(6) for s in g.blocks())
+    assert all(s[1] == 1 and s[3] == prefix + 40 and s[4] in range(count) for s in g.blocks())
+
+
+@pytest.mark.parametrize("heads,dim,count,prefix,block,tile", SHARING)
+@pytest.mark.parametrize("page", [16, 24])
+def test_shared_prefixes(dev, heads, dim, count, prefix, block, tile, page):
+    """Sharing in both kernels, and what can go wrong there: tokens and drafts, sequences without rows, pages
+    that are not mapped (in the prefix for all of the group, behind it for one), infinities and NaN in
+    both, rows behind the last sequence, strides, other lengths in a captured graph."""
+    import torch
+    prefix = prefix // page * page
+    seqs = [((1, 1, 0, 2, 1)[b % 5] if count < 30 else (1, 2, 1, 0, 1, 3)[b % 6], (b * 37) % 90 + 1) for b in range(count)]
+    hole = 5 * tile // page
+    g = Groups(dev, heads, dim, [(prefix, seqs)], page, [(1, 200)], extra_rows=2, seed=page,
+               holes=[(b, j) for b in range(count) for j in (0, hole)] + [(3, prefix // page)])
+    out = g.run()
+    g.check(out)
+    tiles = g.shared_tiles(0)
+    assert tiles == prefix // tile
+    wide = torch.zeros(g.total, (16 + 2 * heads) * dim + 8, dtype=torch.bfloat16, device=dev)
+    parts = wide.split([16 * dim, heads * dim, heads * dim, 8], 1)
+    for to, x in zip(parts, (g.q, g.k, g.v)):
+        to.copy_(x.reshape(g.total, -1))
+    assert torch.equal(out, g.run(q=parts[0], k=parts[1], v=parts[2], q_stride=wide.stride(0), kv_stride=wide.stride(0)))
+    # Captured, with sequences' rows and lengths that others have.
+    captured = torch.zeros_like(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g.make_plan()
+        g.attend(captured)
+    kept = g.rows, g.prior
+    for shift in (1, 2, 0):
+        g.rows = kept[0][shift:count] + kept[0][:shift] + kept[0][count:]
+        g.prior = [p - (p - prefix) * (b == 1) for b, p in enumerate(kept[1])] if shift == 1 else kept[1]
+        g.lengths.copy_(torch.tensor(g.prior, dtype=torch.int32))
+        g.offsets.copy_(torch.tensor(np.cumsum([0] + g.rows), dtype=torch.int32))
+        captured.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        g.check(captured)
+    assert torch.equal(out, captured)
+    # Values that are no numbers: of the prefix, of a row's own, of a key that later rows of a draft see only.
+    first = np.cumsum([0] + g.rows)
+    draft = next(b for b in range(count) if g.rows[b] > 1)
+    g.v[int(first[draft]) + 1, 0, 5] = math.inf
+    g.v[int(first[1]), heads - 1, 7] = NAN
+    g.check(g.run())
+    g.cv[1, g.table[0, hole + 1].item(), 1, heads - 1, 11] = math.inf
+    out = g.run()
+    g.check(out)
+    assert bool(torch.isinf(out[:int(first[count]), 16 - 16 // heads:, 11]).all())
 
 
 @pytest.mark.parametrize("heads,dim", GEOMETRIES)
@@ -226,10 +292,11 @@ def test_infinities_and_nan_of_values(dev, heads, dim):
 
 
 @pytest.mark.parametrize("heads,dim", GEOMETRIES)
-def test_equals_the_extension_without_groups(dev, heads, dim):
-    """No groups, groups of one, and the extension itself: the same cuts and the same sums."""
+@pytest.mark.parametrize("last", [40, 100])
+def test_equals_the_extension_without_groups(dev, heads, dim, last):
+    """No groups, groups of one, and, beyond a few rows, the extension itself: the same cuts and the same sums."""
     import torch
-    rows, keys = [1, 5, 1, 40], [300, 20, 0, 77]
+    rows, keys = [1, 5, 1, last], [300, 20, 0, 77]
     g = Groups(dev, heads, dim, [], 16, alone=list(zip(rows, keys)))
     out = g.run()
     g.check(out)
@@ -243,13 +310,17 @@ def test_equals_the_extension_without_groups(dev, heads, dim):
     tail = (g.config, 1, 4, g.total, g.scale)
     gk.check(gk.flash_attention_extend_paged_bf16(*args, plan, plan.numel(), *tail, ws, ws.numel()))
     torch.cuda.synchronize()
-    assert torch.equal(out, plain)
+    if last == 100:
+        assert torch.equal(out, plain)
     # A plan of the other kind: nothing is written.
     plain.fill_(7.0)
-    gk.check(gk.flash_attention_extend_paged_bf16(*args, g.plan, g.plan_bytes, *tail, ws, ws.numel()))
+    other = torch.zeros(max(plan.numel(), g.plan_bytes), dtype=torch.uint8, device=dev)
+    other[:g.plan_bytes].copy_(g.plan)
+    gk.check(gk.flash_attention_extend_paged_bf16(*args, other, other.numel(), *tail, ws, ws.numel()))
     torch.cuda.synchronize()
     assert bool((plain == 7.0).all())
-    g.plan[:plan.numel()].copy_(plan)
+    other[:plan.numel()].copy_(plan)
+    g.plan, g.plan_bytes = other, other.numel()
     g.attend(plain)
     torch.cuda.synchronize()
     assert bool((plain == 7.0).all())

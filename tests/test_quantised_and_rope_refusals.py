@@ -209,10 +209,11 @@ def test_shared_plan_needs_its_bytes():
     assert n > gk.flash_attention_extend_plan_bytes(cfg(), 4, 10)
     for heads, dim in ((8, 256), (1, 512)):
         c = cfg(heads=heads, dim=dim, batch=4096)
-        last = 0
-        for rows in (0, 1, 2, 63, 64, 65, 1000, 1 << 16, 1 << 24):
-            size = gk.flash_attention_extend_shared_workspace_bytes(c, 64, rows)
-            assert size >= last and gk.flash_attention_extend_shared_plan_bytes(c, 64, rows) > 0
+        last = (0, 0)
+        for rows in (0, 1, 2, 63, 64, 65, 96, 97, 128, 1000, 1 << 16, 1 << 24):
+            size = (gk.flash_attention_extend_shared_workspace_bytes(c, 64, rows),
+                    gk.flash_attention_extend_shared_plan_bytes(c, 64, rows))
+            assert size[0] >= last[0] and size[1] >= last[1] > -1 and size[1] > 0
             last = size
 
 
