@@ -67,7 +67,6 @@ __global__ __launch_bounds__(RopeShape<kDim>::kWaves *kWave) void rope_rows_kern
   const int wave = wave_uniform(t / kWave);
   const int64_t row = blockIdx.x;
   const int32_t position = p.position[row];
-  if (position < 0) return;
 
   // Items of a row: at 8 x 256 pairs of heads, 8 of q, then 4 of k, then 4 of v, two to
   // a wave; at 1 x 512 heads, two of q to a wave and k with the v made of it to the last.
@@ -97,13 +96,23 @@ __global__ __launch_bounds__(RopeShape<kDim>::kWaves *kWave) void rope_rows_kern
     if (S::kHeads == 1 && kind == kK && p.v != nullptr && p.v_out != nullptr)
       raw_v = load128(p.v + row * p.kv_stride + d0);
   }
+  // A wave's items are of one kind.
+  static_assert(kQItems % S::kItems == 0 && (S::kHeads == 1 || S::kHeads / S::kItemHeads % S::kItems == 0));
+  const Kind wave_kind = kind_of(wave * S::kItems);
+  const uint16_t *weight = wave_kind == kQ ? p.q_weight : (wave_kind == kK ? p.k_weight : nullptr);
+  uint4 raw_w = make_uint4(0, 0, 0, 0);
+  if (weight != nullptr) raw_w = load128(weight + d0);
   const int half = p.rotary / 2;
-  for (int i = t; i < half; i += S::kWaves * kWave) {
-    const double turns = (double)position * p.turns[i];
+  static_assert(S::kWaves * kWave >= kMaxPairs, "a thread a pair");
+  const double per_position = t < half ? p.turns[t] : 0.0;
+  // Behind the loads: the row is there, whatever its position.
+  if (position < 0) return;
+  if (t < half) {
+    const double turns = (double)position * per_position;
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-    s_cos[i] = p.amplitude * c;
-    s_sin[i] = p.amplitude * s;
+    s_cos[t] = p.amplitude * c;
+    s_sin[t] = p.amplitude * s;
   }
   __syncthreads();
 
@@ -135,12 +144,11 @@ __global__ __launch_bounds__(RopeShape<kDim>::kWaves *kWave) void rope_rows_kern
       if (p.v_out != nullptr) store_normed(p.v_out + (row * S::kHeads + head) * kDim + d0, x[i]);
       continue;
     }
-    const uint16_t *weight = kind == kQ ? p.q_weight : p.k_weight;
     float y[kPackElems];
     if (weight != nullptr) {
       const float scale = unpacked_scale(x[i], y);
       float w[kPackElems];
-      unpack8(load128(weight + d0), w);
+      unpack8(raw_w, w);
 #pragma unroll
       for (int e = 0; e < kPackElems; ++e) y[e] = y[e] * scale * w[e];
     } else {
