@@ -86,9 +86,9 @@ __global__ __launch_bounds__(kCommonThreads) void common_pages_kernel(SharedPlan
 }
 
 // One workgroup, once a step for all layers.
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWaves = kPlanThreads / kWave;
+template <int kPlanThreads>
 __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(SharedPlanParams p) {
+  constexpr int kPlanWaves = kPlanThreads / kWave;
   struct Lds {
     int32_t begin[kExtendBatch + 1];     // first row of a sequence
     int32_t prior[kExtendBatch];         // keys in the cache
@@ -433,7 +433,14 @@ hipError_t gemma4_flash_attention_extend_shared_plan(
   p.max_prior = (int32_t)std::min<int64_t>((int64_t)config.max_pages_per_seq * config.page_size,
                                            0x7fffffff - total_rows - 256);
   hipLaunchKernelGGL(common_pages_kernel, dim3(batch_size), dim3(kCommonThreads), 0, stream, p);
-  hipLaunchKernelGGL(extend_shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
+  // Where a thread of four waves has a sequence each and no more than a block of rows:
+  // sixteen waves' barriers and spills take 27 to 37 us on the batches of 4 to 40
+  // sequences that four plan in 17 to 27; beyond, these would go round for every 256 blocks.
+  if (batch_size + group_count <= 256 && total_rows / g.rows <= 256) {
+    hipLaunchKernelGGL(extend_shared_plan_kernel<256>, dim3(1), dim3(256), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL(extend_shared_plan_kernel<1024>, dim3(1), dim3(1024), 0, stream, p);
+  }
   return hipGetLastError();
 }
 
