@@ -234,6 +234,33 @@ def test_shared_prefixes(dev, heads, dim, count, prefix, block, tile, page):
     assert bool(torch.isinf(out[:int(first[count]), 16 - 16 // heads:, 11]).all())
 
 
+@pytest.mark.parametrize("heads,dim,count,prefix,block,tile", SHARING)
+def test_pages_past_32_bits(dev, heads, dim, count, prefix, block, tile):
+    """The same pages far apart: byte offsets past 2^32 within a layer, and the same result."""
+    import torch
+    g = Groups(dev, heads, dim, [(prefix, [(1 + b % 2, 11 * b % 70) for b in range(count)])], 64, layers=1)
+    out = g.run(layer=0)
+    g.check(out, layer=0)
+    apart = (5 << 30) // (g.pages * 64 * heads * dim * 2)
+    caches = []
+    for c in (g.ck, g.cv):
+        far = torch.empty(1, g.pages * apart, 64, heads, dim, dtype=torch.bfloat16, device=dev)
+        far[:, ::apart] = c
+        caches.append(far)
+    assert caches[0].numel() * 2 > 2**32 and int(g.table.max()) * apart * 64 * heads * dim * 2 > 2**32
+    g.ck, g.cv = caches
+    g.table = torch.where(g.table >= 0, g.table * apart, g.table)
+    g.config = gk.make_config(1, g.pages * apart, 64, g.max_pages, g.batch, heads, dim, 0)
+    assert torch.equal(out, g.run(layer=0))
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+def test_a_long_prefix(dev, heads, dim):
+    """70000 keys: many steps of a segment, and sums of many."""
+    g = Groups(dev, heads, dim, [(70016, [(1, 3), (2, 0), (1, 700)])], 64, layers=1)
+    g.check(g.run(layer=0), layer=0)
+
+
 @pytest.mark.parametrize("heads,dim", GEOMETRIES)
 @pytest.mark.parametrize("count", [2, 17, 33, 64, 65, 100])
 def test_many_members(dev, heads, dim, count):
