@@ -9,7 +9,15 @@
 // factor and the sums' end, and the loop sees codes only. A code becomes a bf16
 // operand exactly (v_cvt_scalef32_pk_bf16_fp8, two a time), so both products run on
 // v_mfma_f32_16x16x32_bf16 with nothing rounded but the weights, which go in as two
-// bf16 numbers, the nearest and the rest (2^-18 of a weight).
+// bf16 numbers, the nearest and the rest (2^-18 of a weight). The matrix instructions of
+// 8-bit operands would need no conversions, but add up their products to within 2^-12.8
+// of sum |ab| only (measured; bf16 ones 2^-22): in the exponent of a score of 40 that is
+// 0.6% of a weight.
+//
+// What bounds it: HBM where there are keys enough. 48 sequences of 512 to 16 384 keys at 8 x 256
+// (1.5 GB) 259 us, 5.9 TB/s; 24 of 200 to 12 000 at 1 x 512 (124 MB) 33 us, 4.5 TB/s in
+// the split's 27 with 5 of start-up, the rest the combine; one of 1024 at 8 x 256 8.4 as a
+// graph, two launches' latency.
 //
 // Workgroup (KV head, split, sequence); a wave takes 32-key tiles of its own and
 // holds all dims' sums, the waves merge once at the end.

@@ -4,6 +4,10 @@
 // Both move packs of 16 codes, one thread a pack of K and the same of V: 64 bytes
 // of bf16 on one side, 32 of codes on the other, and nothing else per row than its
 // (sequence, position) and page-table entry.
+//
+// What bounds them: HBM, from some thousand rows on (4 prompts at 8 x 256, 133 MB, 28 us,
+// 96% of the rate of a large copy; 24 rings read back, 277 MB, 58 us, 97%). A few rows are a
+// launch: 24 at 1 x 512 3.3 us.
 #include "fp8_common.hpp"
 #include "gemma4_device.hpp"
 

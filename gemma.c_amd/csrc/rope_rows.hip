@@ -9,7 +9,12 @@
 // squares is a reduction over the head's lanes. The rows are asked for first; while
 // they are on their way each pair's angle is worked out once for all heads and put
 // into LDS: the turns position * turns[i] in 64 bits (a position has 31 of them and a
-// turn's part has to keep 24), the whole ones dropped, the rest in 32.
+// turn's part has to keep 24), the whole ones dropped, the rest in 32. One rounding, of
+// the outputs to bf16.
+//
+// What bounds it: HBM. 2048 rows at 1 x 512 (73 MB) 14.6 us, the rate of a large copy;
+// 1348 rows of 12 sequences at 8 x 256 (44 MB) 11.0 us, 82% of it with the launch. All that a
+// row needs is asked for before its position is tested: 12.7 us where that came first.
 #include "gemma4_device.hpp"
 #include "prep_common.hpp"
 
