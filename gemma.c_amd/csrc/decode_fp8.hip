@@ -15,9 +15,9 @@
 // 0.6% of a weight.
 //
 // What bounds it: HBM where there are keys enough. 48 sequences of 512 to 16 384 keys at 8 x 256
-// (1.5 GB) 259 us, 5.9 TB/s; 24 of 200 to 12 000 at 1 x 512 (124 MB) 33 us, 4.5 TB/s in
-// the split's 27 with 5 of start-up, the rest the combine; one of 1024 at 8 x 256 8.4 as a
-// graph, two launches' latency.
+// (1.5 GB) 259 us, 5.9 TB/s; 24 of 200 to 12 000 at 1 x 512 (124 MB) 33 us, 6.6 TB/s in the
+// 18 that it streams, with 2 to the first loads, 3 to join the waves' sums, and the combine;
+// one of 1024 at 8 x 256 8.4 as a graph, two launches' latency.
 //
 // Workgroup (KV head, split, sequence); a wave takes 32-key tiles of its own and
 // holds all dims' sums, the waves merge once at the end.

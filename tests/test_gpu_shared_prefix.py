@@ -404,6 +404,31 @@ def test_captured_with_other_lengths_and_two_at_once(dev, heads, dim):
         x.check(o)
 
 
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+def test_two_graphs_share_a_plan_and_a_workspace(dev, heads, dim):
+    """A small call and a large one in the large one's buffers, each a graph, replayed in turn."""
+    import torch
+    large = Groups(dev, heads, dim, [(1280, [(2, b) for b in range(60)])], 64, seed=1)
+    small = Groups(dev, heads, dim, [(8000, [(1, 10 * b) for b in range(20)])], 64, [(3, 50)], seed=2)
+    assert small.plan_bytes <= large.plan_bytes and small.ws_bytes <= large.ws_bytes
+    small.plan, small.plan_bytes, small.ws, small.ws_bytes = large.plan, large.plan_bytes, large.ws, large.ws_bytes
+    outs, graphs = [], []
+    for g in (large, small):
+        outs.append(torch.full((g.total, 16, dim), 7.0, dtype=torch.bfloat16, device=dev))
+        g.make_plan()
+        g.attend(outs[-1])
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            g.make_plan()
+            g.attend(outs[-1])
+    for which in (0, 1, 1, 0, 0, 1):
+        outs[which].fill_(7.0)
+        graphs[which].replay()
+        torch.cuda.synchronize()
+        (large, small)[which].check(outs[which])
+
+
 def test_runs_are_alike(dev):
     import torch
     g = Groups(dev, 1, 512, [(2048, [(1, 20 * b) for b in range(12)])], 64, layers=1)
