@@ -97,7 +97,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
     int32_t blocks[kExtendBatch * 3 / 2 + 1];  // row blocks before a group's prefix, or a sequence's own
     int32_t share[kPlanShares + 1];      // first segment of a share
     int64_t waves[kPlanWaves];
-    int64_t order[kPlanShares];
+    __attribute__((aligned(16))) uint32_t order[kPlanShares];
     int32_t waves32[kPlanWaves];
     int32_t parts;
     unsigned long long saved;
@@ -235,7 +235,11 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
   const int32_t shares =
       (int32_t)min((int64_t)p.g.shares, max(cost / p.costs.share, (int64_t)1));
   const double step = (double)cost / (double)shares, per_step = 1.0 / step;
-  auto cut_at = [&](int32_t k) { return (int64_t)((double)k * step); };
+  // (One conversion to 32 bits, where that is enough, for a dozen instructions.)
+  auto cut_at = [&](int32_t k) {
+    const double at = (double)k * step;
+    return cost <= 0x7fffffff ? (int64_t)(int32_t)at : (int64_t)at;
+  };
 
   int64_t before = 0;                 // cost of the blocks of earlier rounds
   int64_t counts = 0, partials = 0;   // their segments and merged rows, and partial rows
@@ -251,10 +255,10 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
       if (r.rows == 0) return;
       int32_t k = max((int32_t)((double)begin * per_step), 1);  // about: put right here
       while (k > 1 && cut_at(k - 1) >= begin) --k;
-      while (k < shares && cut_at(k) < begin) ++k;
-      for (; k < shares && cut_at(k) < end; ++k) {
-        f(k, (int32_t)max(cut_at(k) - begin - ahead, (int64_t)0));
-      }
+      int64_t at = cut_at(k);
+      while (k < shares && at < begin) at = cut_at(++k);
+      for (; k < shares && at < end; at = cut_at(++k))
+        f(k, (int32_t)max(at - begin - ahead, (int64_t)0));
     };
     int32_t parts = r.rows > 0 ? 1 : 0, last = 0;
     for_cuts([&](int32_t, int32_t tile) {
@@ -311,6 +315,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
   // once for all its rows (32 sequences, 8000 shared keys, blocks of 2 rows: 49.5 us to
   // 42.4, of 8 rows 46.6 to 44.8).
   static_assert(kPlanShares <= kPlanThreads, "a thread a share");
+  static_assert(kExtend512.shares == kPlanShares && kFew512.shares == kPlanShares);
   const int32_t k = t;
   ExtendShare s = {0, 0, {}, {}};
   if (k < p.g.shares) {
@@ -318,16 +323,23 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
     s.end = lds.share[k + 1];
     if (s.first < s.end) s.segment = segments[s.first];
     const ExtendSegment &g = s.segment;
-    const bool prefix = s.first < s.end && g.tile_lo < lds.tiles0[g.sequence];
-    lds.order[k] = prefix ? (int64_t)g.sequence << 32 | g.tile_lo : (int64_t)1 << 62;
+    const int32_t tiles0 = s.first < s.end ? lds.tiles0[g.sequence] : 0;
+    // Sequence, place in the prefix in 4096ths, share: each once, prefixes' first.
+    static_assert(kExtendBatch <= 1 << 12 && kPlanShares <= 1 << 8, "12, 12 and 8 bits");
+    lds.order[k] = g.tile_lo < tiles0
+                       ? (uint32_t)g.sequence << 20 | (uint32_t)(((int64_t)g.tile_lo << 12) / tiles0) << 8 | k
+                       : 0xFFFFFF00u | k;
   }
   __syncthreads();
   if (k < p.g.shares) {
     int32_t rank = p.heads == 1 ? 0 : k;
     if (p.heads == 1) {
-      const int64_t own = lds.order[k];
-      for (int32_t i = 0; i < p.g.shares; ++i)
-        rank += lds.order[i] < own || (lds.order[i] == own && i < k);
+      const uint32_t own = lds.order[k];
+#pragma unroll 4
+      for (int32_t i = 0; i < kPlanShares; i += 4) {  // 1 x 512 has all of them
+        const uint4 x = *reinterpret_cast<const uint4 *>(&lds.order[i]);
+        rank += (x.x < own) + (x.y < own) + (x.z < own) + (x.w < own);
+      }
     }
     shares_at[rank] = s;
   }
