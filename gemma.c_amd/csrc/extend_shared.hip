@@ -335,7 +335,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
     int32_t rank = p.heads == 1 ? 0 : k;
     if (p.heads == 1) {
       const uint32_t own = lds.order[k];
-#pragma unroll 4
+#pragma unroll 16
       for (int32_t i = 0; i < kPlanShares; i += 4) {  // 1 x 512 has all of them
         const uint4 x = *reinterpret_cast<const uint4 *>(&lds.order[i]);
         rank += (x.x < own) + (x.y < own) + (x.z < own) + (x.w < own);
@@ -446,8 +446,8 @@ hipError_t gemma4_flash_attention_extend_shared_plan(
                                            0x7fffffff - total_rows - 256);
   hipLaunchKernelGGL(common_pages_kernel, dim3(batch_size), dim3(kCommonThreads), 0, stream, p);
   // Where a thread of four waves has a sequence each and no more than a block of rows:
-  // sixteen waves' barriers and spills take 27 to 37 us on the batches of 4 to 40
-  // sequences that four plan in 17 to 27; beyond, these would go round for every 256 blocks.
+  // sixteen waves' barriers and spills take 10 us more on batches of 4 to 40 sequences
+  // (17 to 23 with four); beyond, four would go round for every 256 blocks.
   if (batch_size + group_count <= 256 && total_rows / g.rows <= 256) {
     hipLaunchKernelGGL(extend_shared_plan_kernel<256>, dim3(1), dim3(256), 0, stream, p);
   } else {
