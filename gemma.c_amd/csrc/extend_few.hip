@@ -15,12 +15,12 @@
 // teams' sums are joined at the segment's end, each team a block of columns.
 //
 // What bounds it: a step's 128 KB of K and V at 512 dims come at what a CU's path to its L2
-// carries with two waves a SIMD, 2.1 us a step (of them 0.7 of scores, 0.4 of products with
-// V, 0.7 of waiting for K); a segment's way to its first keys takes 3.6 us, by way of the
-// plan, the page table and the rows, and its end 2.2. Two waves a SIMD because one, with all
-// 512 registers, took 2.9 us a step: its phases, each on another unit, passed one after
-// the other. The loads of the next K go out between the scores' products and those of V
-// between V's: in one piece they held the waves up for 0.5 us each.
+// carries with two waves a SIMD, 2.1 us a step (of them 0.7 of scores, 0.3 of weights, 0.4 of
+// products with V, 0.6 of waiting for K and storing it); a segment's way to its first keys
+// takes 3.6 us, by way of the plan, the page table and the rows, and its end 2.2. Two waves
+// a SIMD because one, with all 512 registers, took 2.9 us a step: its phases, each on another
+// unit, passed one after the other. The loads of the next K go out between the scores'
+// products and those of V between V's: in one piece they held the waves up, 2.5 us a step.
 //
 // Keys that no row of the block sees, or that no page maps, are read from a row of zeros.
 // An infinity or NaN of V in a key that one row sees and another does not meets weight 0
@@ -406,11 +406,14 @@ __global__ __launch_bounds__(Few<kDim>::kThreads) void extend_few_kernel(ExtendP
         const int c = kBlocks == 2 ? team : 0, n = kColumns * c + h;
         const float m_own = lds.top[team][0][n], m_other = lds.top[1 - team][0][n];
         const float m = fmaxf(m_own, m_other);
-        // A team without a visible key has nothing to add, whatever its sums are.
+        // A team without a visible key has nothing to add, whatever its sums are. (Not one whose
+        // only scores are NaN: its l is.)
+        const float l_own = lds.l[team][0][n] + lds.l[team][1][n];
+        const float l_other = lds.l[1 - team][0][n] + lds.l[1 - team][1][n];
+        const bool adds_own = l_own != 0.0f, adds_other = l_other != 0.0f;
         float own = m_own == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_own - m);
         float other = m_other == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_other - m);
-        const float l = (lds.l[team][0][n] + lds.l[team][1][n]) * own +
-                        (lds.l[1 - team][0][n] + lds.l[1 - team][1][n]) * other;
+        const float l = l_own * own + l_other * other;
         if (partial < 0) {
           const float inv = l > 0.0f ? 1.0f / l : 0.0f;
           own *= inv;
@@ -428,8 +431,8 @@ __global__ __launch_bounds__(Few<kDim>::kThreads) void extend_few_kernel(ExtendP
           for (int upper = 0; upper < 2; ++upper)
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-              const float x = (m_own == -INFINITY ? 0.0f : o[i][upper][d] * own) +
-                              (m_other == -INFINITY ? 0.0f : given[i][upper][d] * other);
+              const float x = (adds_own ? o[i][upper][d] * own : 0.0f) +
+                              (adds_other ? given[i][upper][d] * other : 0.0f);
               o[i][upper][d] = x;
               zero[d] = fmaf(x, 0.0f, zero[d]);
             }
@@ -465,8 +468,8 @@ __global__ __launch_bounds__(Few<kDim>::kThreads) void extend_few_kernel(ExtendP
             }
           } else {
             // By columns, once more through LDS: 512 contiguous bytes a store, which takes
-            // half the time of 16 bytes in each of 64 places (4.2 us of a share's to 3.5);
-            // at 256 dims, of half as many, it would cost 0.5.
+            // half the time of 16 bytes in each of 64 places (2.1 us of a share's end to
+            // 1.6); at 256 dims, of half as many, it would cost 0.5 more.
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll

@@ -162,7 +162,7 @@ def test_groups(dev, heads, dim, page, groups, alone):
 
 
 # Of both kernels, by the call's rows: geometry, sequences, prefix keys, rows of a block, keys of a tile.
-SHARING = [(8, 256, 6, 1024, 16, 64), (1, 512, 24, 7168, 2, 64), (8, 256, 70, 640, 64, 32), (1, 512, 104, 2048, 8, 32)]
+SHARING = [(8, 256, 6, 1024, 16, 64), (1, 512, 25, 7168, 2, 64), (8, 256, 70, 640, 64, 32), (1, 512, 104, 2048, 8, 32)]
 
 
 @pytest.mark.parametrize("heads,dim,count,prefix,block,tile", SHARING)
@@ -316,6 +316,36 @@ def test_infinities_and_nan_of_values(dev, heads, dim):
         g.check(out)
         group = 16 // heads
         assert bool(torch.isinf(out[:sum(g.rows), 16 - group:, 11]).all())
+
+
+@pytest.mark.parametrize("heads,dim,count,prefix,block,tile", SHARING)
+def test_large_scores(dev, heads, dim, count, prefix, block, tile):
+    """Scores of hundreds, the largest ones late: the running maximum moves again and again."""
+    import torch
+    g = Groups(dev, heads, dim, [(prefix, [(1 + b % 2, 40 + b) for b in range(count)])], 16)
+    g.q.mul_(24)
+    keys = torch.arange(prefix // 16, device=dev) / (prefix // 16)
+    pages = g.table[0, :len(keys)].long()
+    g.ck[:, pages] *= (0.5 + 0.5 * keys)[None, :, None, None, None].bfloat16()
+    g.check(g.run())
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+@pytest.mark.parametrize("rows", [3, 120])
+def test_nan_of_keys_reaches_the_rows_that_see_them(dev, heads, dim, rows):
+    """A row's only key, keys of one half of a step or one of its quarters alone, one of a draft."""
+    g = Groups(dev, heads, dim, [(320, [(1, 40), (1, 30)])], 16, [(1, 0), (2, 0), (rows, 0), (1, 1), (1, 40), (4, 70)])
+    g.k[2] = NAN            # the one key of its row
+    g.k[4, heads - 1] = NAN  # the second of two
+    first = 5 + rows
+    g.ck[1, g.table[5, 0].item(), 0] = NAN
+    g.ck[1, g.table[6, 2].item(), 3:] = NAN  # keys 35 .. 39 of 41
+    g.k[first + 2 + 2] = NAN                 # of a draft's third row
+    out = g.run()
+    g.check(out)
+    assert bool(out[2].isnan().all()) and not bool(out[3].isnan().any())
+    assert bool(out[first].isnan().all()) and bool(out[first + 1].isnan().all())
+    assert not bool(out[first + 2:first + 4].isnan().any()) and bool(out[first + 4:first + 6].isnan().all())
 
 
 @pytest.mark.parametrize("heads,dim", GEOMETRIES)
