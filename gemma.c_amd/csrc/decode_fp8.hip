@@ -9,7 +9,7 @@
 // factor and the sums' end, and the loop sees codes only. A code becomes a bf16
 // operand exactly (v_cvt_scalef32_pk_bf16_fp8, two a time), so both products run on
 // v_mfma_f32_16x16x32_bf16 with nothing rounded but the weights, which go in as two
-// bf16 numbers, the nearest and the rest (2^-18 of a weight). The matrix instructions of
+// bf16 numbers, the nearest and the rest (2^-17 of a weight). The matrix instructions of
 // 8-bit operands would need no conversions, but add up their products to within 2^-12.8
 // of sum |ab| only (measured; bf16 ones 2^-22): in the exponent of a score of 40 that is
 // 0.6% of a weight.

@@ -74,7 +74,8 @@ __global__ __launch_bounds__(Few<kDim>::kThreads) void extend_few_kernel(ExtendP
   struct Lds {
     uint4 k[kStep * F::kChunks];              // key r's chunk c at c ^ (r % 16)
     uint4 q[2 * kColumns][F::kChunks];        // column n's chunk c at c ^ (n % 16)
-    uint4 weights[2][2][kWave];               // by team and block of columns: operands of P^T
+    uint4 weights[2][2][2][kWave];            // operands of P^T: by team, block of columns, the
+                                              // nearest bf16 of a weight and the rest
     uint64_t k_rows[F::kWaves][kStep];
     uint64_t v_rows[F::kWaves][kStep];
     float top[2][2][2 * kColumns];            // by team and half of its keys
@@ -315,23 +316,34 @@ __global__ __launch_bounds__(Few<kDim>::kThreads) void extend_few_kernel(ExtendP
           for (int c = 0; c < kScored; ++c) {
             const float m = kScored < kBlocks && block0 == 1 ? m_run[kBlocks - 1] : m_run[c];
             const float m_use = m == -INFINITY ? 0.0f : m;
-            // Weights in one bf16, half a step (2^-8) each, as in extend_rows.hip.
+            // A weight is the sum of two bf16, off by 2^-17 of it, as in the decode kernels whose
+            // rows may come here: one alone, off by 2^-8, left the outputs 0.0020 to 0.0023 of their
+            // norm from the 64-bit result, 0.0017 so. The second product of V costs 1 to 2%
+            // where few keys are shared, 7% of 32 tokens after 8000 shared keys at 1 x 512 (35.3
+            // to 37.9 us), 11% of 64.
             float w[4];
+            uint32_t nearest[2], rest[2];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               w[i] = __builtin_amdgcn_exp2f(x[c][i] - m_use);
               l_run[c] += w[i];
             }
-            reinterpret_cast<uint2 *>(&lds.weights[team][block0 + c][lane])[half] =
-                make_uint2(cvt_pk_bf16(w[0], w[1]), cvt_pk_bf16(w[2], w[3]));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              nearest[i] = cvt_pk_bf16(w[2 * i], w[2 * i + 1]);
+              rest[i] = cvt_pk_bf16(w[2 * i] - bf16_lo(nearest[i]), w[2 * i + 1] - bf16_hi(nearest[i]));
+            }
+            auto &to = lds.weights[team][block0 + c];
+            reinterpret_cast<uint2 *>(&to[0][lane])[half] = make_uint2(nearest[0], nearest[1]);
+            reinterpret_cast<uint2 *>(&to[1][lane])[half] = make_uint2(rest[0], rest[1]);
           }
         }
         lds_barrier();
         // ---- the wave's dims over the team's keys
-        bf16x8_t weights[kBlocks];
+        bf16x8_t nearest[kBlocks];
 #pragma unroll
         for (int c = 0; c < kBlocks; ++c)
-          weights[c] = __builtin_bit_cast(bf16x8_t, lds.weights[team][c][lane]);
+          nearest[c] = __builtin_bit_cast(bf16x8_t, lds.weights[team][c][0][lane]);
         auto word = [](const uint4 &x4, int w) __attribute__((always_inline)) -> uint32_t {
           return w == 0 ? x4.x : (w == 1 ? x4.y : (w == 2 ? x4.z : x4.w));
         };
@@ -348,13 +360,26 @@ __global__ __launch_bounds__(Few<kDim>::kThreads) void extend_few_kernel(ExtendP
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           if constexpr (kMore) load_v(2 * w, 2 * w + 2);
+          bf16x8_t rest[kBlocks];  // read for every pair of dims: held all along they would be spilled
+          uint32_t from = lane;
+          asm volatile("" : "+v"(from));
+#pragma unroll
+          for (int c = 0; c < kBlocks; ++c)
+            rest[c] = __builtin_bit_cast(bf16x8_t, lds.weights[team][c][1][from]);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int c = 0; c < kBlocks; ++c) {
             acc[c][2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, low[w]), weights[c], acc[c][2 * w], 0, 0, 0);
+                __builtin_bit_cast(bf16x8_t, low[w]), nearest[c], acc[c][2 * w], 0, 0, 0);
             acc[c][2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, high[w]), weights[c], acc[c][2 * w + 1], 0, 0, 0);
+                __builtin_bit_cast(bf16x8_t, high[w]), nearest[c], acc[c][2 * w + 1], 0, 0, 0);
+          }
+#pragma unroll
+          for (int c = 0; c < kBlocks; ++c) {
+            acc[c][2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8_t, low[w]), rest[c], acc[c][2 * w], 0, 0, 0);
+            acc[c][2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8_t, high[w]), rest[c], acc[c][2 * w + 1], 0, 0, 0);
           }
         }
         if constexpr (kMore) {
