@@ -975,8 +975,11 @@ hipError_t gemma4_decode_split_plan_fp8(Gemma4KvCacheConfig config, int32_t batc
     if (heads != 1) size = std::min<int64_t>(size, whole(std::max<int64_t>(2048, even / 2), kFp8Step));
   } else if (batch_count <= kBalancedBatch) {
     // The lengths make the cut; here the most splits that it can come to, the longest
-    // sequence being about all there is.
-    size = whole(std::min<int64_t>(keys * heads / kFp8Cus, kFp8Long), kFp8Step);
+    // sequence being about all there is: of kFp8Long keys, and no more than kFp8Cus, where the
+    // cut's grow too (Fp8Cut). Partial sums are as many as these.
+    size = whole(std::max<int64_t>(std::min<int64_t>(keys * heads / kFp8Cus, kFp8Long),
+                                   (keys + kFp8Cus - 1) / kFp8Cus),
+                 kFp8Step);
   } else {
     size = whole(keys * heads * batch_count / 2048, kFp8Step);
   }

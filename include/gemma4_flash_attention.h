@@ -404,7 +404,9 @@ hipError_t gemma4_flash_attention_append_decode_paged_fp8(
     Gemma4KvCacheConfig config, int32_t layer, float softmax_scale, int32_t split_size,
     int32_t num_splits, int32_t batch_count, hipStream_t stream);
 
-// gemma4_decode_split_plan for the two calls above.
+// gemma4_decode_split_plan for the two calls above. For up to 64 sequences (and
+// target_workgroups 0) num_splits is at most 256, however many keys there are. The partial
+// buffers hold batch_count * 16 * num_splits rows of 1, 1 and head_dim floats.
 hipError_t gemma4_decode_split_plan_fp8(Gemma4KvCacheConfig config, int32_t batch_count,
                                         int32_t max_live_keys, int32_t target_workgroups,
                                         int32_t *split_size, int32_t *num_splits);

@@ -72,3 +72,9 @@ def test_cuts_that_grow(dev, heads, dim, keys):
 def test_one_long_among_empty(dev, heads, dim):
     c = Cache(dev, heads, dim, [0] * 31 + [9000] + [0] * 31 + [1], page=64, layers=1)
     c.check(c.decode(layer=0), layer=0)
+
+
+def test_longer_than_256_splits_of_512(dev):
+    c = Cache(dev, 1, 512, [140_001, 300], page=64, layers=1)
+    assert c.plan() == (640, 219)
+    c.check(c.decode(layer=0), layer=0)
