@@ -169,3 +169,26 @@ def test_all_rows_in_parts(dev, heads, dim):
     g.check_some(out, range(0, g.total, 7), layer=0)
     g.check_plan()
     assert g.shared_tiles(0) == 100
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+@pytest.mark.parametrize("count", [1, 40])
+def test_few_rows_in_large_blocks(dev, heads, dim, count):
+    """A stated total_rows beyond the few rows' limit, with rows that no sequence holds, takes the larger
+    blocks; those rows need not be there."""
+    import torch
+    limit = 96 if heads == 1 else 64
+    # (A chunk alone, or single tokens behind a prefix.)
+    groups, alone = ([], [(40, 9000)]) if count == 1 else ([(6400, [(1, b % 30) for b in range(count)])], [])
+    g = Guarded(dev, heads, dim, groups, 64, alone, layers=1, extra_rows=limit + 1 - 40)
+    few, rows = 40, slice(0, 40)
+    assert g.total == limit + 1
+    g.q, g.k, g.v = (x[rows].contiguous() for x in (g.q, g.k, g.v))
+    g.make_plan()
+    out = torch.full((few + 1, 16, dim), 7.0, dtype=torch.bfloat16, device=dev)
+    g.attend(out, layer=0)
+    torch.cuda.synchronize()
+    g.check_some(out, range(0, few, 3), layer=0)
+    assert bool((out[few:] == 7.0).all())
+    g.check_plan()
+    assert max(s[1] for s in g.blocks()) == (8 if heads == 1 else 40)
