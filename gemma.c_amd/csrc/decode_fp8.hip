@@ -232,7 +232,7 @@ struct Fp8Split {
   }
 };
 
-// ---- 8 x 256 ------------------------------------------------------------------------
+// ---- 8 x 256, and 1 x 512 in longer splits ---------------------------------------------
 template <int kDim, int kWaves>
 __global__ __launch_bounds__(kWaves *kWave, kDim == 256 ? 2 : 1) void decode_fp8_kernel(
     Fp8DecodeParams p) {
@@ -814,7 +814,7 @@ __global__ __launch_bounds__(256, 2) void decode_fp8_short_kernel(Fp8DecodeParam
                                                                 acc[6][i] * v_scale, acc[7][i] * v_scale);
     }
     if (wave == 0 && g == 0) {
-      // A NaN has made every sum NaN, and has to reach the output: see the 8 x 256 kernel.
+      // A NaN has made every sum NaN, and has to reach the output: see above.
       p.partial_m[slot] = odd && top == -INFINITY ? 0.0f : top * kLn2;
       p.partial_l[slot] = odd ? 1.0f : l_all;
     }

@@ -95,7 +95,7 @@ inline ExtendPlanLayout extend_layout(const ExtendGeometry &g, int32_t batch, in
 }
 // The plan of a batch in groups: besides these, for every row of a sequence whose
 // prefix is attended with its group its own block (ExtendMerge, index: the row
-// within it; parts 0 elsewhere), and the leading pages a sequence has in common with
+// within it; other rows' are neither written nor read), and the leading pages a sequence has in common with
 // the one before it. All of such a row's parts are partial sums, at least one of the
 // prefix and one behind it.
 struct ExtendSharedLayout {

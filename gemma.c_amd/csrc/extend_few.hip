@@ -14,9 +14,9 @@
 // keys that an operand holds of two dims. K is read in whole rows and turned in LDS. The two
 // teams' sums are joined at the segment's end, each team a block of columns.
 //
-// What bounds it: a step's 128 KB of K and V at 512 dims come out of the L2s at 15.6 TB/s
-// in all, 2.1 us a step (of them 0.7 of scores, 0.3 of weights, 0.4 of
-// products with V, 0.6 of waiting for K and storing it); a segment's way to its first keys
+// What bounds it: a step's 128 KB of K and V at 512 dims come out of the L2s at 14 TB/s
+// in all, 2.4 us a step (0.7 of scores, 0.3 of weights, 0.7 of products with V, 0.3 of them
+// of the weights' second halves, 0.6 of waiting for K and storing it); a segment's way to its first keys
 // takes 3.6 us, by way of the plan, the page table and the rows, and its end 2.2. Two waves
 // a SIMD because one, with all 512 registers, took 2.9 us a step: its phases, each on another
 // unit, passed one after the other. The loads of the next K go out between the scores'

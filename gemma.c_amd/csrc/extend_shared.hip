@@ -353,11 +353,16 @@ __global__ __launch_bounds__(kPlanThreads) void extend_shared_plan_kernel(Shared
 bool shared_sizes_ok(const Gemma4KvCacheConfig &c, int32_t batch, int32_t total_rows) {
   return extend_sizes_ok(c, batch, total_rows) && c.window_size == 0;
 }
-// Rows of a call up to which they go to extend_few.hip's kernel. Both kernels on one group
-// of 32 (us, few against large blocks): rows 32 and 64 after 4096 shared keys 30 and 38
-// against 40 and 47 at 1 x 512, 30 and 35 against 31 and 33 at 8 x 256; after 500, 16 and 22
-// against 28 and 30, 18 and 19 against 19 and 22. At 128 rows after 4096 keys it is 63
-// against 54, and 49 against 38: each of many blocks reads the prefix.
+// Rows of a call up to which they go to extend_few.hip's kernel. Each of its small blocks reads
+// all keys, so it depends on the keys as well, which only the device knows. Both kernels
+// (us, few against large blocks) on tokens after 500, 4096, 16384 and 65536 shared keys, at
+// 1 x 512 16 of them 13.4 : 17.5, 26.8 : 37.7, 38 : 43, 99 : 68, 64 of them 18.1 : 23.2,
+// 40.4 : 46.0, 100 : 69, 402 : 168; at 8 x 256 14.8 : 14.5, 22.5 : 22.1, 35 : 37, 107 : 119 and
+// 26.1 : 25.0, 43.8 : 32.7, 91 : 50, 307 : 132. A chunk of 64 rows after 4096, 16384 and
+// 65536 keys of its own: 35.5 : 44.9, 91 : 71, 337 : 175, and 30.0 : 30.1, 74 : 44, 269 : 118.
+// That is a line at about 400 000 rows x keys at 1 x 512, and at 8 x 256, beyond one block of
+// 16 rows, at 200 000. A caller beyond it states more rows than there are (see the
+// header).
 constexpr int32_t kFewRows512 = 96, kFewRows256 = 64;
 bool few_rows(const Gemma4KvCacheConfig &c, int32_t total_rows) {
   return total_rows <= (c.num_heads == 1 ? kFewRows512 : kFewRows256);

@@ -218,8 +218,8 @@ hipError_t gemma4_rope_frequencies(double *turns, float *amplitude, int32_t rota
 // rows: q and k get the learned RMSNorm of d_q_norm_weight / d_k_norm_weight [head_dim]
 // (null: none) and the rotation of their first rotary_dim dims, a multiple of 16, in
 // pairs (i, i + rotary_dim / 2) or, interleaved != 0, (2 i, 2 i + 1), by
-// position * d_turns[i] turns (d_turns [rotary_dim / 2] on the device, of any finite
-// values) and times `amplitude`; v gets scale-free RMSNorm, eps 1e-6. d_v null with d_v_out: v
+// position * d_turns[i] turns (d_turns [rotary_dim / 2] on the device; the products, in 64
+// bits, are finite) and times `amplitude`; v gets scale-free RMSNorm, eps 1e-6. d_v null with d_v_out: v
 // from the raw k, as in the reference's global layers; both null: no v. q [rows][16][head_dim], rows
 // q_stride elements apart, k and v [rows][num_heads][head_dim], rows kv_stride apart
 // (multiples of 8 up to 2^30; 0: packed). The outputs are packed and overlap no input.
@@ -302,15 +302,28 @@ hipError_t gemma4_flash_attention_extend_paged_bf16(
 // scored once for all its rows. Sequences d_group_offsets[i] .. d_group_offsets[i + 1]
 // are group i (d_group_offsets [group_count + 1], ascending, at most batch_size; those
 // past the last are in none); how far its tables agree the plan finds out itself, and it shares the
-// whole tiles (of 32 or 64 keys) that all of the group have in the cache, where that saves time:
-// groups that share nothing cost as much as without. A group's sequences that bring no
-// rows limit what it shares as the others do. group_count is at most 2048. Full-length
+// whole tiles (of 32 or 64 keys) that all of the group have in the cache, where that saves time.
+// A group's sequences that bring no rows limit what it shares as the others do. group_count is at most 2048. Full-length
 // caches, no window; rows, offsets, lengths, geometries, limits and results as above (the
 // sums' order differs, so results may by their last bit).
 // No counterpart in the reference.
 //
 // A plan of one kind is refused by the other kind's attention, which then writes nothing.
 // The plan holds for the page table it was made of, too.
+//
+// What it costs where nothing is shared: the plan compares tables in a launch of its own and
+// takes 5 to 8 us longer (13 to 25 us, 46 for one row after 8192 keys), and the workspace
+// has room for two sums of every row, 32 * head_dim * 4 bytes a row and up to twice that
+// where blocks are not full (8192 rows of 64 sequences 435 MB at 8 x 256 and 745 at 1 x 512,
+// the extension above 66 and 134): chunks of prompts that share nothing are for that.
+// Single tokens of few sequences are faster through the decode entry points: with 2000 keys
+// shared, this call is from 16 sequences on at 1 x 512 (20 us, 22 there) and from 4 at
+// 8 x 256 (13, 17).
+// Calls of up to 96 rows at 1 x 512 and 64 at 8 x 256 are laid out in blocks of a few, which
+// is faster while rows times keys stay below about 400 000 and 200 000 (64 rows after 4096
+// keys of their own at 1 x 512 36 us, 44 by the extension above; after 65536 337 and 174).
+// A caller with longer contexts states a total_rows above the limit, 97 or 65: rows behind
+// the last offset are not touched, nor need they be there.
 size_t gemma4_flash_attention_extend_shared_plan_bytes(Gemma4KvCacheConfig config,
                                                        int32_t batch_size, int32_t total_rows);
 size_t gemma4_flash_attention_extend_shared_workspace_bytes(Gemma4KvCacheConfig config,

@@ -133,15 +133,15 @@ hipError_t gemma4_kv_cache_write_prefill_bf16(
 // [num_layers][num_heads], fixed while a cache is in use (null: 1; positive and
 // finite). The codes are floating-point numbers of four significant bits from 2^-6 to 448
 // and in steps of 2^-9 below, so a scale only has to keep what occurs within that range:
-// prepared rows are RMS-normed, |x| <= sqrt(head_dim) * max |weight|, and that bound / 448
-// never saturates. No counterparts in the reference.
+// prepared rows are RMS-normed, |x| <= sqrt(head_dim) * max |weight| (times the rotation's
+// amplitude for K), and that bound / 448 never saturates. No counterparts in the reference.
 // The page pool serves such a cache as it is, its rows are half as long: reserve, release,
 // gemma4_kv_cache_fork_bf16 and gemma4_kv_cache_compact_bf16 with head_dim / 2 in the
 // config and the codes as bf16.
 //
 // Writes prepared rows as gemma4_kv_cache_write_bf16 does (the same tokens are skipped,
-// the same rows of a lap stay): code = x / scale to the nearest code, ties to even,
-// beyond +-448 to that; NaN stays NaN. k and v rows are kv_stride elements apart
+// the same rows of a lap stay): code = x / scale, the quotient
+// rounded to 32 bits, to the nearest code, ties to even, beyond +-448 to that; NaN stays NaN. k and v rows are kv_stride elements apart
 // (a multiple of 8 up to 2^30; 0: packed). head_dim is a multiple of 16; caches, k
 // and v are 16-byte aligned; token_count * num_heads * head_dim / 16 < 2^32 - 256.
 hipError_t gemma4_kv_cache_write_fp8(uint8_t *d_cache_k, uint8_t *d_cache_v,
@@ -153,7 +153,7 @@ hipError_t gemma4_kv_cache_write_fp8(uint8_t *d_cache_k, uint8_t *d_cache_v,
                                      hipStream_t stream);
 
 // Reads rows back: row i of k and v gets the values of (d_token_batch[i],
-// d_token_position[i]), rounded to bf16 once; a row whose token the write would skip is
+// d_token_position[i]), the products in 32 bits rounded to bf16; a row whose token the write would skip is
 // left as it was. Over a ring a position names its slot, whichever lap it holds. Packed
 // rows are a bf16 cache of their own (page tables that count up), over which a prompt's
 // chunk attends. Limits as above.
