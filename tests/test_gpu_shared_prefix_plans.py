@@ -192,3 +192,28 @@ def test_few_rows_in_large_blocks(dev, heads, dim, count):
     assert bool((out[few:] == 7.0).all())
     g.check_plan()
     assert max(s[1] for s in g.blocks()) == (8 if heads == 1 else 40)
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+def test_the_most_sequences_and_groups(dev, heads, dim):
+    """4096 sequences in 2048 groups, some of none."""
+    groups = [(64 + 16 * (g % 3), [(1, g % 4), (g % 2, 5)]) if g % 8 else (32, []) for g in range(2048)]
+    alone = [(1, b % 6) for b in range(4096 - sum(len(m) for _, m in groups))]
+    g = Guarded(dev, heads, dim, groups, 16, alone, layers=1)
+    assert g.batch == 4096 and g.group_count == 2048
+    out = g.run(layer=0)
+    g.check_some(out, range(0, g.total, 23), layer=0)
+    covered = g.check_plan()
+    assert (covered >= np.concatenate([p + 1 + np.arange(n) for p, n in zip(g.prior, g.rows)])).all()
+
+
+@pytest.mark.parametrize("heads,dim", GEOMETRIES)
+@pytest.mark.parametrize("page", [1, 7, 100, 1024])
+@pytest.mark.parametrize("count", [12, 110])
+def test_page_sizes(dev, heads, dim, page, count):
+    """Pages of one key, of sizes that no tile divides, longer than many tiles; in both kernels."""
+    prefix = 2048 // page * page
+    g = Guarded(dev, heads, dim, [(prefix, [(1 + (b % 4 == 0), b % 37) for b in range(count)])], page, [(3, 0), (1, 90)], layers=1)
+    out = g.run(layer=0)
+    g.check_some(out, range(0, g.total, 1 + count // 40), layer=0)
+    assert all(bool((b == 0xA5).all()) for b in g.behind)
